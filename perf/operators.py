@@ -5,7 +5,7 @@ normalisation with an activation on channels-last maps, and the clipping of grad
 
     vit_amd.diff_attention(q, k, v, lam, lambda_init, key_lens=None, causal=False)
     vit_amd.group_norm(x, num_groups, weight, bias, eps, activation)
-    vit_amd.clip_grad_norm_(tensors, max_norm)
+    vit_amd.clip_grad_norm_(parameters, max_norm)
 """
 import math
 
@@ -160,7 +160,9 @@ def prepare(case, seed):
                     state["buffers"].append(flat)
                     grads += list(flat.split(part))                              # odd offsets, as in a bucket
         norm = 1e-2 * math.sqrt(sum(sizes))
-        state["grads"] = grads
+        state["params"] = [g.detach() for g in grads]                            # only their .grad is looked at
+        for p, g in zip(state["params"], grads):
+            p.grad = g
         state["max_norm"] = 0.37 * norm if case["clips"] else 4.0 * norm
         state["tighten"] = 1.0 - 2.0 ** -11 if case["clips"] else 1.0
     return state
@@ -255,7 +257,7 @@ def run(state):
                      lambda x, w, b: vit_amd.group_norm(x, s["groups"], w, b, 1e-5, s["act"]))
     # the bound tightens a little from step to step, so that a pass clips what the pass before it has clipped
     if own:
-        norm, buffers = vit_amd.clip_grad_norm_(s["grads"], s["max_norm"]), s["buffers"]
+        norm, buffers = vit_amd.clip_grad_norm_(s["params"], s["max_norm"]), s["buffers"]
     else:
         norm, buffers = _plain_clip(s)
     s["max_norm"] *= s["tighten"]
