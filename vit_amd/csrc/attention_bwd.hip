@@ -140,7 +140,7 @@ __device__ __forceinline__ void attn_bwd_owner_block(const char* r1, const char*
                     }
                 }
             // element i of a lane: resident row rb*32 + 8 (i >> 2) + 4 hh + (i & 3), owner row = the lane's.
-            // Two elements per instruction (packed f32): p = exp2(s c - L), dS = p (dP - D); the factor `scale` of
+            // Two elements side by side: p = exp2(s c - L), dS = p (dP - D); the factor `scale` of
             // dQ and dK is applied once to the finished sums.
             f32x16 pr;
 #pragma unroll

@@ -144,7 +144,7 @@ __device__ __forceinline__ void epilogue_tile(const GemmArgs& p, const f32x4 (&a
                     const f32x4 a = acc[nt][pass * 2 + m2];
                     float v0, v1, v2, v3;
                     if constexpr (LNIN) {
-                        // on packed f32 arithmetic (v_pk_fma_f32): two instructions per pair of values
+                        // two multiply-adds per value
                         const f32x2 ra = {ab8[pass * 2 + m2][0], ab8[pass * 2 + m2][0]};
                         const f32x2 rb = {ab8[pass * 2 + m2][1], ab8[pass * 2 + m2][1]};
                         const f32x2 lo = f32x2{a[0], a[1]} * ra + (rb * f32x2{s4[nt][0], s4[nt][1]} + f32x2{b4[nt][0], b4[nt][1]});
@@ -307,7 +307,7 @@ __device__ __forceinline__ void epilogue_tile(const GemmArgs& p, const f32x4 (&a
                     if constexpr (LNOUT) {
                         // the new row's bf16 copy (the next GEMM's operand) and this strip's share of its LayerNorm
                         // statistics: 16 lanes hold the row's 64 columns of this wave
-                        const f32x2 vlo = {v[0], v[1]}, vhi = {v[2], v[3]};      // packed f32: 5 instructions for both sums
+                        const f32x2 vlo = {v[0], v[1]}, vhi = {v[2], v[3]};      // two values side by side
                         const f32x2 s2 = vlo + vhi, q2 = vhi * vhi + vlo * vlo;
                         const float ps = row16_sum(s2[0] + s2[1]);
                         const float pq = row16_sum(q2[0] + q2[1]);

@@ -66,15 +66,14 @@ __device__ __forceinline__ float dgelu_erf(float x) {
     return fmaf(x * e, 0.39894228040143267794f, cdf);
 }
 
-// The same function on packed f32 arithmetic (v_pk_mul_f32 / v_pk_fma_f32: twice the throughput of scalar
-// VALU code, and no transcendental) for the fused GEMM epilogue, where GELU of 128 accumulators per lane is
-// what the epilogue's time goes to.
+// The same function without a transcendental, four values at a time, for the fused GEMM epilogue, where GELU of 128
+// accumulators per lane is what the epilogue's time goes to.
 //   gelu(x) = x Phi(x),  Phi(u) - 1/2 = u P(u^2) for u = clamp(x, -4, 4)
 // P is a degree-6 minimax polynomial (weighted for the error of x Phi) with u P(u^2) pinned to 1/2 at u = 4,
 // so that gelu(x) = x (or 0) exactly beyond the clamp, where the true value differs from that by at most
 // 4 Phi(-4) = 1.3e-4.  |error of gelu| <= 1.9e-4 over all x in f32 arithmetic: below half a bf16 ulp of any
 // result larger than 0.1 in size.
-// Two pairs run in lockstep: dependent v_pk_fma_f32 need a wait state between them, which the second chain fills.
+// Four chains run in lockstep, so that no multiply-add waits for the one before it.
 __device__ __forceinline__ void gelu_erf_x4(f32x2& a, f32x2& b) {
     const f32x2 ua = {__builtin_amdgcn_fmed3f(a[0], -4.0f, 4.0f), __builtin_amdgcn_fmed3f(a[1], -4.0f, 4.0f)};
     const f32x2 ub = {__builtin_amdgcn_fmed3f(b[0], -4.0f, 4.0f), __builtin_amdgcn_fmed3f(b[1], -4.0f, 4.0f)};
@@ -91,7 +90,7 @@ __device__ __forceinline__ void gelu_erf_x4(f32x2& a, f32x2& b) {
     b = b * pb;
 }
 
-// d/dx gelu(x) = Phi(x) + x phi(x) for two values on packed arithmetic, with Phi from the polynomial of
+// d/dx gelu(x) = Phi(x) + x phi(x) for two values, with Phi from the polynomial of
 // gelu_erf_x4 (|error| <= 3.3e-4 absolute: below a bf16 ulp of the gradients it scales wherever the derivative
 // exceeds 0.1) and phi(x) = exp2(-x^2 log2(e) / 2) / sqrt(2 pi).  The GEMM epilogue of the training step's
 // GELU backward evaluates 128 of these per lane.
