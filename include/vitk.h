@@ -322,6 +322,55 @@ int vitk_gemm_ln_bias_gelu(const void* A, const void* Wg, const float* ab, const
 int vitk_qkv_proj_ln(const void* A, const void* Wg, const float* ab, const float* colsum, const float* c, void* qkv,
                      int batch, int ntok, int heads, int hd, void* stream);
 
+/* ---- group normalisation with an activation, channels last ---------------------------------------------
+ * y = act((x - mean_g) rstd_g * weight[c] + bias[c]) on x [batch, pixels, channels] (a channels-last feature map, or
+ * tokens), statistics per sample over all pixels of channels / groups neighbouring channels, biased variance, eps inside
+ * the root: nn.GroupNorm and the activation behind it, for the convolutional stems whose norm layer the reference leaves
+ * to the caller (models/resnet.py). */
+
+#define VITK_ACT_NONE 0
+#define VITK_ACT_RELU 1
+#define VITK_ACT_GELU_ERF 2  /* exact erf, as nn.GELU() */
+#define VITK_ACT_SILU 3
+
+/* f32 values of scratch for vitk_group_norm (backward = 0) or vitk_group_norm_backward; -1 for sizes it does not take. */
+int64_t vitk_group_norm_workspace(int batch, int pixels, int channels, int groups, int dtype, int backward);
+
+/* x, y: bf16 or f32 (dtype) [batch, pixels, channels], contiguous, any alignment that the type has, distinct buffers.
+ * weight, bias: f32 [channels], either may be NULL (1, 0).  mean, rstd: f32 [batch, groups] for the backward, or both NULL. */
+int vitk_group_norm(const void* x, const float* weight, const float* bias, void* y, float* mean, float* rstd,
+                    float* workspace, int64_t workspace_floats, int batch, int pixels, int channels, int groups, float eps,
+                    int act, int dtype, void* stream);
+
+/* dx (x's type), dweight, dbias (f32 [channels], each may be NULL) from the output gradient dy and the
+ * forward's mean and rstd.  Sums in f32, in a fixed order: results are reproducible. */
+int vitk_group_norm_backward(const void* x, const float* weight, const float* bias, const void* dy, const float* mean,
+                             const float* rstd, void* dx, float* dweight, float* dbias, float* workspace,
+                             int64_t workspace_floats, int batch, int pixels, int channels, int groups, int act, int dtype,
+                             void* stream);
+
+/* ---- global gradient norm and clipping -----------------------------------------------------------------
+ * clip_grad_norm_ of the training step (main.py:221-223) over a list of n device tensors of any sizes: addr, size
+ * (elements, 0 allowed) and dtype (VITK_F32 / VITK_BF16) are HOST arrays, read before the call returns.  Tensors are dense
+ * and aligned to their type. */
+
+#define VITK_NORM_2 0        /* sqrt of the sum of squares, added in f64 */
+#define VITK_NORM_INF 1      /* largest magnitude */
+
+/* f64 values that `partials` has to hold for a list of n tensors. */
+int64_t vitk_grad_norm_workspace(int n);
+
+/* Leaves the list's partial sums in partials and, if norm is not NULL, the norm in *norm (f32, on the device).  A NaN
+ * anywhere gives NaN. */
+int vitk_grad_norm(const uint64_t* addr, const int64_t* size, const int* dtype, int n, int norm_kind, double* partials,
+                   int64_t n_partials, float* norm, void* stream);
+
+/* g *= min(1, max_norm / (norm + 1e-6)) in place for every tensor of the list, from the partial sums that vitk_grad_norm
+ * left for the same list on the same stream; writes the norm before clipping to *norm if that is not NULL and the list
+ * holds a value.  Gradients under the bound are not touched.  Tensors that share memory: VITK_ERR_INVALID. */
+int vitk_grad_clip(const uint64_t* addr, const int64_t* size, const int* dtype, int n, int norm_kind, const double* partials,
+                   int64_t n_partials, double max_norm, float* norm, void* stream);
+
 /* ---- for callers that cannot allocate ------------------------------------------------------------- */
 
 /* Optional set-up for the current device: resolves the library's built-in scratch (used by

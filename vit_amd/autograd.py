@@ -15,6 +15,7 @@ cd = compute dtype of the GEMM operands: torch.bfloat16, or torch.float32 in the
 """
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from . import ops
 from .lib import ACT_GELU, ACT_TANH, EPI_BIAS, EPI_GELU, EPI_RESIDUAL, EPI_TANH, VitkError
@@ -300,6 +301,27 @@ class AttentionFn(torch.autograd.Function):
         for i in range(3):
             dqkv[i].copy_(grads[i])
         return dqkv, None
+
+
+class GroupNormFn(torch.autograd.Function):
+    """act(GroupNorm(x)) on x [batch, ..., channels]; the backward recomputes the normalised values from x and the saved
+    mean and rstd."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, num_groups, eps, activation):
+        y, mean, rstd = ops.group_norm(x, num_groups, weight, bias, eps, activation, stats=True)
+        ctx.save_for_backward(x, weight, bias, mean, rstd)
+        ctx.num_groups, ctx.activation = num_groups, activation
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        x, weight, bias, mean, rstd = ctx.saved_tensors
+        want_w, want_b = weight is not None and ctx.needs_input_grad[1], bias is not None and ctx.needs_input_grad[2]
+        dx, dw, db = ops.group_norm_backward(x, ctx.num_groups, weight, bias, g.contiguous(), mean, rstd, ctx.activation,
+                                             param_grads=want_w or want_b)
+        return dx, dw.view(weight.shape) if want_w else None, db.view(bias.shape) if want_b else None, None, None, None
 
 
 class PatchEmbedFn(torch.autograd.Function):

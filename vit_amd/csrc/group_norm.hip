@@ -1,0 +1,613 @@
+// Group normalisation with an activation behind it, on channels-last maps (gfx950 / CDNA4): forward and backward.
+//
+// x [batch, pixels, channels], group g of a sample = channels g*Cg .. g*Cg + Cg - 1 of all its pixels:
+//     h = (x - mean_g) rstd_g,   z = h w[c] + b[c],   y = act(z)
+// Backward, with dz = dy act'(z) and n = pixels * Cg:
+//     dx = rstd_g (dz w - m1_g - h m2_g),  m1 = sum_g(dz w) / n,  m2 = sum_g(dz w h) / n
+//     dw[c] = sum dz h,  db[c] = sum dz   over samples and pixels
+//
+// Bound by HBM (forward: x read, y written; backward: x and dy read, dx written).  A lane owns V channels (16 bytes where
+// the channel count and the pointers allow it, else one value) and walks down the pixels, so that a wave reads whole
+// runs of a pixel's channels; statistics are kept per channel and put together into groups only at the end of a
+// workgroup, which leaves the group width free (any divisor of the channels).
+//
+// Statistics are first and second moments about the lane's first value, merged pairwise by
+//     M2 = M2a + M2b + (mean_b - mean_a)^2 na nb / (na + nb),
+// all in f32: no cancellation where the mean is large against the deviation, as sums of squares would have.
+#include "vitk_common.h"
+#include "vitk_kernels.h"
+
+namespace vitk {
+
+namespace {
+
+constexpr int kT = 256;                 // threads of the two-pass kernels
+
+struct Mom {
+    float n, mean, m2;
+};
+
+__device__ __forceinline__ Mom merge(const Mom& a, const Mom& b) {
+    if (b.n == 0.f) return a;
+    if (a.n == 0.f) return b;
+    const float n = a.n + b.n;
+    const float f = b.n / n, d = b.mean - a.mean;
+    return Mom{n, fmaf(d, f, a.mean), a.m2 + b.m2 + d * d * a.n * f};
+}
+
+__device__ __forceinline__ Mom wave_merge(Mom m) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        // both partners merge in the same order, so that all lanes end with the same bits
+        const Mom p = {__shfl_xor(m.n, o, 64), __shfl_xor(m.mean, o, 64), __shfl_xor(m.m2, o, 64)};
+        const bool low = (threadIdx.x & o) == 0;
+        m = low ? merge(m, p) : merge(p, m);
+    }
+    return m;
+}
+
+// V values of T: raw registers and their f32 values
+template <class T, int V>
+struct Raw;
+template <>
+struct Raw<bf16_t, 8> {
+    u32x4 r;
+    __device__ __forceinline__ void load(const bf16_t* p) { r = *reinterpret_cast<const u32x4*>(p); }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            v[2 * j] = bf16_lo(r[j]);
+            v[2 * j + 1] = bf16_hi(r[j]);
+        }
+    }
+    __device__ __forceinline__ static void store(bf16_t* p, const float (&v)[8]) {
+        *reinterpret_cast<u32x4*>(p) = u32x4{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])};
+    }
+};
+template <>
+struct Raw<bf16_t, 1> {
+    uint16_t r;
+    __device__ __forceinline__ void load(const bf16_t* p) { r = *reinterpret_cast<const uint16_t*>(p); }
+    __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = __builtin_bit_cast(float, (uint32_t)r << 16); }
+    __device__ __forceinline__ static void store(bf16_t* p, const float (&v)[1]) {
+        *reinterpret_cast<uint16_t*>(p) = (uint16_t)pack_bf16(v[0], 0.f);
+    }
+};
+template <>
+struct Raw<float, 4> {
+    f32x4 r;
+    __device__ __forceinline__ void load(const float* p) { r = *reinterpret_cast<const f32x4*>(p); }
+    __device__ __forceinline__ void get(float (&v)[4]) const {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = r[j];
+    }
+    __device__ __forceinline__ static void store(float* p, const float (&v)[4]) {
+        *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
+    }
+};
+template <>
+struct Raw<float, 1> {
+    float r;
+    __device__ __forceinline__ void load(const float* p) { r = *p; }
+    __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = r; }
+    __device__ __forceinline__ static void store(float* p, const float (&v)[1]) { *p = v[0]; }
+};
+
+__device__ __forceinline__ float sigmoid(float z) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896340736f));
+}
+
+template <int ACT>
+__device__ __forceinline__ float act_of(float z) {
+    if constexpr (ACT == GN_RELU) return z > 0.f ? z : (z == z ? 0.f : z);      // a NaN stays one
+    if constexpr (ACT == GN_GELU) return gelu_erf(z);
+    if constexpr (ACT == GN_SILU) return z * sigmoid(z);
+    return z;
+}
+
+template <int ACT>
+__device__ __forceinline__ float dact_of(float z) {
+    if constexpr (ACT == GN_RELU) return z > 0.f ? 1.f : 0.f;
+    if constexpr (ACT == GN_GELU) return dgelu_erf(z);
+    if constexpr (ACT == GN_SILU) {
+        const float s = sigmoid(z);
+        return s * fmaf(z, 1.0f - s, 1.0f);
+    }
+    return 1.f;
+}
+
+struct Geometry {
+    int S, C, G, Cg;          // pixels, channels, groups, channels of a group
+    int cv;                   // lanes side by side in a slab = slab channels / V
+    int slabs;                // slabs of cv * V channels (the last one may be short)
+    int chunk;                // pixels of a workgroup
+    int chunks;
+};
+
+// ---- forward, two passes over x ------------------------------------------------------------------------------
+
+// Moments of every group over one chunk of pixels and one slab of channels:
+// part[((b * chunks + chunk) * slabs + slab) * G + g] for the groups that the slab touches.
+template <class T, int V>
+__global__ __launch_bounds__(kT) void gn_moments(const T* __restrict__ x, Mom* __restrict__ part, Geometry q) {
+    __shared__ float s_mean[kT * V], s_m2[kT * V];
+    const int tid = threadIdx.x;
+    const int rows = kT / q.cv;
+    const int row = tid / q.cv, col = tid - row * q.cv;
+    const int slab = blockIdx.y, b = blockIdx.z;
+    const int c0 = slab * q.cv * V;
+    const int wc = min(q.cv * V, q.C - c0);             // channels of this slab
+    const int s0 = blockIdx.x * q.chunk, s1 = min(s0 + q.chunk, q.S);
+    if (row < rows && col * V < wc) {
+        float x0[V], a1[V], a2[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) x0[j] = a1[j] = a2[j] = 0.f;
+        const T* p = x + ((int64_t)b * q.S) * q.C + c0 + col * V;
+        int s = s0 + row;
+        float n = 0.f;
+        if (s < s1) {
+            Raw<T, V> r;
+            r.load(p + (int64_t)s * q.C);
+            r.get(x0);
+            n = 1.f;
+            s += rows;
+        }
+        auto add = [&](const Raw<T, V>& r) {
+            float v[V];
+            r.get(v);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float d = v[j] - x0[j];
+                a1[j] += d;
+                a2[j] = fmaf(d, d, a2[j]);
+            }
+        };
+        constexpr int U = 8;
+        for (; s + (U - 1) * rows < s1; s += U * rows) {
+            Raw<T, V> r[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) r[u].load(p + (int64_t)(s + u * rows) * q.C);
+#pragma unroll
+            for (int u = 0; u < U; ++u) add(r[u]);
+            n += U;
+        }
+        for (; s < s1; s += rows) {
+            Raw<T, V> r;
+            r.load(p + (int64_t)s * q.C);
+            add(r);
+            n += 1.f;
+        }
+        const float inv = n > 0.f ? 1.0f / n : 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            s_mean[row * wc + col * V + j] = fmaf(a1[j], inv, x0[j]);
+            s_m2[row * wc + col * V + j] = fmaxf(fmaf(-a1[j] * inv, a1[j], a2[j]), a2[j] == a2[j] ? 0.f : a2[j]);
+        }
+    }
+    __syncthreads();
+    const int g0 = c0 / q.Cg, g1 = (c0 + wc - 1) / q.Cg;
+    const int lane = tid & 63;
+    Mom* out = part + (((int64_t)b * q.chunks + blockIdx.x) * q.slabs + slab) * q.G;
+    for (int g = g0 + (tid >> 6); g <= g1; g += kT / 64) {
+        const int lo = max(g * q.Cg - c0, 0), hi = min((g + 1) * q.Cg - c0, wc);
+        const int w = hi - lo;
+        Mom m = {0.f, 0.f, 0.f};
+        for (int i = lane; i < rows * w; i += 64) {
+            const int r = i / w, c = lo + i - r * w;
+            const int len = s1 - s0 - r;
+            const float n = len > 0 ? (float)((len + rows - 1) / rows) : 0.f;
+            m = merge(m, Mom{n, s_mean[r * wc + c], s_m2[r * wc + c]});
+        }
+        m = wave_merge(m);
+        if (lane == 0) out[g] = m;
+    }
+}
+
+// mean and rstd of the groups g0..g1 of sample b from the partial moments, into shared memory (index g - g0)
+__device__ __forceinline__ void merge_groups(const Mom* __restrict__ part, const Geometry& q, int V, int b, int g0, int g1,
+                                             float eps, float* s_mean, float* s_rstd) {
+    const int lane = threadIdx.x & 63, nw = blockDim.x >> 6;
+    for (int g = g0 + (threadIdx.x >> 6); g <= g1; g += nw) {
+        const int first = (g * q.Cg) / (q.cv * V), last = ((g + 1) * q.Cg - 1) / (q.cv * V);   // slabs that touch the group
+        const int ns = last - first + 1;
+        Mom m = {0.f, 0.f, 0.f};
+        for (int i = lane; i < q.chunks * ns; i += 64) {
+            const int ch = i / ns, sl = first + i - ch * ns;
+            m = merge(m, part[(((int64_t)b * q.chunks + ch) * q.slabs + sl) * q.G + g]);
+        }
+        m = wave_merge(m);
+        if (lane == 0) {
+            s_mean[g - g0] = m.mean;
+            s_rstd[g - g0] = rsqrtf(m.m2 / m.n + eps);
+        }
+    }
+}
+
+template <class T, int V, int ACT>
+__global__ __launch_bounds__(kT) void gn_apply(const T* __restrict__ x, const Mom* __restrict__ part,
+                                               const float* __restrict__ weight, const float* __restrict__ bias,
+                                               T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out,
+                                               Geometry q, float eps) {
+    __shared__ float s_mean[kT * V], s_rstd[kT * V];
+    const int tid = threadIdx.x;
+    const int rows = kT / q.cv;
+    const int row = tid / q.cv, col = tid - row * q.cv;
+    const int slab = blockIdx.y, b = blockIdx.z;
+    const int c0 = slab * q.cv * V;
+    const int wc = min(q.cv * V, q.C - c0);
+    const int g0 = c0 / q.Cg, g1 = (c0 + wc - 1) / q.Cg;
+    merge_groups(part, q, V, b, g0, g1, eps, s_mean, s_rstd);
+    __syncthreads();
+    if (mean_out && blockIdx.x == 0)
+        for (int g = g0 + tid; g <= g1; g += kT) {
+            mean_out[b * q.G + g] = s_mean[g - g0];         // a group of several slabs is written by each, the same bits
+            rstd_out[b * q.G + g] = s_rstd[g - g0];
+        }
+    if (row >= rows || col * V >= wc) return;
+    float mu[V], a[V], sh[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int c = c0 + col * V + j, g = c / q.Cg - g0;
+        mu[j] = s_mean[g];
+        a[j] = s_rstd[g] * (weight ? weight[c] : 1.f);
+        sh[j] = bias ? bias[c] : 0.f;
+    }
+    // the last chunks first: the moments' pass has read them last
+    const int ch = q.chunks - 1 - blockIdx.x;
+    const int s0 = ch * q.chunk, s1 = min(s0 + q.chunk, q.S);
+    const int64_t base = ((int64_t)b * q.S) * q.C + c0 + col * V;
+    auto one = [&](const Raw<T, V>& r, int s) {
+        float v[V];
+        r.get(v);
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = act_of<ACT>(fmaf(v[j] - mu[j], a[j], sh[j]));
+        Raw<T, V>::store(y + base + (int64_t)s * q.C, v);
+    };
+    int s = s0 + row;
+    constexpr int U = 4;
+    for (; s + (U - 1) * rows < s1; s += U * rows) {
+        Raw<T, V> r[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) r[u].load(x + base + (int64_t)(s + u * rows) * q.C);
+#pragma unroll
+        for (int u = 0; u < U; ++u) one(r[u], s + u * rows);
+    }
+    for (; s < s1; s += rows) {
+        Raw<T, V> r;
+        r.load(x + base + (int64_t)s * q.C);
+        one(r, s);
+    }
+}
+
+// ---- backward, two passes over x and dy ------------------------------------------------------------------------
+
+// Per chunk and channel the sums of dz and dz h (chan[(b * chunks + chunk) * 2 + {0, 1}][C]), per chunk, slab and group
+// those of dz w and dz w h (grp[((b * chunks + chunk) * slabs + slab) * G + g][2]).
+template <class T, int V, int ACT>
+__global__ __launch_bounds__(kT) void gn_bwd_sums(const T* __restrict__ x, const T* __restrict__ dy,
+                                                  const float* __restrict__ weight, const float* __restrict__ bias,
+                                                  const float* __restrict__ mean, const float* __restrict__ rstd,
+                                                  float* __restrict__ chan, float* __restrict__ grp, Geometry q) {
+    __shared__ float s_1[kT * V], s_2[kT * V];
+    const int tid = threadIdx.x;
+    const int rows = kT / q.cv;
+    const int row = tid / q.cv, col = tid - row * q.cv;
+    const int slab = blockIdx.y, b = blockIdx.z;
+    const int c0 = slab * q.cv * V;
+    const int wc = min(q.cv * V, q.C - c0);
+    const int s0 = blockIdx.x * q.chunk, s1 = min(s0 + q.chunk, q.S);
+    if (row < rows && col * V < wc) {
+        float mu[V], rs[V], w[V], sh[V], a1[V], a2[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int c = c0 + col * V + j, g = b * q.G + c / q.Cg;
+            mu[j] = mean[g];
+            rs[j] = rstd[g];
+            w[j] = weight ? weight[c] : 1.f;
+            sh[j] = bias ? bias[c] : 0.f;
+            a1[j] = a2[j] = 0.f;
+        }
+        const int64_t base = ((int64_t)b * q.S) * q.C + c0 + col * V;
+        auto add = [&](const Raw<T, V>& rx, const Raw<T, V>& rg) {
+            float v[V], g[V];
+            rx.get(v);
+            rg.get(g);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float h = (v[j] - mu[j]) * rs[j];
+                const float dz = ACT == GN_NONE ? g[j] : g[j] * dact_of<ACT>(fmaf(h, w[j], sh[j]));
+                a1[j] += dz;
+                a2[j] = fmaf(dz, h, a2[j]);
+            }
+        };
+        int s = s0 + row;
+        constexpr int U = 4;
+        for (; s + (U - 1) * rows < s1; s += U * rows) {
+            Raw<T, V> rx[U], rg[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                rx[u].load(x + base + (int64_t)(s + u * rows) * q.C);
+                rg[u].load(dy + base + (int64_t)(s + u * rows) * q.C);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) add(rx[u], rg[u]);
+        }
+        for (; s < s1; s += rows) {
+            Raw<T, V> rx, rg;
+            rx.load(x + base + (int64_t)s * q.C);
+            rg.load(dy + base + (int64_t)s * q.C);
+            add(rx, rg);
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            s_1[row * wc + col * V + j] = a1[j];
+            s_2[row * wc + col * V + j] = a2[j];
+        }
+    }
+    __syncthreads();
+    float* o1 = chan + ((int64_t)b * q.chunks + blockIdx.x) * 2 * q.C + c0;
+    for (int c = tid; c < wc; c += kT) {
+        float t1 = s_1[c], t2 = s_2[c];
+        for (int r = 1; r < rows; ++r) {
+            t1 += s_1[r * wc + c];
+            t2 += s_2[r * wc + c];
+        }
+        o1[c] = t1;
+        o1[q.C + c] = t2;
+        const float w = weight ? weight[c0 + c] : 1.f;
+        s_1[c] = t1 * w;                                   // row 0, column c: read by this thread alone
+        s_2[c] = t2 * w;
+    }
+    __syncthreads();
+    const int g0 = c0 / q.Cg, g1 = (c0 + wc - 1) / q.Cg;
+    const int lane = tid & 63;
+    float* og = grp + (((int64_t)b * q.chunks + blockIdx.x) * q.slabs + slab) * q.G * 2;
+    for (int g = g0 + (tid >> 6); g <= g1; g += kT / 64) {
+        const int lo = max(g * q.Cg - c0, 0), hi = min((g + 1) * q.Cg - c0, wc);
+        float t1 = 0.f, t2 = 0.f;
+        for (int c = lo + lane; c < hi; c += 64) {
+            t1 += s_1[c];
+            t2 += s_2[c];
+        }
+        t1 = wave_sum(t1);
+        t2 = wave_sum(t2);
+        if (lane == 0) {
+            og[2 * g] = t1;
+            og[2 * g + 1] = t2;
+        }
+    }
+}
+
+template <class T, int V, int ACT>
+__global__ __launch_bounds__(kT) void gn_bwd_apply(const T* __restrict__ x, const T* __restrict__ dy,
+                                                   const float* __restrict__ weight, const float* __restrict__ bias,
+                                                   const float* __restrict__ mean, const float* __restrict__ rstd,
+                                                   const float* __restrict__ grp, T* __restrict__ dx, Geometry q) {
+    __shared__ float s_1[kT * V], s_2[kT * V];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int rows = kT / q.cv;
+    const int row = tid / q.cv, col = tid - row * q.cv;
+    const int slab = blockIdx.y, b = blockIdx.z;
+    const int c0 = slab * q.cv * V;
+    const int wc = min(q.cv * V, q.C - c0);
+    const int g0 = c0 / q.Cg, g1 = (c0 + wc - 1) / q.Cg;
+    const float inv_n = 1.0f / ((float)q.S * (float)q.Cg);
+    for (int g = g0 + (tid >> 6); g <= g1; g += kT / 64) {
+        const int first = (g * q.Cg) / (q.cv * V), last = ((g + 1) * q.Cg - 1) / (q.cv * V);
+        const int ns = last - first + 1;
+        float t1 = 0.f, t2 = 0.f;
+        for (int i = lane; i < q.chunks * ns; i += 64) {
+            const int ch = i / ns, sl = first + i - ch * ns;
+            const float* p = grp + ((((int64_t)b * q.chunks + ch) * q.slabs + sl) * q.G + g) * 2;
+            t1 += p[0];
+            t2 += p[1];
+        }
+        t1 = wave_sum(t1);
+        t2 = wave_sum(t2);
+        if (lane == 0) {
+            s_1[g - g0] = t1 * inv_n;
+            s_2[g - g0] = t2 * inv_n;
+        }
+    }
+    __syncthreads();
+    if (row >= rows || col * V >= wc) return;
+    float mu[V], rs[V], w[V], sh[V], m1[V], m2[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int c = c0 + col * V + j, g = c / q.Cg;
+        mu[j] = mean[b * q.G + g];
+        rs[j] = rstd[b * q.G + g];
+        w[j] = weight ? weight[c] : 1.f;
+        sh[j] = bias ? bias[c] : 0.f;
+        m1[j] = s_1[g - g0];
+        m2[j] = s_2[g - g0];
+    }
+    const int ch = q.chunks - 1 - blockIdx.x;
+    const int s0 = ch * q.chunk, s1 = min(s0 + q.chunk, q.S);
+    const int64_t base = ((int64_t)b * q.S) * q.C + c0 + col * V;
+    auto one = [&](const Raw<T, V>& rx, const Raw<T, V>& rg, int s) {
+        float v[V], g[V];
+        rx.get(v);
+        rg.get(g);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float h = (v[j] - mu[j]) * rs[j];
+            const float dz = ACT == GN_NONE ? g[j] : g[j] * dact_of<ACT>(fmaf(h, w[j], sh[j]));
+            v[j] = rs[j] * (fmaf(dz, w[j], -m1[j]) - h * m2[j]);
+        }
+        Raw<T, V>::store(dx + base + (int64_t)s * q.C, v);
+    };
+    int s = s0 + row;
+    constexpr int U = 2;
+    for (; s + (U - 1) * rows < s1; s += U * rows) {
+        Raw<T, V> rx[U], rg[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            rx[u].load(x + base + (int64_t)(s + u * rows) * q.C);
+            rg[u].load(dy + base + (int64_t)(s + u * rows) * q.C);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) one(rx[u], rg[u], s + u * rows);
+    }
+    for (; s < s1; s += rows) {
+        Raw<T, V> rx, rg;
+        rx.load(x + base + (int64_t)s * q.C);
+        rg.load(dy + base + (int64_t)s * q.C);
+        one(rx, rg, s);
+    }
+}
+
+// dweight[c] = sum of chan[r][1][c], dbias[c] = sum of chan[r][0][c] over the rows r, in a fixed order: a workgroup takes
+// 64 of the 2 C columns, its 16 waves every 16th row each, then the 16 sums are added in wave order.
+__global__ __launch_bounds__(1024) void gn_bwd_params(const float* __restrict__ chan, int rows, int C,
+                                                      float* __restrict__ dweight, float* __restrict__ dbias) {
+    __shared__ float red[16][64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int col = blockIdx.x * 64 + lane;
+    const int64_t stride = 2 * (int64_t)C;
+    float acc = 0.f;
+    if (col < 2 * C) {
+        int r = w;
+        for (; r + 7 * 16 < rows; r += 8 * 16) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = chan[(int64_t)(r + 16 * j) * stride + col];
+            acc += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+        }
+        for (; r < rows; r += 16) acc += chan[(int64_t)r * stride + col];
+    }
+    red[w][lane] = acc;
+    __syncthreads();
+    if (w == 0 && col < 2 * C) {
+        float t = red[0][lane];
+#pragma unroll
+        for (int j = 1; j < 16; ++j) t += red[j][lane];
+        if (col < C) {
+            if (dbias) dbias[col] = t;
+        } else if (dweight) {
+            dweight[col - C] = t;
+        }
+    }
+}
+
+int vec_of(int esize, int C, bool aligned) {
+    const int v = 16 / esize;
+    return aligned && C % v == 0 ? v : 1;
+}
+
+// How the work is cut: slabs of at most 256 lanes of V channels, and so many chunks of pixels that about 2,048
+// workgroups share the batch (eight of 256 threads on every CU), with at least four pixels to a lane where there are
+// that many and at most 128 chunks, since every workgroup of the second pass reads a sample's partial sums again.
+Geometry geometry(int B, int S, int C, int G, int V) {
+    Geometry q;
+    q.S = S; q.C = C; q.G = G; q.Cg = C / G;
+    const int lanes = C / V;
+    q.slabs = (lanes + kT - 1) / kT;
+    q.cv = (lanes + q.slabs - 1) / q.slabs;
+    const int rows = kT / q.cv;
+    int64_t chunks = 2048 / ((int64_t)B * q.slabs);
+    const int64_t most = S / (4 * (int64_t)rows);
+    if (chunks > most) chunks = most;
+    if (chunks > 128) chunks = 128;
+    if (chunks < 1) chunks = 1;
+    q.chunk = (int)((S + chunks - 1) / chunks);
+    q.chunks = (S + q.chunk - 1) / q.chunk;
+    return q;
+}
+
+template <class F>
+hipError_t by_act(int act, F&& f) {
+    switch (act) {
+        case GN_RELU: return f(std::integral_constant<int, GN_RELU>{});
+        case GN_GELU: return f(std::integral_constant<int, GN_GELU>{});
+        case GN_SILU: return f(std::integral_constant<int, GN_SILU>{});
+        default: return f(std::integral_constant<int, GN_NONE>{});
+    }
+}
+
+template <class T, int V>
+hipError_t forward(const T* x, const float* weight, const float* bias, T* y, float* mean, float* rstd, Mom* part, int B,
+                   int S, int C, int G, float eps, int act, hipStream_t s) {
+    const Geometry q = geometry(B, S, C, G, V);
+    const dim3 grid(q.chunks, q.slabs, B);
+    hipLaunchKernelGGL((gn_moments<T, V>), grid, dim3(kT), 0, s, x, part, q);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    return by_act(act, [&](auto a) {
+        hipLaunchKernelGGL((gn_apply<T, V, decltype(a)::value>), grid, dim3(kT), 0, s, x, part, weight, bias, y, mean, rstd, q, eps);
+        return hipGetLastError();
+    });
+}
+
+template <class T, int V>
+hipError_t backward(const T* x, const float* weight, const float* bias, const T* dy, const float* mean, const float* rstd,
+                    T* dx, float* dweight, float* dbias, float* ws, int B, int S, int C, int G, int act, hipStream_t s) {
+    const Geometry q = geometry(B, S, C, G, V);
+    float* chan = ws;
+    float* grp = ws + (int64_t)B * q.chunks * 2 * C;
+    const dim3 grid(q.chunks, q.slabs, B);
+    hipError_t e = by_act(act, [&](auto a) {
+        hipLaunchKernelGGL((gn_bwd_sums<T, V, decltype(a)::value>), grid, dim3(kT), 0, s, x, dy, weight, bias, mean, rstd, chan, grp, q);
+        hipError_t r = hipGetLastError();
+        if (r != hipSuccess) return r;
+        hipLaunchKernelGGL((gn_bwd_apply<T, V, decltype(a)::value>), grid, dim3(kT), 0, s, x, dy, weight, bias, mean, rstd, grp, dx, q);
+        return hipGetLastError();
+    });
+    if (e != hipSuccess || (!dweight && !dbias)) return e;
+    hipLaunchKernelGGL(gn_bwd_params, dim3((2 * C + 63) / 64), dim3(1024), 0, s, chan, B * q.chunks, C, dweight, dbias);
+    return hipGetLastError();
+}
+
+bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace
+
+// f32 values of scratch: what the forward (backward = false) or the backward needs at most, whatever the alignment
+int64_t group_norm_workspace(int B, int S, int C, int G, bool bf16, bool backward) {
+    int64_t most = 0;
+    for (const bool al : {false, true}) {
+        const Geometry q = geometry(B, S, C, G, vec_of(bf16 ? 2 : 4, C, al));
+        const int64_t blocks = (int64_t)B * q.chunks;
+        const int64_t n = backward ? blocks * 2 * C + blocks * q.slabs * G * 2 : blocks * q.slabs * G * 3;
+        most = n > most ? n : most;
+    }
+    return most;
+}
+
+hipError_t launch_group_norm(const void* x, const float* weight, const float* bias, void* y, float* mean, float* rstd,
+                             float* ws, int B, int S, int C, int G, float eps, int act, bool bf16, hipStream_t s) {
+    Mom* part = reinterpret_cast<Mom*>(ws);
+    const bool al = aligned(x) && aligned(y);
+    if (bf16) {
+        auto xb = reinterpret_cast<const bf16_t*>(x);
+        auto yb = reinterpret_cast<bf16_t*>(y);
+        return vec_of(2, C, al) == 8 ? forward<bf16_t, 8>(xb, weight, bias, yb, mean, rstd, part, B, S, C, G, eps, act, s)
+                                     : forward<bf16_t, 1>(xb, weight, bias, yb, mean, rstd, part, B, S, C, G, eps, act, s);
+    }
+    auto xf = reinterpret_cast<const float*>(x);
+    auto yf = reinterpret_cast<float*>(y);
+    return vec_of(4, C, al) == 4 ? forward<float, 4>(xf, weight, bias, yf, mean, rstd, part, B, S, C, G, eps, act, s)
+                                 : forward<float, 1>(xf, weight, bias, yf, mean, rstd, part, B, S, C, G, eps, act, s);
+}
+
+hipError_t launch_group_norm_backward(const void* x, const float* weight, const float* bias, const void* dy, const float* mean,
+                                      const float* rstd, void* dx, float* dweight, float* dbias, float* ws, int B, int S,
+                                      int C, int G, int act, bool bf16, hipStream_t s) {
+    const bool al = aligned(x) && aligned(dy) && aligned(dx);
+    if (bf16) {
+        auto xb = reinterpret_cast<const bf16_t*>(x);
+        auto gb = reinterpret_cast<const bf16_t*>(dy);
+        auto db = reinterpret_cast<bf16_t*>(dx);
+        return vec_of(2, C, al) == 8
+                   ? backward<bf16_t, 8>(xb, weight, bias, gb, mean, rstd, db, dweight, dbias, ws, B, S, C, G, act, s)
+                   : backward<bf16_t, 1>(xb, weight, bias, gb, mean, rstd, db, dweight, dbias, ws, B, S, C, G, act, s);
+    }
+    auto xf = reinterpret_cast<const float*>(x);
+    auto gf = reinterpret_cast<const float*>(dy);
+    auto df = reinterpret_cast<float*>(dx);
+    return vec_of(4, C, al) == 4
+               ? backward<float, 4>(xf, weight, bias, gf, mean, rstd, df, dweight, dbias, ws, B, S, C, G, act, s)
+               : backward<float, 1>(xf, weight, bias, gf, mean, rstd, df, dweight, dbias, ws, B, S, C, G, act, s);
+}
+
+}  // namespace vitk

@@ -2,8 +2,13 @@
 // reporting.  Declarations and the reference call sites each entry point
 // replaces are in include/vitk.h.
 #include <stdarg.h>
-#include <atomic>
 #include <stdio.h>
+
+#include <algorithm>
+#include <atomic>
+#include <exception>
+#include <utility>
+#include <vector>
 
 #include "../../include/vitk.h"
 #include "gemm_plan.h"
@@ -70,7 +75,7 @@ int dense(const char* name, const void* A, const void* W, const float* bias, con
 
 extern "C" {
 
-int vitk_version(void) { return 10; }
+int vitk_version(void) { return 11; }
 
 const char* vitk_last_error(void) { return g_err; }
 
@@ -577,6 +582,116 @@ int vitk_gemm_plan(int M, int N, int K, int cus, int* plan) {
     const int out[10] = {pl.mtot, pl.tiles_m, pl.tiles_n, pl.gn, pl.mixed, pl.xcd_units, pl.ha, pl.na, pl.hb, pl.nb};
     for (int i = 0; i < 10; ++i) plan[i] = out[i];
     return VITK_OK;
+}
+
+// ---- group normalisation with an activation ----------------------------------------------------
+
+static int group_norm_sizes(const char* name, int batch, int pixels, int channels, int groups, int act, int dtype) {
+    if (batch <= 0 || pixels <= 0 || channels <= 0 || groups <= 0)
+        return fail(VITK_ERR_INVALID, "%s: non-positive size batch=%d pixels=%d channels=%d groups=%d", name, batch, pixels, channels, groups);
+    if (channels % groups != 0) return fail(VITK_ERR_INVALID, "%s: %d channels do not divide into %d groups", name, channels, groups);
+    if (act < VITK_ACT_NONE || act > VITK_ACT_SILU) return fail(VITK_ERR_INVALID, "%s: activation=%d", name, act);
+    if (dtype != VITK_F32 && dtype != VITK_BF16) return fail(VITK_ERR_UNSUPPORTED, "%s: dtype=%d", name, dtype);
+    if (batch > 65535 || channels > (1 << 20) || (int64_t)batch * groups > INT32_MAX || pixels > (1 << 30))
+        return fail(VITK_ERR_UNSUPPORTED, "%s: batch=%d (at most 65535), channels=%d (2^20), pixels=%d (2^30)", name, batch, channels, pixels);
+    return VITK_OK;
+}
+
+int64_t vitk_group_norm_workspace(int batch, int pixels, int channels, int groups, int dtype, int backward) {
+    if (group_norm_sizes("vitk_group_norm_workspace", batch, pixels, channels, groups, VITK_ACT_NONE, dtype)) return -1;
+    return group_norm_workspace(batch, pixels, channels, groups, dtype == VITK_BF16, backward != 0);
+}
+
+int vitk_group_norm(const void* x, const float* weight, const float* bias, void* y, float* mean, float* rstd,
+                    float* workspace, int64_t workspace_floats, int batch, int pixels, int channels, int groups, float eps,
+                    int act, int dtype, void* stream) {
+    const char* name = "vitk_group_norm";
+    if (!x || !y || !workspace) return fail(VITK_ERR_INVALID, "%s: null pointer", name);
+    if ((mean == nullptr) != (rstd == nullptr)) return fail(VITK_ERR_INVALID, "%s: mean and rstd come together", name);
+    const int rc = group_norm_sizes(name, batch, pixels, channels, groups, act, dtype);
+    if (rc) return rc;
+    const bool bf = dtype == VITK_BF16;
+    const int64_t need = group_norm_workspace(batch, pixels, channels, groups, bf, false);
+    if (workspace_floats < need) return fail(VITK_ERR_INVALID, "%s: workspace of %lld floats, %lld needed", name, (long long)workspace_floats, (long long)need);
+    return launched(launch_group_norm(x, weight, bias, y, mean, rstd, workspace, batch, pixels, channels, groups, eps, act, bf,
+                                      reinterpret_cast<hipStream_t>(stream)), name);
+}
+
+int vitk_group_norm_backward(const void* x, const float* weight, const float* bias, const void* dy, const float* mean,
+                             const float* rstd, void* dx, float* dweight, float* dbias, float* workspace,
+                             int64_t workspace_floats, int batch, int pixels, int channels, int groups, int act, int dtype,
+                             void* stream) {
+    const char* name = "vitk_group_norm_backward";
+    if (!x || !dy || !mean || !rstd || !dx || !workspace) return fail(VITK_ERR_INVALID, "%s: null pointer", name);
+    const int rc = group_norm_sizes(name, batch, pixels, channels, groups, act, dtype);
+    if (rc) return rc;
+    const bool bf = dtype == VITK_BF16;
+    const int64_t need = group_norm_workspace(batch, pixels, channels, groups, bf, true);
+    if (workspace_floats < need) return fail(VITK_ERR_INVALID, "%s: workspace of %lld floats, %lld needed", name, (long long)workspace_floats, (long long)need);
+    return launched(launch_group_norm_backward(x, weight, bias, dy, mean, rstd, dx, dweight, dbias, workspace, batch, pixels,
+                                               channels, groups, act, bf, reinterpret_cast<hipStream_t>(stream)), name);
+}
+
+// ---- global gradient norm and clipping -----------------------------------------------------------
+
+static int grad_list(const char* name, const uint64_t* addr, const int64_t* size, const int* dtype, int n, int norm_kind,
+                     bool written) {
+    if (n < 0 || (n > 0 && (!addr || !size || !dtype))) return fail(VITK_ERR_INVALID, "%s: null pointer", name);
+    if (norm_kind != VITK_NORM_2 && norm_kind != VITK_NORM_INF) return fail(VITK_ERR_INVALID, "%s: norm_kind=%d", name, norm_kind);
+    bool ordered = true;
+    uint64_t end = 0;
+    for (int i = 0; i < n; ++i) {
+        if (dtype[i] != VITK_F32 && dtype[i] != VITK_BF16) return fail(VITK_ERR_UNSUPPORTED, "%s: dtype %d of tensor %d", name, dtype[i], i);
+        if (size[i] < 0 || size[i] >= (int64_t)1 << 46) return fail(VITK_ERR_INVALID, "%s: size %lld of tensor %d", name, (long long)size[i], i);
+        if (size[i] == 0) continue;
+        const int es = dtype[i] == VITK_BF16 ? 2 : 4;
+        if (!addr[i] || addr[i] % es) return fail(VITK_ERR_INVALID, "%s: null or misaligned tensor %d", name, i);
+        ordered &= addr[i] >= end;
+        end = addr[i] + (uint64_t)size[i] * es;
+    }
+    if (!written || ordered) return VITK_OK;
+    // Tensors that share memory would be scaled by two workgroups at once.
+    try {
+        std::vector<std::pair<uint64_t, uint64_t>> spans;
+        spans.reserve(n);
+        for (int i = 0; i < n; ++i)
+            if (size[i] > 0) spans.emplace_back(addr[i], addr[i] + (uint64_t)size[i] * (dtype[i] == VITK_BF16 ? 2 : 4));
+        std::sort(spans.begin(), spans.end());
+        for (size_t i = 1; i < spans.size(); ++i)
+            if (spans[i].first < spans[i - 1].second) return fail(VITK_ERR_INVALID, "%s: two of the tensors share memory", name);
+    } catch (const std::exception&) {
+        return fail(VITK_ERR_INVALID, "%s: out of host memory", name);
+    }
+    return VITK_OK;
+}
+
+int64_t vitk_grad_norm_workspace(int n) {
+    if (n < 0) return -1;
+    return ((int64_t)n + kGradTensorsPerLaunch - 1) / kGradTensorsPerLaunch * kGradPartialsPerLaunch;
+}
+
+int vitk_grad_norm(const uint64_t* addr, const int64_t* size, const int* dtype, int n, int norm_kind, double* partials,
+                   int64_t n_partials, float* norm, void* stream) {
+    const char* name = "vitk_grad_norm";
+    const int rc = grad_list(name, addr, size, dtype, n, norm_kind, false);
+    if (rc) return rc;
+    if (!partials && (n > 0 || norm)) return fail(VITK_ERR_INVALID, "%s: null pointer", name);
+    if (n_partials < vitk_grad_norm_workspace(n))
+        return fail(VITK_ERR_INVALID, "%s: %lld partial sums, %lld needed", name, (long long)n_partials, (long long)vitk_grad_norm_workspace(n));
+    return launched(launch_grad_norm(addr, size, dtype, n, norm_kind == VITK_NORM_INF, partials, norm, reinterpret_cast<hipStream_t>(stream)), name);
+}
+
+int vitk_grad_clip(const uint64_t* addr, const int64_t* size, const int* dtype, int n, int norm_kind, const double* partials,
+                   int64_t n_partials, double max_norm, float* norm, void* stream) {
+    const char* name = "vitk_grad_clip";
+    const int rc = grad_list(name, addr, size, dtype, n, norm_kind, true);
+    if (rc) return rc;
+    if (!partials && n > 0) return fail(VITK_ERR_INVALID, "%s: null pointer", name);
+    if (!(max_norm >= 0.0)) return fail(VITK_ERR_INVALID, "%s: max_norm=%g must not be negative", name, max_norm);
+    if (n_partials < vitk_grad_norm_workspace(n))
+        return fail(VITK_ERR_INVALID, "%s: %lld partial sums, %lld needed", name, (long long)n_partials, (long long)vitk_grad_norm_workspace(n));
+    return launched(launch_grad_scale(addr, size, dtype, n, norm_kind == VITK_NORM_INF, partials,
+                                      grad_partials(addr, size, dtype, n), max_norm, norm, reinterpret_cast<hipStream_t>(stream)), name);
 }
 
 int vitk_init(void) {

@@ -100,4 +100,22 @@ hipError_t launch_patch_f32(const float* img, const float* w, const float* bias,
 hipError_t launch_attention_f32(const float* q, const float* k, const float* v, float* out, int batch, int heads,
                                 int ntok, int hd, float scale, hipStream_t s);
 
+// group normalisation with an activation (group_norm.hip)
+enum GroupNormAct { GN_NONE = 0, GN_RELU = 1, GN_GELU = 2, GN_SILU = 3 };
+int64_t group_norm_workspace(int B, int S, int C, int G, bool bf16, bool backward);
+hipError_t launch_group_norm(const void* x, const float* weight, const float* bias, void* y, float* mean, float* rstd,
+                             float* ws, int B, int S, int C, int G, float eps, int act, bool bf16, hipStream_t s);
+hipError_t launch_group_norm_backward(const void* x, const float* weight, const float* bias, const void* dy, const float* mean,
+                                      const float* rstd, void* dx, float* dweight, float* dbias, float* ws, int B, int S,
+                                      int C, int G, int act, bool bf16, hipStream_t s);
+
+// global gradient norm and clipping (grad_clip.hip): one launch covers kGradTensorsPerLaunch tensors and leaves at most
+// kGradPartialsPerLaunch partial sums
+constexpr int kGradTensorsPerLaunch = 184, kGradPartialsPerLaunch = 1024;
+int grad_partials(const uint64_t* addr, const int64_t* size, const int* bf16, int n);
+hipError_t launch_grad_norm(const uint64_t* addr, const int64_t* size, const int* bf16, int n, bool inf, double* partials,
+                            float* norm, hipStream_t s);
+hipError_t launch_grad_scale(const uint64_t* addr, const int64_t* size, const int* bf16, int n, bool inf,
+                             const double* partials, int npartials, double max_norm, float* norm, hipStream_t s);
+
 }  // namespace vitk

@@ -11,12 +11,14 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("VITK_LIB") or os.path.join(_HERE, "libvitk.so")
 
 VITK_F32, VITK_BF16 = 0, 1
-ABI_VERSION = 10
+VITK_ERR_UNSUPPORTED = 2
+ABI_VERSION = 11
 
 _p = ctypes.c_void_p
 _i = ctypes.c_int
 _i64 = ctypes.c_int64
 _f = ctypes.c_float
+_d = ctypes.c_double
 
 # name -> argument types; every function returns int except where noted.
 SIGNATURES = {
@@ -55,11 +57,24 @@ SIGNATURES = {
     "vitk_ln_finalize": [_p, _p, _i, _i, _f, _p],
     "vitk_gemm_ln_bias_gelu": [_p, _p, _p, _p, _p, _p, _i, _i, _i, _p],
     "vitk_qkv_proj_ln": [_p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p],
+    "vitk_group_norm": [_p, _p, _p, _p, _p, _p, _p, _i64, _i, _i, _i, _i, _f, _i, _i, _p],
+    "vitk_group_norm_backward": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i, _i, _i, _i, _i, _i, _p],
+    "vitk_grad_norm": [_p, _p, _p, _i, _i, _p, _i64, _p, _p],
+    "vitk_grad_clip": [_p, _p, _p, _i, _i, _p, _i64, _d, _p, _p],
+}
+# scratch sizes: int64 results, -1 for what the entry point does not take
+WORKSPACES = {
+    "vitk_gemm_tn_workspace": [_i, _i, _i],
+    "vitk_gemm_tn_colsum_workspace": [_i, _i, _i],
+    "vitk_group_norm_workspace": [_i, _i, _i, _i, _i, _i],
+    "vitk_grad_norm_workspace": [_i],
 }
 EPI_BIAS, EPI_GELU, EPI_RESIDUAL, EPI_TANH = 0, 1, 2, 3      # vitk_gemm_f32 epilogues (include/vitk.h)
 ACT_GELU, ACT_TANH = 0, 1                                    # vitk_gemm_grad_act
-EXPORTS = sorted(list(SIGNATURES) + ["vitk_version", "vitk_last_error", "vitk_set_debug_variant", "vitk_set_cu_limit",
-                                    "vitk_gemm_tn_workspace", "vitk_gemm_tn_colsum_workspace"])
+GROUP_NORM_ACTS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}   # vitk_group_norm
+NORM_2, NORM_INF = 0, 1                                      # vitk_grad_norm
+EXPORTS = sorted(list(SIGNATURES) + list(WORKSPACES) + ["vitk_version", "vitk_last_error", "vitk_set_debug_variant",
+                                                        "vitk_set_cu_limit"])
 
 _lib = None
 
@@ -86,9 +101,10 @@ def load():
     lib.vitk_set_debug_variant.argtypes = [_i, _i]
     lib.vitk_set_cu_limit.restype = None
     lib.vitk_set_cu_limit.argtypes = [_i]
-    for fn in (lib.vitk_gemm_tn_workspace, lib.vitk_gemm_tn_colsum_workspace):
+    for name, args in WORKSPACES.items():
+        fn = getattr(lib, name)
         fn.restype = _i64
-        fn.argtypes = [_i, _i, _i]
+        fn.argtypes = args
     for name, args in SIGNATURES.items():
         fn = getattr(lib, name)
         fn.restype = _i

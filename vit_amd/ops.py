@@ -608,3 +608,146 @@ def colsum_static(g, out=None):
     with torch.cuda.device(g.device), _span("colsum"):
         _lib.check(L.vitk_colsum_bf16_static(_ptr(g), _ptr(out), R, M, _stream()), L)
     return out
+
+
+# ---- group normalisation with an activation, channels last -----------------------------------------
+
+_DTYPE_CODES = {torch.float32: _lib.VITK_F32, torch.bfloat16: _lib.VITK_BF16}
+
+
+def _gn_sizes(x, num_groups, weight, bias, activation):
+    if x.dtype not in _DTYPE_CODES:
+        raise _lib.VitkError(f"group_norm: x must be bf16 or f32, got {x.dtype}")
+    _chk(x, x.dtype, "x")
+    if x.dim() < 2:
+        raise _lib.VitkError(f"group_norm: expected [batch, ..., channels], got {tuple(x.shape)}")
+    C, B = x.shape[-1], x.shape[0]
+    if num_groups < 1 or C % num_groups:
+        raise _lib.VitkError(f"group_norm: {C} channels do not divide into {num_groups} groups")
+    if activation not in _lib.GROUP_NORM_ACTS:
+        raise _lib.VitkError(f"group_norm: activation must be one of {sorted(_lib.GROUP_NORM_ACTS)}, got {activation!r}")
+    for n, t in (("weight", weight), ("bias", bias)):
+        if t is not None:
+            _chk(t, torch.float32, n)
+            if t.numel() != C:
+                raise _lib.VitkError(f"group_norm: {n} has {t.numel()} elements, expected {C}")
+            if t.device != x.device:
+                raise _lib.VitkError(f"group_norm: {n} is on {t.device}, x on {x.device}")
+    return B, (x.numel() // (B * C) if B * C else 0), C
+
+
+def _scratch(floats, device):
+    # from torch's allocator, per call: it is the calling stream's (or the capturing graph's) own, whatever else runs
+    return torch.empty(floats, dtype=torch.float32, device=device)
+
+
+def group_norm(x, num_groups, weight, bias, eps, activation="none", stats=False):
+    """(y, mean, rstd): y = act(GroupNorm(x)) for x bf16 / f32 [batch, ..., channels]; mean, rstd f32 [batch, groups]
+    with `stats`, else None."""
+    L = _lib.load()
+    B, S, C = _gn_sizes(x, num_groups, weight, bias, activation)
+    y = torch.empty_like(x)
+    mean = rstd = None
+    if stats:
+        mean, rstd = torch.empty(2, B, num_groups, dtype=torch.float32, device=x.device).unbind(0)
+    if x.numel() == 0:
+        return y, mean, rstd
+    code = _DTYPE_CODES[x.dtype]
+    n = L.vitk_group_norm_workspace(B, S, C, num_groups, code, 0)
+    if n < 0:
+        _lib.check(_lib.VITK_ERR_UNSUPPORTED, L)
+    ws = _scratch(n, x.device)
+    with _span("group_norm"):
+        _lib.check(L.vitk_group_norm(_ptr(x), _ptr(weight), _ptr(bias), _ptr(y), _ptr(mean), _ptr(rstd), _ptr(ws), n, B, S, C,
+                                     num_groups, float(eps), _lib.GROUP_NORM_ACTS[activation], code, _stream()), L)
+    return y, mean, rstd
+
+
+def group_norm_backward(x, num_groups, weight, bias, dy, mean, rstd, activation="none", param_grads=True):
+    """(dx, dweight, dbias) of group_norm(); dweight and dbias f32 [channels], or None without `param_grads`."""
+    L = _lib.load()
+    B, S, C = _gn_sizes(x, num_groups, weight, bias, activation)
+    _chk(dy, x.dtype, "dy")
+    if dy.shape != x.shape:
+        raise _lib.VitkError(f"group_norm_backward: dy {tuple(dy.shape)} vs x {tuple(x.shape)}")
+    for n, t in (("mean", mean), ("rstd", rstd)):
+        _chk(t, torch.float32, n)
+        if t.numel() != B * num_groups:
+            raise _lib.VitkError(f"group_norm_backward: {n} has {t.numel()} elements, expected {B * num_groups}")
+    dx = torch.empty_like(x)
+    dw = db = None
+    if param_grads:
+        dw, db = torch.empty(2, C, dtype=torch.float32, device=x.device).unbind(0)
+    if x.numel() == 0:
+        return dx, dw if dw is None else dw.zero_(), db if db is None else db.zero_()
+    code = _DTYPE_CODES[x.dtype]
+    n = L.vitk_group_norm_workspace(B, S, C, num_groups, code, 1)
+    if n < 0:
+        _lib.check(_lib.VITK_ERR_UNSUPPORTED, L)
+    ws = _scratch(n, x.device)
+    with _span("group_norm_backward"):
+        _lib.check(L.vitk_group_norm_backward(_ptr(x), _ptr(weight), _ptr(bias), _ptr(dy), _ptr(mean), _ptr(rstd), _ptr(dx),
+                                              _ptr(dw), _ptr(db), _ptr(ws), n, B, S, C, num_groups,
+                                              _lib.GROUP_NORM_ACTS[activation], code, _stream()), L)
+    return dx, dw, db
+
+
+# ---- global gradient norm and clipping -------------------------------------------------------------
+
+def _dense(t):
+    """Whether the tensor's elements fill one run of memory (in any order of its dimensions)."""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if st != want:
+            return False
+        want *= n
+    return True
+
+
+class GradList:
+    """The host arrays that the vitk_grad_* entry points take: addresses, sizes and types of dense bf16 / f32 tensors of
+    one device."""
+
+    def __init__(self, tensors):
+        codes = _DTYPE_CODES
+        dev = tensors[0].get_device()
+        addr, size, kind = [], [], []
+        for t in tensors:
+            if t.layout is not torch.strided or t.dtype not in codes:
+                raise _lib.VitkError(f"gradients must be dense bf16 or f32 tensors, got {t.dtype}, {t.layout}")
+            if not t.is_cuda or t.get_device() != dev:
+                raise _lib.VitkError(f"gradients must be on one CUDA/HIP device, got {tensors[0].device} and {t.device}")
+            if not _dense(t):
+                raise _lib.VitkError(f"a gradient of shape {tuple(t.shape)} and strides {t.stride()} does not fill its memory")
+            addr.append(t.data_ptr())
+            size.append(t.numel())
+            kind.append(codes[t.dtype])
+        n = self.n = len(addr)
+        c = _lib.ctypes
+        self.addr, self.size, self.kind = (c.c_uint64 * n)(*addr), (c.c_int64 * n)(*size), (c.c_int * n)(*kind)
+        self.device = tensors[0].device
+
+
+def grad_norm(grads, kind=_lib.NORM_2, want_norm=True):
+    """(partials, norm): the partial sums grad_clip() takes and, with `want_norm`, the norm as an f32 scalar on the
+    device; `grads` a GradList."""
+    L = _lib.load()
+    need = L.vitk_grad_norm_workspace(grads.n)
+    partials = torch.empty(need, dtype=torch.float64, device=grads.device)
+    norm = torch.empty((), dtype=torch.float32, device=grads.device) if want_norm else None
+    with _span("grad_norm"):
+        _lib.check(L.vitk_grad_norm(grads.addr, grads.size, grads.kind, grads.n, kind, _ptr(partials), need, _ptr(norm),
+                                    _stream()), L)
+    return partials, norm
+
+
+def grad_clip(grads, partials, max_norm, kind=_lib.NORM_2, norm=None):
+    """g *= min(1, max_norm / (norm + 1e-6)) in place, from grad_norm()'s partial sums of the same GradList; the norm goes
+    to `norm` (f32 scalar) if given."""
+    L = _lib.load()
+    with _span("grad_clip"):
+        _lib.check(L.vitk_grad_clip(grads.addr, grads.size, grads.kind, grads.n, kind, _ptr(partials), partials.numel(),
+                                    float(max_norm), _ptr(norm), _stream()), L)
+    return norm

@@ -47,6 +47,55 @@ def accuracy(output, target, topk=(1,)):
     return res
 
 
+def _norm_kind(norm_type):
+    if float(norm_type) == 2.0:
+        return _lib.NORM_2
+    if float(norm_type) == math.inf:
+        return _lib.NORM_INF
+    raise _lib.VitkError(f"norm_type must be 2 or inf, got {norm_type!r}")
+
+
+def grad_norm(tensors, norm_type=2.0):
+    """Norm of all the tensors' values taken together (sqrt of the sum of squares, or the largest magnitude) as an f32
+    scalar on their device; bf16 and f32 tensors of any sizes, dense, on one device.  NaN if any value is one."""
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    kind = _norm_kind(norm_type)
+    if not tensors:
+        return torch.tensor(0.0)
+    grads = _ops.GradList(tensors)
+    with torch.cuda.device(grads.device):
+        return _ops.grad_norm(grads, kind)[1]
+
+
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """Scale the parameters' gradients in place so that their common norm is at most max_norm, and return the norm they
+    had (f32 scalar on their device): torch.nn.utils.clip_grad_norm_ of the reference's training step (main.py:221-223),
+    with the same factor min(1, max_norm / (norm + 1e-6)).
+
+    Two kernel launches for up to 184 tensors and no host synchronisation (error_if_nonfinite has to wait for the norm).
+    Gradients of bf16 or f32, dense, on one device, no two sharing memory.  A norm of NaN makes every gradient NaN and one of inf
+    makes them 0 (NaN where they are infinite), as in torch."""
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
+    tensors = [p.grad for p in parameters if p.grad is not None]
+    kind = _norm_kind(norm_type)
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise _lib.VitkError(f"max_norm must not be negative, got {max_norm}")
+    if not tensors:
+        return torch.tensor(0.0)
+    grads = _ops.GradList(tensors)
+    with torch.cuda.device(grads.device):
+        if error_if_nonfinite or not any(grads.size):
+            partials, norm = _ops.grad_norm(grads, kind)
+            if error_if_nonfinite and not math.isfinite(float(norm)):
+                raise _lib.VitkError(f"the gradients' norm is {float(norm)}, so they cannot be clipped (error_if_nonfinite)")
+            _ops.grad_clip(grads, partials, max_norm, kind)
+            return norm
+        partials, _ = _ops.grad_norm(grads, kind, want_norm=False)
+        norm = torch.empty((), dtype=torch.float32, device=grads.device)
+        return _ops.grad_clip(grads, partials, max_norm, kind, norm)
+
+
 def pos_embed_scale(pos_embed, img_size, patch_size, mode='constant', order=1):
     """pos_embed [1, 1 + g*g, D] -> [1, 1 + G*G, D], G = img_size // patch_size; returned on the input's
     device and dtype.  Unchanged (the same tensor) when the lengths already agree, as in the reference."""
