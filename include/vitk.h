@@ -322,6 +322,38 @@ int vitk_gemm_ln_bias_gelu(const void* A, const void* Wg, const float* ab, const
 int vitk_qkv_proj_ln(const void* A, const void* Wg, const float* ab, const float* colsum, const float* c, void* qkv,
                      int batch, int ntok, int heads, int hd, void* stream);
 
+/* ---- differential attention ------------------------------------------------------------------------
+ * The difference of two softmax maps with a learned weight, on the same q/k/v that vitk_attention takes with every head's
+ * channels halved between the maps (models/transformer.py:43-46 holds the one-map form):
+ *   P_m = softmax_s(scale q[b,t,h,m,:] . k[b,s,h',m,:]),  h' = h / (heads / kv_heads)
+ *   out[b,t,h,:] = sum_s (P_1 - w_h P_2) v[b,s,h',:],  w_h = exp(lam_0 . lam_1) - exp(lam_2 . lam_3) + lambda_init
+ * q [batch, nq, heads, 2, d], k [batch, nk, kv_heads, 2, d], v [batch, nk, kv_heads, 2 d], bf16 or f32 (dtype), with any
+ * strides that are multiples of 16 bytes (last dimension dense): strides is a HOST array of 11 element strides, q's and
+ * k's (sample, token, head, map) and v's (sample, token, head).  lam f32 [4, lam_heads, d], lam_heads = heads or 1 (one
+ * for all).  key_lens (int32 [batch] on the device, or NULL): keys from key_lens[b] on are hidden and never read; values
+ * outside 0..nk count as 0 or nk.  causal: query t sees keys up to t + nk - nq.  A row that sees no key gives 0.
+ * d a multiple of 8 up to 64; scale > 0; probabilities, sums and accumulators in f32. */
+
+/* f32 values of scratch (0: none needed); -1 for sizes it does not take. */
+int64_t vitk_diff_attention_workspace(int batch, int nq, int nk, int heads, int kv_heads, int d, int dtype, int backward);
+
+/* out [batch, nq, heads, 2 d] in q's type, contiguous.  For the backward also, together or all NULL: out2 (the second
+ * map's sum P_2 v, out's shape), lse f32 [2, batch, heads, nq] (log2 of the denominators of exp(scale s)) and weight f32
+ * [heads]. */
+int vitk_diff_attention(const void* q, const void* k, const void* v, const int64_t* strides, const float* lam, int lam_heads,
+                        float lambda_init, float scale, const int* key_lens, int causal, void* out, void* out2, float* lse,
+                        float* weight, float* workspace, int64_t workspace_floats, int batch, int nq, int nk, int heads,
+                        int kv_heads, int d, int dtype, void* stream);
+
+/* Gradients from the forward's inputs and results and dout (out's shape): dq, dk, dv (shapes of q, k, v, element strides
+ * in the HOST array grad_strides as above) and dlam (f32, lam's shape; may be NULL).  Hidden keys get 0.  No atomics:
+ * results are reproducible. */
+int vitk_diff_attention_backward(const void* q, const void* k, const void* v, const int64_t* strides, const float* lam,
+                                 int lam_heads, float scale, const int* key_lens, int causal, const void* out, const void* out2,
+                                 const float* lse, const float* weight, const void* dout, void* dq, void* dk, void* dv,
+                                 const int64_t* grad_strides, float* dlam, float* workspace, int64_t workspace_floats, int batch,
+                                 int nq, int nk, int heads, int kv_heads, int d, int dtype, void* stream);
+
 /* ---- group normalisation with an activation, channels last ---------------------------------------------
  * y = act((x - mean_g) rstd_g * weight[c] + bias[c]) on x [batch, pixels, channels] (a channels-last feature map, or
  * tokens), statistics per sample over all pixels of channels / groups neighbouring channels, biased variance, eps inside

@@ -303,6 +303,26 @@ class AttentionFn(torch.autograd.Function):
         return dqkv, None
 
 
+class DiffAttentionFn(torch.autograd.Function):
+    """out = (P_1 - w P_2) v of ops.diff_attention; the backward rebuilds the probabilities from q, k and the saved
+    denominators."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, lam, lambda_init, scale, key_lens, causal):
+        out, out2, lse, weight = ops.diff_attention(q, k, v, lam, lambda_init, scale, key_lens, causal, train=True)
+        ctx.save_for_backward(q, k, v, lam, key_lens, out, out2, lse, weight)
+        ctx.scale, ctx.causal = scale, causal
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        q, k, v, lam, key_lens, out, out2, lse, weight = ctx.saved_tensors
+        dq, dk, dv, dlam = ops.diff_attention_backward(q, k, v, lam, ctx.scale, key_lens, ctx.causal, out, out2, lse, weight,
+                                                       g.contiguous(), lam_grad=ctx.needs_input_grad[3])
+        return dq, dk, dv, dlam, None, None, None, None
+
+
 class GroupNormFn(torch.autograd.Function):
     """act(GroupNorm(x)) on x [batch, ..., channels]; the backward recomputes the normalised values from x and the saved
     mean and rstd."""

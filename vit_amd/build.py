@@ -15,8 +15,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libvitk.so")
 SOURCES = ["vitk_api.hip", "gemm.hip", "gemm_pipe.hip", "gemm_pp.hip", "attention.hip", "rowops.hip", "f32path.hip", "backward.hip", "gemm_tn.hip", "attention_bwd.hip",
-           "group_norm.hip", "grad_clip.hip"]
-HEADERS = [os.path.join(CSRC, "vitk_common.h"), os.path.join(CSRC, "vitk_kernels.h"), os.path.join(CSRC, "gemm_common.h"), os.path.join(CSRC, "gemm_plan.h"),
+           "group_norm.hip", "grad_clip.hip", "diff_attention.hip", "diff_attention_bwd.hip"]
+HEADERS = [os.path.join(CSRC, "vitk_common.h"), os.path.join(CSRC, "vitk_kernels.h"), os.path.join(CSRC, "gemm_common.h"), os.path.join(CSRC, "gemm_plan.h"), os.path.join(CSRC, "diff_attention.h"),
            os.path.join(os.path.dirname(HERE), "include", "vitk.h")]
 FLAGS = ["-O3", "-std=c++17", "--offload-arch=gfx950", "-fPIC", "-ffp-contract=fast"]
 # Packed f32 instructions (v_pk_add/mul/fma_f32) are switched off: some of their forms have given wrong results on this

@@ -118,4 +118,33 @@ hipError_t launch_grad_norm(const uint64_t* addr, const int64_t* size, const int
 hipError_t launch_grad_scale(const uint64_t* addr, const int64_t* size, const int* bf16, int n, bool inf,
                              const double* partials, int npartials, double max_norm, float* norm, hipStream_t s);
 
+// differential attention (diff_attention.hip, diff_attention_bwd.hip); strides in elements, the last dimension dense
+struct DiffArgs {
+    const void *q, *k, *v;        // [batch, nq, heads, 2, d], [batch, nk, kv_heads, 2, d], [batch, nk, kv_heads, 2 d]
+    int64_t qs[4], ks[4], vs[3];  // strides: sample, token, head, map (v: sample, token, head)
+    const float* lam;             // f32 [4, lam_heads, d], lam_heads = 1 or heads
+    const int* key_lens;          // [batch] or nullptr
+    int batch, nq, nk, heads, kv_heads, group, d, lam_heads;   // group = heads / kv_heads
+    int causal;
+    float scale, lambda_init;
+};
+// forward: out [batch, nq, heads, 2 d]; for the backward also out2 (the second map's product with V, out's shape), lse
+// f32 [2, batch, heads, nq] and weight f32 [heads], or all three nullptr
+struct DiffOut {
+    void *out, *out2;
+    float *lse, *weight;
+};
+int64_t diff_attention_workspace(const DiffArgs& a, bool bf16);
+hipError_t launch_diff_attention(const DiffArgs& a, const DiffOut& o, float* ws, bool bf16, hipStream_t s);
+// backward: dq, dk, dv with the strides dqs, dks, dvs; dlam f32 [4, lam_heads, d]
+struct DiffGrads {
+    const void *out, *out2, *dout;   // [batch, nq, heads, 2 d]
+    const float *lse, *weight;
+    void *dq, *dk, *dv;
+    int64_t dqs[4], dks[4], dvs[3];
+    float* dlam;
+};
+int64_t diff_attention_bwd_workspace(const DiffArgs& a, bool bf16);
+hipError_t launch_diff_attention_backward(const DiffArgs& a, const DiffGrads& g, float* ws, bool bf16, hipStream_t s);
+
 }  // namespace vitk

@@ -6,7 +6,7 @@ VitkError for what they do not take; there is no CPU path.
 import torch
 
 from . import ops
-from .autograd import GroupNormFn
+from .autograd import DiffAttentionFn, GroupNormFn
 from .lib import VitkError
 
 
@@ -32,3 +32,24 @@ def group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, activation="none
         if _needs_grad(x, weight, bias):
             return GroupNormFn.apply(x, weight, bias, num_groups, eps, activation)
         return ops.group_norm(x, num_groups, weight, bias, eps, activation)[0]
+
+
+def diff_attention(q, k, v, lam, lambda_init=0.8, scale=None, key_lens=None, causal=False):
+    """Differential attention: per head h the difference of two softmax maps with a learned weight,
+
+        out[:, :, h] = (softmax(scale q_1 k_1^T) - w_h softmax(scale q_2 k_2^T)) v
+        w_h = exp(lam[0] . lam[1]) - exp(lam[2] . lam[3]) + lambda_init
+
+    q [B, Nq, H, 2, d], k [B, Nk, K, 2, d], v [B, Nk, K, 2d] (bf16 or f32; d a multiple of 8 up to 64; H a multiple of K,
+    query heads h * H / K ... share key head h), out [B, Nq, H, 2d].  Any strides in multiples of 16 bytes with a dense last
+    dimension: the fused projection's qkv [3, B, H, N, 2d] goes in as `qkv[i].view(B, H, N, 2, d).permute(0, 2, 1, 3, 4)`.
+    lam f32 [4, H, d], or [4, d] for all heads; scale defaults to d ** -0.5 and must be positive.
+    key_lens (int32 [B] on the device) hides the keys from key_lens[b] on: they are never read and get no gradient.  causal:
+    query t sees keys up to t + Nk - Nq (the last query all of them).  A row without a visible key gives 0 and no gradient.
+    Single query tokens against a long cache take a form that splits the keys.  Differentiable once in q, k, v and lam."""
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    with _on_device(q):
+        if _needs_grad(q, k, v, lam):
+            return DiffAttentionFn.apply(q, k, v, lam, lambda_init, scale, key_lens, causal)
+        return ops.diff_attention(q, k, v, lam, lambda_init, scale, key_lens, causal)[0]

@@ -57,6 +57,9 @@ SIGNATURES = {
     "vitk_ln_finalize": [_p, _p, _i, _i, _f, _p],
     "vitk_gemm_ln_bias_gelu": [_p, _p, _p, _p, _p, _p, _i, _i, _i, _p],
     "vitk_qkv_proj_ln": [_p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p],
+    "vitk_diff_attention": [_p, _p, _p, _p, _p, _i, _f, _f, _p, _i, _p, _p, _p, _p, _p, _i64, _i, _i, _i, _i, _i, _i, _i, _p],
+    "vitk_diff_attention_backward": [_p, _p, _p, _p, _p, _i, _f, _p, _i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64,
+                                     _i, _i, _i, _i, _i, _i, _i, _p],
     "vitk_group_norm": [_p, _p, _p, _p, _p, _p, _p, _i64, _i, _i, _i, _i, _f, _i, _i, _p],
     "vitk_group_norm_backward": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i, _i, _i, _i, _i, _i, _p],
     "vitk_grad_norm": [_p, _p, _p, _i, _i, _p, _i64, _p, _p],
@@ -66,6 +69,7 @@ SIGNATURES = {
 WORKSPACES = {
     "vitk_gemm_tn_workspace": [_i, _i, _i],
     "vitk_gemm_tn_colsum_workspace": [_i, _i, _i],
+    "vitk_diff_attention_workspace": [_i, _i, _i, _i, _i, _i, _i, _i],
     "vitk_group_norm_workspace": [_i, _i, _i, _i, _i, _i],
     "vitk_grad_norm_workspace": [_i],
 }

@@ -610,10 +610,103 @@ def colsum_static(g, out=None):
     return out
 
 
-# ---- group normalisation with an activation, channels last -----------------------------------------
+# ---- differential attention --------------------------------------------------------------------------
 
 _DTYPE_CODES = {torch.float32: _lib.VITK_F32, torch.bfloat16: _lib.VITK_BF16}
 
+
+def _scratch(floats, device):
+    # from torch's allocator, per call: it is the calling stream's (or the capturing graph's) own, whatever else runs
+    return torch.empty(floats, dtype=torch.float32, device=device)
+
+
+def _strides(*tensors):
+    """Host array of the element strides of all but the last dimension (0 where a dimension has one entry)."""
+    st = [s if n > 1 else 0 for t in tensors for s, n in zip(t.stride()[:-1], t.shape)]
+    return (_lib.ctypes.c_int64 * len(st))(*st)
+
+
+def _diff_sizes(q, k, v, lam, key_lens):
+    code = _DTYPE_CODES.get(q.dtype)
+    if code is None or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise _lib.VitkError(f"diff_attention: q, k and v must be bf16 or f32 alike, got {q.dtype}, {k.dtype}, {v.dtype}")
+    if q.dim() != 5 or k.dim() != 5 or v.dim() != 4:
+        raise _lib.VitkError(f"diff_attention: expected q [B,Nq,H,2,d], k [B,Nk,K,2,d], v [B,Nk,K,2d], got {tuple(q.shape)}, "
+                             f"{tuple(k.shape)}, {tuple(v.shape)}")
+    B, nq, H, two, d = q.shape
+    nk, K = k.shape[1], k.shape[2]
+    if two != 2 or tuple(k.shape) != (B, nk, K, 2, d) or tuple(v.shape) != (B, nk, K, 2 * d) or K < 1 or H % K:
+        raise _lib.VitkError(f"diff_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not match")
+    if lam.dtype != torch.float32 or not lam.is_contiguous() or tuple(lam.shape) not in ((4, d), (4, H, d)):
+        raise _lib.VitkError(f"diff_attention: lam must be contiguous f32 [4,{d}] or [4,{H},{d}], got {lam.dtype} {tuple(lam.shape)}")
+    if key_lens is not None and (key_lens.dtype != torch.int32 or tuple(key_lens.shape) != (B,) or not key_lens.is_contiguous()):
+        raise _lib.VitkError(f"diff_attention: key_lens must be contiguous int32 [{B}], got {key_lens.dtype} {tuple(key_lens.shape)}")
+    dev = q.get_device()
+    for n, t in (("q", q), ("k", k), ("v", v), ("lam", lam), ("key_lens", key_lens)):
+        if t is not None and (not t.is_cuda or t.get_device() != dev):
+            raise _lib.VitkError(f"diff_attention: {n} is on {t.device}, q on {q.device}")
+    if q.numel() and k.numel() and (q.stride(4) != 1 or k.stride(4) != 1 or v.stride(3) != 1):
+        raise _lib.VitkError("diff_attention: the last dimension of q, k and v must be dense")
+    return B, nq, nk, H, K, d, code
+
+
+def diff_attention(q, k, v, lam, lambda_init, scale, key_lens=None, causal=False, train=False):
+    """(out, out2, lse, weight): out [B, Nq, H, 2d] = (P_1 - w P_2) v; the rest is what the backward needs, None without
+    `train`.  Sizes with nothing to attend to give zeros."""
+    B, nq, nk, H, K, d, code = _diff_sizes(q, k, v, lam, key_lens)
+    out = torch.empty(B, nq, H, 2 * d, dtype=q.dtype, device=q.device)
+    if q.numel() == 0 or k.numel() == 0:
+        return out.zero_(), None, None, None
+    L = _lib.load()
+    out2 = lse = weight = None
+    if train:
+        out2 = torch.empty_like(out)
+        lse = torch.empty(2, B, H, nq, dtype=torch.float32, device=q.device)
+        weight = torch.empty(H, dtype=torch.float32, device=q.device)
+    n = L.vitk_diff_attention_workspace(B, nq, nk, H, K, d, code, 0)
+    ws = _scratch(n, q.device) if n > 0 else None
+    with _span("diff_attention"):
+        _lib.check(L.vitk_diff_attention(_ptr(q), _ptr(k), _ptr(v), _strides(q, k, v), _ptr(lam), 1 if lam.dim() == 2 else H,
+                                         float(lambda_init), float(scale), _ptr(key_lens), int(causal), _ptr(out), _ptr(out2),
+                                         _ptr(lse), _ptr(weight), _ptr(ws), max(n, 0), B, nq, nk, H, K, d, code, _stream()), L)
+    return out, out2, lse, weight
+
+
+def _grad_like(t):
+    g = torch.empty_like(t)                       # keeps the order of a dense tensor's dimensions
+    return g if g.stride(-1) == 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+def diff_attention_backward(q, k, v, lam, scale, key_lens, causal, out, out2, lse, weight, dout, lam_grad=True):
+    """(dq, dk, dv, dlam) of diff_attention(); dlam None without `lam_grad`."""
+    B, nq, nk, H, K, d, code = _diff_sizes(q, k, v, lam, key_lens)
+    dq, dk, dv = _grad_like(q), _grad_like(k), _grad_like(v)
+    dlam = torch.empty_like(lam) if lam_grad else None
+    if q.numel() == 0 or k.numel() == 0:
+        return dq.zero_(), dk.zero_(), dv.zero_(), None if dlam is None else dlam.zero_()
+    L = _lib.load()
+    for n, t in (("out", out), ("out2", out2), ("dout", dout)):
+        _chk(t, q.dtype, n)
+        if tuple(t.shape) != (B, nq, H, 2 * d):
+            raise _lib.VitkError(f"diff_attention_backward: {n} {tuple(t.shape)} vs [{B},{nq},{H},{2 * d}]")
+    _chk(lse, torch.float32, "lse")
+    _chk(weight, torch.float32, "weight")
+    if lse.numel() != 2 * B * H * nq or weight.numel() != H:
+        raise _lib.VitkError(f"diff_attention_backward: lse {tuple(lse.shape)}, weight {tuple(weight.shape)}")
+    n = L.vitk_diff_attention_workspace(B, nq, nk, H, K, d, code, 1)
+    if n < 0:
+        raise _lib.VitkError(f"diff_attention_backward: unsupported sizes q {tuple(q.shape)}, k {tuple(k.shape)}")
+    ws = _scratch(n, q.device)
+    with _span("diff_attention_backward"):
+        _lib.check(L.vitk_diff_attention_backward(_ptr(q), _ptr(k), _ptr(v), _strides(q, k, v), _ptr(lam),
+                                                  1 if lam.dim() == 2 else H, float(scale), _ptr(key_lens), int(causal),
+                                                  _ptr(out), _ptr(out2), _ptr(lse), _ptr(weight), _ptr(dout), _ptr(dq), _ptr(dk),
+                                                  _ptr(dv), _strides(dq, dk, dv), _ptr(dlam), _ptr(ws), n, B, nq, nk, H, K, d,
+                                                  code, _stream()), L)
+    return dq, dk, dv, dlam
+
+
+# ---- group normalisation with an activation, channels last -----------------------------------------
 
 def _gn_sizes(x, num_groups, weight, bias, activation):
     if x.dtype not in _DTYPE_CODES:
@@ -634,11 +727,6 @@ def _gn_sizes(x, num_groups, weight, bias, activation):
             if t.device != x.device:
                 raise _lib.VitkError(f"group_norm: {n} is on {t.device}, x on {x.device}")
     return B, (x.numel() // (B * C) if B * C else 0), C
-
-
-def _scratch(floats, device):
-    # from torch's allocator, per call: it is the calling stream's (or the capturing graph's) own, whatever else runs
-    return torch.empty(floats, dtype=torch.float32, device=device)
 
 
 def group_norm(x, num_groups, weight, bias, eps, activation="none", stats=False):
