@@ -338,10 +338,10 @@ int vitk_qkv_proj_ln(const void* A, const void* Wg, const float* ab, const float
 int64_t vitk_diff_attention_workspace(int batch, int nq, int nk, int heads, int kv_heads, int d, int dtype, int backward);
 
 /* out [batch, nq, heads, 2 d] in q's type, contiguous.  For the backward also, together or all NULL: out2 (the second
- * map's sum P_2 v, out's shape), lse f32 [2, batch, heads, nq] (log2 of the denominators of exp(scale s)) and weight f32
- * [heads]. */
+ * map's sum P_2 v, out's shape), stats f32 [4, batch, heads, nq] (per map a reference point m, then per map
+ * 1 / sum of exp2(scale log2(e) s - m)) and weight f32 [heads]. */
 int vitk_diff_attention(const void* q, const void* k, const void* v, const int64_t* strides, const float* lam, int lam_heads,
-                        float lambda_init, float scale, const int* key_lens, int causal, void* out, void* out2, float* lse,
+                        float lambda_init, float scale, const int* key_lens, int causal, void* out, void* out2, float* stats,
                         float* weight, float* workspace, int64_t workspace_floats, int batch, int nq, int nk, int heads,
                         int kv_heads, int d, int dtype, void* stream);
 
@@ -350,7 +350,7 @@ int vitk_diff_attention(const void* q, const void* k, const void* v, const int64
  * results are reproducible. */
 int vitk_diff_attention_backward(const void* q, const void* k, const void* v, const int64_t* strides, const float* lam,
                                  int lam_heads, float scale, const int* key_lens, int causal, const void* out, const void* out2,
-                                 const float* lse, const float* weight, const void* dout, void* dq, void* dk, void* dv,
+                                 const float* stats, const float* weight, const void* dout, void* dq, void* dk, void* dv,
                                  const int64_t* grad_strides, float* dlam, float* workspace, int64_t workspace_floats, int batch,
                                  int nq, int nk, int heads, int kv_heads, int d, int dtype, void* stream);
 

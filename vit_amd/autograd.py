@@ -309,16 +309,16 @@ class DiffAttentionFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, lam, lambda_init, scale, key_lens, causal):
-        out, out2, lse, weight = ops.diff_attention(q, k, v, lam, lambda_init, scale, key_lens, causal, train=True)
-        ctx.save_for_backward(q, k, v, lam, key_lens, out, out2, lse, weight)
+        out, out2, stats, weight = ops.diff_attention(q, k, v, lam, lambda_init, scale, key_lens, causal, train=True)
+        ctx.save_for_backward(q, k, v, lam, key_lens, out, out2, stats, weight)
         ctx.scale, ctx.causal = scale, causal
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        q, k, v, lam, key_lens, out, out2, lse, weight = ctx.saved_tensors
-        dq, dk, dv, dlam = ops.diff_attention_backward(q, k, v, lam, ctx.scale, key_lens, ctx.causal, out, out2, lse, weight,
+        q, k, v, lam, key_lens, out, out2, stats, weight = ctx.saved_tensors
+        dq, dk, dv, dlam = ops.diff_attention_backward(q, k, v, lam, ctx.scale, key_lens, ctx.causal, out, out2, stats, weight,
                                                        g.contiguous(), lam_grad=ctx.needs_input_grad[3])
         return dq, dk, dv, dlam, None, None, None, None
 

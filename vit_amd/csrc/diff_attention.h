@@ -16,7 +16,6 @@ namespace diff {
 typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
 
 constexpr float kNoScore = -1.0e30f;       // the running maximum before the first key
-constexpr float kNoKeys = 1.0e30f;         // log2 of the denominator of a row without keys: exp2(s - kNoKeys) = 0
 constexpr float kLog2e = 1.44269504088896340736f;
 
 template <class T>
@@ -175,14 +174,24 @@ __device__ __forceinline__ int key_limit(const DiffArgs& a, int len, int tok) {
     return lim < len ? (lim > 0 ? lim : 0) : len;
 }
 
-// w_h = exp(lam0 . lam1) - exp(lam2 . lam3) + lambda_init; both half-waves share the sums of a lane's head
+// w_h = exp(lam0 . lam1) - exp(lam2 . lam3) + lambda_init; the half-waves share the sums of a lane's head, all loads at once
+template <int DP>
 __device__ __forceinline__ float map_weight(const DiffArgs& a, int head, int hh) {
     const float* p = a.lam + (a.lam_heads == 1 ? 0 : (int64_t)head * a.d);
     const int64_t vs = (int64_t)a.lam_heads * a.d;
     float s1 = 0.f, s2 = 0.f;
-    for (int e = hh; e < a.d; e += 2) {
-        s1 = fmaf(p[e], p[vs + e], s1);
-        s2 = fmaf(p[2 * vs + e], p[3 * vs + e], s2);
+#pragma unroll
+    for (int t = 0; t < DP / 8; ++t) {
+        if (8 * t >= a.d) break;
+        const f32x4* e = reinterpret_cast<const f32x4*>(p + 8 * t + 4 * hh);
+        const f32x4 x = e[0], y = *reinterpret_cast<const f32x4*>(p + vs + 8 * t + 4 * hh);
+        const f32x4 z = *reinterpret_cast<const f32x4*>(p + 2 * vs + 8 * t + 4 * hh);
+        const f32x4 u = *reinterpret_cast<const f32x4*>(p + 3 * vs + 8 * t + 4 * hh);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            s1 = fmaf(x[j], y[j], s1);
+            s2 = fmaf(z[j], u[j], s2);
+        }
     }
     return expf(both_sum(s1)) - expf(both_sum(s2)) + a.lambda_init;
 }

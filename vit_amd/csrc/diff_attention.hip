@@ -129,7 +129,7 @@ __global__ __launch_bounds__(NW * 64, KEYS || sizeof(T) == 4 ? 1 : 2) void diff_
                 qf[m][t] = *reinterpret_cast<const Chunk*>(c < dc ? (const void*)(qg + m * a.qs[3] + c * PER) : (const void*)kZeros);
             }
     }
-    const float weight = map_weight(a, place.head, hh);
+    const float weight = map_weight<DP>(a, place.head, hh);
 
     f32x16 acc[2][DB];
     float m_run[2] = {kNoScore, kNoScore}, l_run[2] = {0.f, 0.f};
@@ -231,9 +231,10 @@ __global__ __launch_bounds__(NW * 64, KEYS || sizeof(T) == 4 ? 1 : 2) void diff_
                 if (out2) store4(out2 + orow + col, y);
             }
         if (out2 && hh == 0) {
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
-                o.lse[m * lmap + lrow] = l_tot[m] == 0.f ? kNoKeys : m_run[m] + __builtin_amdgcn_logf(l_tot[m]);
+            o.stats[lrow] = l_tot[0] == 0.f ? 0.f : m_run[0];
+            o.stats[lmap + lrow] = l_tot[1] == 0.f ? 0.f : m_run[1];
+            o.stats[2 * lmap + lrow] = i1;
+            o.stats[3 * lmap + lrow] = i2;
             if (b == 0 && place.tok == 0) o.weight[place.head] = weight;
         }
     } else {
@@ -321,8 +322,10 @@ __global__ __launch_bounds__(NW * 64, KEYS || sizeof(T) == 4 ? 1 : 2) void diff_
                 ml[3] = sum[1];
             } else if (out2) {
 #pragma unroll
-                for (int m = 0; m < 2; ++m)
-                    o.lse[m * lmap + lrow] = sum[m] == 0.f ? kNoKeys : top[m] + __builtin_amdgcn_logf(sum[m]);
+                for (int m = 0; m < 2; ++m) {
+                    o.stats[m * lmap + lrow] = sum[m] == 0.f ? 0.f : top[m];
+                    o.stats[(2 + m) * lmap + lrow] = sum[m] == 0.f ? 0.f : 1.0f / sum[m];
+                }
                 if (b == 0 && place.tok == 0) o.weight[place.head] = weight;
             }
         }
@@ -353,11 +356,12 @@ __global__ __launch_bounds__(256) void diff_fwd_join(DiffArgs a, DiffOut o, cons
         }
         s_top[hh][r] = top;
         s_inv[hh][r] = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
-        const float w = map_weight(a, pl.head, hh);
+        const float w = map_weight<DV / 2>(a, pl.head, hh);
         if (hh == 0) s_w[r] = w;
         if (o.out2 && r < live) {
-            o.lse[((int64_t)hh * a.batch * a.heads + (int64_t)b * a.heads + pl.head) * a.nq + pl.tok] =
-                sum == 0.f ? kNoKeys : top + __builtin_amdgcn_logf(sum);
+            const int64_t lmap = (int64_t)a.batch * a.heads * a.nq, at = ((int64_t)b * a.heads + pl.head) * a.nq + pl.tok;
+            o.stats[hh * lmap + at] = sum == 0.f ? 0.f : top;
+            o.stats[(2 + hh) * lmap + at] = s_inv[hh][r];
             if (b == 0 && pl.tok == 0 && hh == 0) o.weight[pl.head] = w;
         }
     }

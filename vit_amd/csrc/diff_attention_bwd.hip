@@ -1,5 +1,6 @@
 // Differential attention, backward (gfx950 / CDNA4).  With P_m rebuilt from the scores and the forward's denominators
-// (P_m = exp2(scale log2(e) q_m . k_m - lse_m)):
+// (P_m = exp2(scale log2(e) q_m . k_m - m_m) / l_m with the reference point and the sum that the forward leaves: the
+// exponent is small where the probability is large, so a probability is exact to a few 2^-24):
 //     dA   = dO V^T                         the gradient of P_1 - w P_2
 //     D_m  = sum over keys of P_m dA = dO . (P_m V):   D_2 = dO . O_2,  D_1 = dO . O + w D_2
 //     dS_1 = P_1 (dA - D_1),  dS_2 = -w P_2 (dA - D_2)
@@ -11,6 +12,13 @@
 #include <type_traits>
 
 #include "diff_attention.h"
+
+#ifndef KVOCC
+#define KVOCC 1
+#endif
+#ifndef KVRC
+#define KVRC 32
+#endif
 
 namespace vitk {
 
@@ -103,7 +111,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void diff_bwd_q(DiffAr
     const int64_t lrow = ((int64_t)b * a.heads + place.head) * a.nq + place.tok;
     const int64_t lmap = (int64_t)a.batch * a.heads * a.nq;
     const float weight = g.weight[place.head];
-    const float lse[2] = {g.lse[lrow], g.lse[lmap + lrow]};
+    const float ref[2] = {g.stats[lrow], g.stats[lmap + lrow]};
+    const float inv[2] = {g.stats[2 * lmap + lrow], g.stats[3 * lmap + lrow]};
 
     Chunk qf[2][KT], of[2 * KT];
     float dd[2];
@@ -170,8 +179,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void diff_bwd_q(DiffAr
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const float p1 = __builtin_amdgcn_exp2f(fmaf(s[0][i], sc, -lse[0]));
-                const float p2 = __builtin_amdgcn_exp2f(fmaf(s[1][i], sc, -lse[1]));
+                const float p1 = __builtin_amdgcn_exp2f(fmaf(s[0][i], sc, -ref[0]));       // times 1 / l at the end
+                const float p2 = __builtin_amdgcn_exp2f(fmaf(s[1][i], sc, -ref[1]));
                 dw = fmaf(p2, da[i], dw);
                 s[0][i] = p1 * (da[i] - dd[0]);
                 s[1][i] = p2 * (da[i] - dd[1]);
@@ -194,7 +203,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void diff_bwd_q(DiffAr
         __syncthreads();
     }
 
-    dw = both_sum(dw);
+    dw = both_sum(dw) * inv[1];
     if (hh == 0) s_dw[wave * 32 + r] = row < nrows ? -dw : 0.f;
     __syncthreads();
     for (int h = tid; h < a.group; h += 256) {
@@ -208,7 +217,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void diff_bwd_q(DiffAr
     T* out = reinterpret_cast<T*>(g.dq) + b * g.dqs[0] + place.tok * g.dqs[1] + place.head * g.dqs[2];
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-        const float f = m == 0 ? a.scale : -weight * a.scale;
+        const float f = m == 0 ? inv[0] * a.scale : -weight * inv[1] * a.scale;
 #pragma unroll
         for (int e = 0; e < EB; ++e)
 #pragma unroll
@@ -222,17 +231,17 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void diff_bwd_q(DiffAr
 }
 
 // dK and dV of 128 keys
-template <class T, int DP>
-__global__ __launch_bounds__(256, 1) void diff_bwd_kv(DiffArgs a, DiffGrads g, const float* __restrict__ ws_d, int tiles) {
+template <class T, int DP, int RC>
+__global__ __launch_bounds__(256, KVOCC) void diff_bwd_kv(DiffArgs a, DiffGrads g, const float* __restrict__ ws_d, int tiles) {
     constexpr int DV = 2 * DP;
     constexpr int RB = row_bytes<T, DV>();
     constexpr int PER = Op<T>::kPer;
     constexpr int DPC = DP / PER, KT = DPC / 2;
     constexpr int DB = DV / 32, EB = (DP + 31) / 32;
-    constexpr int RC = 32, TILE = RC * RB;                            // rows of a chunk
+    constexpr int TILE = RC * RB;                                     // RC: rows of a chunk
     typedef typename Op<T>::Chunk Chunk;
     __shared__ __align__(16) char bufs[2][2 * TILE];                  // Q of both maps, dO
-    __shared__ __align__(16) float s_row[2][5][RC];                   // lse_1, lse_2, D_1, D_2, w of the rows
+    __shared__ __align__(16) float s_row[2][6][RC];                   // m_1, m_2, 1 / l_1, w / l_2, D_1, D_2 of the rows
     __shared__ __align__(16) int s_lim[2][RC];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -264,7 +273,7 @@ __global__ __launch_bounds__(256, 1) void diff_bwd_kv(DiffArgs a, DiffGrads g, c
     const T* og = reinterpret_cast<const T*>(g.dout) + (int64_t)b * a.nq * a.heads * 2 * a.d + s_c * PER;
     const int64_t lmap = (int64_t)a.batch * a.heads * a.nq;
     u32x4 held[PASSES];
-    float held_r[5];
+    float held_r[6];
     int held_l = 0;
     auto fetch = [&](int c) {
 #pragma unroll
@@ -280,16 +289,17 @@ __global__ __launch_bounds__(256, 1) void diff_bwd_kv(DiffArgs a, DiffGrads g, c
         if (tid < RC) {
             const int row = c * RC + tid;
             held_l = 0;
-            held_r[0] = held_r[1] = kNoKeys;
-            held_r[2] = held_r[3] = held_r[4] = 0.f;
+#pragma unroll
+            for (int j = 0; j < 6; ++j) held_r[j] = 0.f;
             if (row < nrows) {
                 const RowPlace pl = row_place(a, kh, row);
                 const int64_t at = ((int64_t)b * a.heads + pl.head) * a.nq + pl.tok;
-                held_r[0] = g.lse[at];
-                held_r[1] = g.lse[lmap + at];
-                held_r[2] = ws_d[at];
-                held_r[3] = ws_d[lmap + at];
-                held_r[4] = g.weight[pl.head];
+                held_r[0] = g.stats[at];
+                held_r[1] = g.stats[lmap + at];
+                held_r[2] = g.stats[2 * lmap + at];
+                held_r[3] = g.stats[3 * lmap + at] * g.weight[pl.head];
+                held_r[4] = ws_d[at];
+                held_r[5] = ws_d[lmap + at];
                 held_l = key_limit(a, len, pl.tok);
             }
         }
@@ -304,7 +314,7 @@ __global__ __launch_bounds__(256, 1) void diff_bwd_kv(DiffArgs a, DiffGrads g, c
         }
         if (tid < RC) {
 #pragma unroll
-            for (int j = 0; j < 5; ++j) s_row[k][j][tid] = held_r[j];
+            for (int j = 0; j < 6; ++j) s_row[k][j][tid] = held_r[j];
             s_lim[k][tid] = held_l;
         }
     };
@@ -338,6 +348,55 @@ __global__ __launch_bounds__(256, 1) void diff_bwd_kv(DiffArgs a, DiffGrads g, c
     for (int d = 0; d < DB; ++d) dv[d] = zero16();
     const float sc = a.scale * kLog2e;
 
+    auto work = [&](const char* qt, const char* ot, int k, int rb, bool masked) {
+                    f32x16 s[2], da = zero16();
+        #pragma unroll
+                    for (int m = 0; m < 2; ++m) {
+                        s[m] = zero16();
+        #pragma unroll
+                        for (int t = 0; t < KT; ++t) s[m] = Op<T>::mma(chunk_at<T, RB>(qt, rb + r, m * DPC + 2 * t + hh), kf[m][t], s[m]);
+                    }
+        #pragma unroll
+                    for (int t = 0; t < 2 * KT; ++t) da = Op<T>::mma(chunk_at<T, RB>(ot, rb + r, 2 * t + hh), vf[t], da);
+                    f32x16 pa;
+        #pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int at = rb + 8 * q + 4 * hh;
+                        auto row4 = [&](int j) { return *reinterpret_cast<const f32x4*>(&s_row[k][j][at]); };
+                        const f32x4 m1 = row4(0), m2 = row4(1), i1 = row4(2), w2 = row4(3), d1 = row4(4), d2 = row4(5);
+        #pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int i = 4 * q + j;
+                            float p1 = __builtin_amdgcn_exp2f(fmaf(s[0][i], sc, -m1[j])) * i1[j];
+                            float wp2 = __builtin_amdgcn_exp2f(fmaf(s[1][i], sc, -m2[j])) * w2[j];
+                            if (masked && key >= s_lim[k][at + j]) p1 = wp2 = 0.f;
+                            pa[i] = p1 - wp2;
+                            s[0][i] = p1 * (da[i] - d1[j]);
+                            s[1][i] = wp2 * (d2[j] - da[i]);
+                        }
+                    }
+        #pragma unroll
+                    for (int st = 0; st < 2; ++st) {
+                        Slice<T> p, d0, d1;
+                        p.take(pa, st);
+                        d0.take(s[0], st);
+                        d1.take(s[1], st);
+        #pragma unroll
+                        for (int d = 0; d < DB; ++d) {
+                            Trans<T, RB> o;
+                            o.load(ot, rb + 16 * st, d * 32, lane);
+                            dv[d] = mma_t(o, p, dv[d]);
+                        }
+        #pragma unroll
+                        for (int e = 0; e < EB; ++e) {
+                            Trans<T, RB> q0, q1;
+                            q0.load(qt, rb + 16 * st, e * 32, lane);
+                            q1.load(qt, rb + 16 * st, DP + e * 32, lane);
+                            dk[0][e] = mma_t(q0, d0, dk[0][e]);
+                            dk[1][e] = mma_t(q1, d1, dk[1][e]);
+                        }
+                    }
+    };
     if (first < c1) put(0);
     __syncthreads();
     for (int c = first; c < c1; ++c) {
@@ -346,59 +405,13 @@ __global__ __launch_bounds__(256, 1) void diff_bwd_kv(DiffArgs a, DiffGrads g, c
         const char* ot = qt + TILE;
         const bool more = c + 1 < c1;
         if (more) fetch(c + 1);
-        // the chunk's last row sees most: nothing to do where that is below the wave's keys
-        const int last = (c + 1) * RC < nrows ? (c + 1) * RC : nrows;
-        const int most = key_limit(a, len, row_place(a, kh, last - 1).tok), least = key_limit(a, len, row_place(a, kh, c * RC).tok);
-        if (key0 < most) {
-            f32x16 s[2], da = zero16();
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                s[m] = zero16();
-#pragma unroll
-                for (int t = 0; t < KT; ++t) s[m] = Op<T>::mma(chunk_at<T, RB>(qt, r, m * DPC + 2 * t + hh), kf[m][t], s[m]);
-            }
-#pragma unroll
-            for (int t = 0; t < 2 * KT; ++t) da = Op<T>::mma(chunk_at<T, RB>(ot, r, 2 * t + hh), vf[t], da);
-            f32x16 pa;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int at = 8 * q + 4 * hh;
-                const f32x4 l1 = *reinterpret_cast<const f32x4*>(&s_row[k][0][at]), l2 = *reinterpret_cast<const f32x4*>(&s_row[k][1][at]);
-                const f32x4 d1 = *reinterpret_cast<const f32x4*>(&s_row[k][2][at]), d2 = *reinterpret_cast<const f32x4*>(&s_row[k][3][at]);
-                const f32x4 w4 = *reinterpret_cast<const f32x4*>(&s_row[k][4][at]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int i = 4 * q + j;
-                    float p1 = __builtin_amdgcn_exp2f(fmaf(s[0][i], sc, -l1[j]));
-                    float p2 = __builtin_amdgcn_exp2f(fmaf(s[1][i], sc, -l2[j]));
-                    if (key0 + 32 > least && key >= s_lim[k][at + j]) p1 = p2 = 0.f;
-                    const float wp2 = w4[j] * p2;
-                    pa[i] = p1 - wp2;
-                    s[0][i] = p1 * (da[i] - d1[j]);
-                    s[1][i] = -wp2 * (da[i] - d2[j]);
-                }
-            }
-#pragma unroll
-            for (int st = 0; st < 2; ++st) {
-                Slice<T> p, d0, d1;
-                p.take(pa, st);
-                d0.take(s[0], st);
-                d1.take(s[1], st);
-#pragma unroll
-                for (int d = 0; d < DB; ++d) {
-                    Trans<T, RB> o;
-                    o.load(ot, 16 * st, d * 32, lane);
-                    dv[d] = mma_t(o, p, dv[d]);
-                }
-#pragma unroll
-                for (int e = 0; e < EB; ++e) {
-                    Trans<T, RB> q0, q1;
-                    q0.load(qt, 16 * st, e * 32, lane);
-                    q1.load(qt, 16 * st, DP + e * 32, lane);
-                    dk[0][e] = mma_t(q0, d0, dk[0][e]);
-                    dk[1][e] = mma_t(q1, d1, dk[1][e]);
-                }
-            }
+        for (int rb = 0; rb < RC; rb += 32) {
+            // the block's last row sees most: nothing to do where that is below the wave's keys
+            const int at0 = c * RC + rb, last = at0 + 32 < nrows ? at0 + 32 : nrows;
+            const int most = at0 < nrows ? key_limit(a, len, row_place(a, kh, last - 1).tok) : 0;
+            const int least = at0 < nrows ? key_limit(a, len, row_place(a, kh, at0).tok) : 0;
+            if (key0 < most) work(qt, ot, k, rb, key0 + 32 > least);
         }
         if (more) put(k ^ 1);
         __syncthreads();
@@ -478,7 +491,7 @@ hipError_t launch(const DiffArgs& a, const DiffGrads& g, float* ws, hipStream_t 
     hipLaunchKernelGGL((diff_bwd_q<T, DP>), dim3((int)(bks * qt)), dim3(256), 0, s, a, g, ws_d, ws_w, qt);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((diff_bwd_kv<T, DP>), dim3((int)(bks * kt)), dim3(256), 0, s, a, g, ws_d, kt);
+    hipLaunchKernelGGL((diff_bwd_kv<T, DP, KVRC>), dim3((int)(bks * kt)), dim3(256), 0, s, a, g, ws_d, kt);
     e = hipGetLastError();
     if (e != hipSuccess || !g.dlam) return e;
     hipLaunchKernelGGL(diff_bwd_lam, dim3(a.lam_heads), dim3(256), 0, s, a, ws_w, qt, g.dlam);

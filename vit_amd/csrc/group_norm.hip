@@ -11,9 +11,14 @@
 // runs of a pixel's channels; statistics are kept per channel and put together into groups only at the end of a
 // workgroup, which leaves the group width free (any divisor of the channels).
 //
-// Statistics are first and second moments about the lane's first value, merged pairwise by
-//     M2 = M2a + M2b + (mean_b - mean_a)^2 na nb / (na + nb),
-// all in f32: no cancellation where the mean is large against the deviation, as sums of squares would have.
+// Two forms.  Where the channels of some whole groups over all pixels of a sample fit one workgroup's registers (rows of 64
+// bytes at least), it reads them once, does everything and writes the result.  Else two passes: one leaves the moments of
+// every chunk of pixels, the next one puts them together again in every workgroup (a few hundred values) and applies them.
+//
+// All statistics in f32, without the cancellation that sums of squares have where the mean is large against the deviation:
+// lanes add first and second moments about their first value, moments of parts are joined about a mean of their own.
+#include <type_traits>
+
 #include "vitk_common.h"
 #include "vitk_kernels.h"
 
@@ -21,29 +26,24 @@ namespace vitk {
 
 namespace {
 
-constexpr int kT = 256;                 // threads of the two-pass kernels
+constexpr int kT = 256;       // threads of the two-pass kernels
 
 struct Mom {
     float n, mean, m2;
 };
 
-__device__ __forceinline__ Mom merge(const Mom& a, const Mom& b) {
-    if (b.n == 0.f) return a;
-    if (a.n == 0.f) return b;
-    const float n = a.n + b.n;
-    const float f = b.n / n, d = b.mean - a.mean;
-    return Mom{n, fmaf(d, f, a.mean), a.m2 + b.m2 + d * d * a.n * f};
+// sum over L neighbouring lanes (a power of two), in every lane of them
+__device__ __forceinline__ float lanes_sum(float v, int L) {
+    for (int o = L >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
 }
 
-__device__ __forceinline__ Mom wave_merge(Mom m) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        // both partners merge in the same order, so that all lanes end with the same bits
-        const Mom p = {__shfl_xor(m.n, o, 64), __shfl_xor(m.mean, o, 64), __shfl_xor(m.m2, o, 64)};
-        const bool low = (threadIdx.x & o) == 0;
-        m = low ? merge(m, p) : merge(p, m);
-    }
-    return m;
+// f(group, lane of it) for ng groups by the workgroup's threads, L neighbouring lanes to a group (power of two up to 64);
+// every lane of a wave makes every call, with group < ng or not
+template <int NT, class F>
+__device__ __forceinline__ void by_groups(int ng, int L, F&& f) {
+    const int per = NT / L;
+    for (int g = 0; g < ng; g += per) f(g + (int)threadIdx.x / L, (int)threadIdx.x & (L - 1));
 }
 
 // V values of T: raw registers and their f32 values
@@ -122,6 +122,7 @@ struct Geometry {
     int slabs;                // slabs of cv * V channels (the last one may be short)
     int chunk;                // pixels of a workgroup
     int chunks;
+    int L;                    // lanes that put a group together
 };
 
 // ---- forward, two passes over x ------------------------------------------------------------------------------
@@ -186,41 +187,63 @@ __global__ __launch_bounds__(kT) void gn_moments(const T* __restrict__ x, Mom* _
     }
     __syncthreads();
     const int g0 = c0 / q.Cg, g1 = (c0 + wc - 1) / q.Cg;
-    const int lane = tid & 63;
     Mom* out = part + (((int64_t)b * q.chunks + blockIdx.x) * q.slabs + slab) * q.G;
-    for (int g = g0 + (tid >> 6); g <= g1; g += kT / 64) {
-        const int lo = max(g * q.Cg - c0, 0), hi = min((g + 1) * q.Cg - c0, wc);
-        const int w = hi - lo;
-        Mom m = {0.f, 0.f, 0.f};
-        for (int i = lane; i < rows * w; i += 64) {
-            const int r = i / w, c = lo + i - r * w;
-            const int len = s1 - s0 - r;
-            const float n = len > 0 ? (float)((len + rows - 1) / rows) : 0.f;
-            m = merge(m, Mom{n, s_mean[r * wc + c], s_m2[r * wc + c]});
+    const int len = s1 - s0;
+    by_groups<kT>(g1 - g0 + 1, q.L, [&](int gi, int l) {
+        const int g = g0 + gi;
+        const bool on = g <= g1;
+        const int lo = on ? max(g * q.Cg - c0, 0) : 0, hi = on ? min((g + 1) * q.Cg - c0, wc) : 0;
+        const int live = min(rows, len);                             // rows that hold a pixel
+        const float m0 = s_mean[lo], total = (float)len * (float)(hi - lo);
+        float t = 0.f;
+        for (int r = 0; r < live; ++r) {
+            const float n = (float)((len - r + rows - 1) / rows);
+            for (int c = lo + l; c < hi; c += q.L) t = fmaf(n, s_mean[r * wc + c] - m0, t);
         }
-        m = wave_merge(m);
-        if (lane == 0) out[g] = m;
-    }
+        const float mean = m0 + lanes_sum(t, q.L) / total;
+        t = 0.f;
+        for (int r = 0; r < live; ++r) {
+            const float n = (float)((len - r + rows - 1) / rows);
+            for (int c = lo + l; c < hi; c += q.L) {
+                const float d = s_mean[r * wc + c] - mean;
+                t += fmaf(n * d, d, s_m2[r * wc + c]);
+            }
+        }
+        t = lanes_sum(t, q.L);
+        if (on && l == 0) out[g] = Mom{total, mean, t};
+    });
 }
 
-// mean and rstd of the groups g0..g1 of sample b from the partial moments, into shared memory (index g - g0)
+// mean and rstd of the groups g0..g1 of sample b from the partial moments, into shared memory (index g - g0).  The parts'
+// moments are taken about the first part's mean; what that mean is off by counts at most (parts) times in the deviation,
+// since the first part's own share of it does.
 __device__ __forceinline__ void merge_groups(const Mom* __restrict__ part, const Geometry& q, int V, int b, int g0, int g1,
                                              float eps, float* s_mean, float* s_rstd) {
-    const int lane = threadIdx.x & 63, nw = blockDim.x >> 6;
-    for (int g = g0 + (threadIdx.x >> 6); g <= g1; g += nw) {
+    by_groups<kT>(g1 - g0 + 1, q.L, [&](int gi, int l) {
+        const bool on = g0 + gi <= g1;
+        const int g = on ? g0 + gi : g1;
         const int first = (g * q.Cg) / (q.cv * V), last = ((g + 1) * q.Cg - 1) / (q.cv * V);   // slabs that touch the group
         const int ns = last - first + 1;
-        Mom m = {0.f, 0.f, 0.f};
-        for (int i = lane; i < q.chunks * ns; i += 64) {
-            const int ch = i / ns, sl = first + i - ch * ns;
-            m = merge(m, part[(((int64_t)b * q.chunks + ch) * q.slabs + sl) * q.G + g]);
+        const Mom* p = part + ((int64_t)b * q.chunks * q.slabs + first) * q.G + g;
+        const float m0 = p->mean;
+        float n = 0.f, t1 = 0.f, t2 = 0.f;
+        for (int i = l; i < q.chunks * ns; i += q.L) {
+            const int ch = ns == 1 ? i : i / ns, sl = i - ch * ns;
+            const Mom m = p[((int64_t)ch * q.slabs + sl) * q.G];
+            const float d = m.mean - m0;
+            n += m.n;
+            t1 = fmaf(m.n, d, t1);
+            t2 += fmaf(m.n * d, d, m.m2);
         }
-        m = wave_merge(m);
-        if (lane == 0) {
-            s_mean[g - g0] = m.mean;
-            s_rstd[g - g0] = rsqrtf(m.m2 / m.n + eps);
+        n = lanes_sum(n, q.L);
+        t1 = lanes_sum(t1, q.L) / n;
+        t2 = lanes_sum(t2, q.L) / n;
+        if (on && l == 0) {
+            s_mean[gi] = m0 + t1;
+            const float var = t2 - t1 * t1;
+            s_rstd[gi] = rsqrtf((var > 0.f || var != var ? var : 0.f) + eps);
         }
-    }
+    });
 }
 
 template <class T, int V, int ACT>
@@ -236,6 +259,19 @@ __global__ __launch_bounds__(kT) void gn_apply(const T* __restrict__ x, const Mo
     const int c0 = slab * q.cv * V;
     const int wc = min(q.cv * V, q.C - c0);
     const int g0 = c0 / q.Cg, g1 = (c0 + wc - 1) / q.Cg;
+    // the last chunks first: the moments' pass has read them last; the first values are on their way while the groups are
+    // put together
+    const int ch = q.chunks - 1 - blockIdx.x;
+    const int s0 = ch * q.chunk, s1 = min(s0 + q.chunk, q.S);
+    const int64_t base = ((int64_t)b * q.S) * q.C + c0 + col * V;
+    const bool live = row < rows && col * V < wc;
+    constexpr int U = 4;
+    Raw<T, V> ahead[U];
+    if (live) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (s0 + row + u * rows < s1) ahead[u].load(x + base + (int64_t)(s0 + row + u * rows) * q.C);
+    }
     merge_groups(part, q, V, b, g0, g1, eps, s_mean, s_rstd);
     __syncthreads();
     if (mean_out && blockIdx.x == 0)
@@ -243,7 +279,7 @@ __global__ __launch_bounds__(kT) void gn_apply(const T* __restrict__ x, const Mo
             mean_out[b * q.G + g] = s_mean[g - g0];         // a group of several slabs is written by each, the same bits
             rstd_out[b * q.G + g] = s_rstd[g - g0];
         }
-    if (row >= rows || col * V >= wc) return;
+    if (!live) return;
     float mu[V], a[V], sh[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -252,10 +288,6 @@ __global__ __launch_bounds__(kT) void gn_apply(const T* __restrict__ x, const Mo
         a[j] = s_rstd[g] * (weight ? weight[c] : 1.f);
         sh[j] = bias ? bias[c] : 0.f;
     }
-    // the last chunks first: the moments' pass has read them last
-    const int ch = q.chunks - 1 - blockIdx.x;
-    const int s0 = ch * q.chunk, s1 = min(s0 + q.chunk, q.S);
-    const int64_t base = ((int64_t)b * q.S) * q.C + c0 + col * V;
     auto one = [&](const Raw<T, V>& r, int s) {
         float v[V];
         r.get(v);
@@ -264,7 +296,9 @@ __global__ __launch_bounds__(kT) void gn_apply(const T* __restrict__ x, const Mo
         Raw<T, V>::store(y + base + (int64_t)s * q.C, v);
     };
     int s = s0 + row;
-    constexpr int U = 4;
+#pragma unroll
+    for (int u = 0; u < U; ++u, s += rows)
+        if (s < s1) one(ahead[u], s);
     for (; s + (U - 1) * rows < s1; s += U * rows) {
         Raw<T, V> r[U];
 #pragma unroll
@@ -360,22 +394,23 @@ __global__ __launch_bounds__(kT) void gn_bwd_sums(const T* __restrict__ x, const
     }
     __syncthreads();
     const int g0 = c0 / q.Cg, g1 = (c0 + wc - 1) / q.Cg;
-    const int lane = tid & 63;
     float* og = grp + (((int64_t)b * q.chunks + blockIdx.x) * q.slabs + slab) * q.G * 2;
-    for (int g = g0 + (tid >> 6); g <= g1; g += kT / 64) {
-        const int lo = max(g * q.Cg - c0, 0), hi = min((g + 1) * q.Cg - c0, wc);
+    by_groups<kT>(g1 - g0 + 1, q.L, [&](int gi, int l) {
+        const int g = g0 + gi;
+        const bool on = g <= g1;
+        const int lo = on ? max(g * q.Cg - c0, 0) : 0, hi = on ? min((g + 1) * q.Cg - c0, wc) : 0;
         float t1 = 0.f, t2 = 0.f;
-        for (int c = lo + lane; c < hi; c += 64) {
+        for (int c = lo + l; c < hi; c += q.L) {
             t1 += s_1[c];
             t2 += s_2[c];
         }
-        t1 = wave_sum(t1);
-        t2 = wave_sum(t2);
-        if (lane == 0) {
+        t1 = lanes_sum(t1, q.L);
+        t2 = lanes_sum(t2, q.L);
+        if (on && l == 0) {
             og[2 * g] = t1;
             og[2 * g + 1] = t2;
         }
-    }
+    });
 }
 
 template <class T, int V, int ACT>
@@ -384,7 +419,7 @@ __global__ __launch_bounds__(kT) void gn_bwd_apply(const T* __restrict__ x, cons
                                                    const float* __restrict__ mean, const float* __restrict__ rstd,
                                                    const float* __restrict__ grp, T* __restrict__ dx, Geometry q) {
     __shared__ float s_1[kT * V], s_2[kT * V];
-    const int tid = threadIdx.x, lane = tid & 63;
+    const int tid = threadIdx.x;
     const int rows = kT / q.cv;
     const int row = tid / q.cv, col = tid - row * q.cv;
     const int slab = blockIdx.y, b = blockIdx.z;
@@ -392,25 +427,42 @@ __global__ __launch_bounds__(kT) void gn_bwd_apply(const T* __restrict__ x, cons
     const int wc = min(q.cv * V, q.C - c0);
     const int g0 = c0 / q.Cg, g1 = (c0 + wc - 1) / q.Cg;
     const float inv_n = 1.0f / ((float)q.S * (float)q.Cg);
-    for (int g = g0 + (tid >> 6); g <= g1; g += kT / 64) {
+    const int ch = q.chunks - 1 - blockIdx.x;
+    const int s0 = ch * q.chunk, s1 = min(s0 + q.chunk, q.S);
+    const int64_t base = ((int64_t)b * q.S) * q.C + c0 + col * V;
+    const bool live = row < rows && col * V < wc;
+    constexpr int U = 2;
+    Raw<T, V> ax[U], ag[U];
+    if (live) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (s0 + row + u * rows < s1) {
+                ax[u].load(x + base + (int64_t)(s0 + row + u * rows) * q.C);
+                ag[u].load(dy + base + (int64_t)(s0 + row + u * rows) * q.C);
+            }
+    }
+    by_groups<kT>(g1 - g0 + 1, q.L, [&](int gi, int l) {
+        const bool on = g0 + gi <= g1;
+        const int g = on ? g0 + gi : g1;
         const int first = (g * q.Cg) / (q.cv * V), last = ((g + 1) * q.Cg - 1) / (q.cv * V);
         const int ns = last - first + 1;
+        const float* p = grp + (((int64_t)b * q.chunks * q.slabs + first) * q.G + g) * 2;
         float t1 = 0.f, t2 = 0.f;
-        for (int i = lane; i < q.chunks * ns; i += 64) {
-            const int ch = i / ns, sl = first + i - ch * ns;
-            const float* p = grp + ((((int64_t)b * q.chunks + ch) * q.slabs + sl) * q.G + g) * 2;
-            t1 += p[0];
-            t2 += p[1];
+        for (int i = l; i < q.chunks * ns; i += q.L) {
+            const int c = ns == 1 ? i : i / ns, sl = i - c * ns;
+            const float* e = p + ((int64_t)c * q.slabs + sl) * q.G * 2;
+            t1 += e[0];
+            t2 += e[1];
         }
-        t1 = wave_sum(t1);
-        t2 = wave_sum(t2);
-        if (lane == 0) {
-            s_1[g - g0] = t1 * inv_n;
-            s_2[g - g0] = t2 * inv_n;
+        t1 = lanes_sum(t1, q.L);
+        t2 = lanes_sum(t2, q.L);
+        if (on && l == 0) {
+            s_1[gi] = t1 * inv_n;
+            s_2[gi] = t2 * inv_n;
         }
-    }
+    });
     __syncthreads();
-    if (row >= rows || col * V >= wc) return;
+    if (!live) return;
     float mu[V], rs[V], w[V], sh[V], m1[V], m2[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -422,9 +474,6 @@ __global__ __launch_bounds__(kT) void gn_bwd_apply(const T* __restrict__ x, cons
         m1[j] = s_1[g - g0];
         m2[j] = s_2[g - g0];
     }
-    const int ch = q.chunks - 1 - blockIdx.x;
-    const int s0 = ch * q.chunk, s1 = min(s0 + q.chunk, q.S);
-    const int64_t base = ((int64_t)b * q.S) * q.C + c0 + col * V;
     auto one = [&](const Raw<T, V>& rx, const Raw<T, V>& rg, int s) {
         float v[V], g[V];
         rx.get(v);
@@ -438,7 +487,9 @@ __global__ __launch_bounds__(kT) void gn_bwd_apply(const T* __restrict__ x, cons
         Raw<T, V>::store(dx + base + (int64_t)s * q.C, v);
     };
     int s = s0 + row;
-    constexpr int U = 2;
+#pragma unroll
+    for (int u = 0; u < U; ++u, s += rows)
+        if (s < s1) one(ax[u], ag[u], s);
     for (; s + (U - 1) * rows < s1; s += U * rows) {
         Raw<T, V> rx[U], rg[U];
 #pragma unroll
@@ -455,6 +506,246 @@ __global__ __launch_bounds__(kT) void gn_bwd_apply(const T* __restrict__ x, cons
         rg.load(dy + base + (int64_t)s * q.C);
         one(rx, rg, s);
     }
+}
+
+// ---- one pass: whole groups of a sample in one workgroup's registers -------------------------------------------
+
+// Thread t holds chunk t % wv (V channels, all of one group) of pixels t / wv, + R, + 2 R, ... (R = NT / wv), at most NV.
+struct Slab {
+    int S, C, G, Cg;
+    int W, wv;                // channels of a workgroup (whole groups), W / V
+    int L;                    // lanes that put a group together
+    int paired;
+};
+
+// Workgroup -> (slab, sample).  Paired: the two slabs of 64 bytes that share a 128-byte line go to workgroups 8 apart, which
+// one XCD runs, so that its L2 fetches and writes whole lines.
+__device__ __forceinline__ void slab_place(const Slab& q, int& slab, int& b) {
+    const int n = q.C / q.W, id = blockIdx.x;
+    if (q.paired) {
+        const int pair = (id >> 4) * 8 + (id & 7), half = (id >> 3) & 1, m = n >> 1;
+        b = pair / m;
+        slab = (pair - b * m) * 2 + half;
+    } else {
+        b = id / n;
+        slab = id - b * n;
+    }
+}
+
+// sums of two values per thread over the threads of each group: s_out[0 / 1][group of the slab]; two barriers
+template <int NT, int V>
+__device__ __forceinline__ void slab_sums(const Slab& q, int R, float v1, float v2, float (*s_in)[NT], float (*s_out)[NT]) {
+    const int tid = threadIdx.x, gv = q.Cg / V;                      // gv: threads side by side in a group
+    s_in[0][tid] = v1;                                               // [pixel row][chunk] as the threads lie
+    s_in[1][tid] = v2;
+    __syncthreads();
+    by_groups<NT>(q.W / q.Cg, q.L, [&](int g, int l) {
+        const bool on = g < q.W / q.Cg;
+        float t1 = 0.f, t2 = 0.f;
+        if (on)
+            for (int i = l; i < R * gv; i += q.L) {
+                const int r = i / gv, at = r * q.wv + g * gv + i - r * gv;
+                t1 += s_in[0][at];
+                t2 += s_in[1][at];
+            }
+        t1 = lanes_sum(t1, q.L);
+        t2 = lanes_sum(t2, q.L);
+        if (on && l == 0) {
+            s_out[0][g] = t1;
+            s_out[1][g] = t2;
+        }
+    });
+    __syncthreads();
+}
+
+template <class T, int V, int ACT, int NT, int NV>
+__global__ __launch_bounds__(NT) void gn_slab(const T* __restrict__ x, const float* __restrict__ weight,
+                                              const float* __restrict__ bias, T* __restrict__ y, float* __restrict__ mean_out,
+                                              float* __restrict__ rstd_out, Slab q, float eps) {
+    __shared__ float s_in[2][NT], s_out[2][NT];
+    const int tid = threadIdx.x;
+    const int R = NT / q.wv, row = tid / q.wv, col = tid - row * q.wv;
+    int slab_id, b;
+    slab_place(q, slab_id, b);
+    const int c0 = slab_id * q.W;
+    const int gl = col * V / q.Cg;                                   // group within the slab
+    const int64_t base = ((int64_t)b * q.S) * q.C + c0 + col * V;
+    const bool live = row < R;
+    Raw<T, V> r[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (live && row + i * R < q.S) r[i].load(x + base + (int64_t)(row + i * R) * q.C);
+    float w[V], sh[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        w[j] = live && weight ? weight[c0 + col * V + j] : 1.f;
+        sh[j] = live && bias ? bias[c0 + col * V + j] : 0.f;
+    }
+    const float inv_n = 1.0f / ((float)q.S * (float)q.Cg);
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (live && row + i * R < q.S) {
+            float v[V];
+            r[i].get(v);
+#pragma unroll
+            for (int j = 0; j < V; ++j) t += v[j];
+        }
+    slab_sums<NT, V>(q, R, t, 0.f, s_in, s_out);
+    const float mu0 = s_out[0][gl] * inv_n;
+    // second moment about the mean as summed, and what that mean is off by
+    float t1 = 0.f, t2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (live && row + i * R < q.S) {
+            float v[V];
+            r[i].get(v);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float d = v[j] - mu0;
+                t1 += d;
+                t2 = fmaf(d, d, t2);
+            }
+        }
+    slab_sums<NT, V>(q, R, t1, t2, s_in, s_out);
+    const float off = s_out[0][gl] * inv_n;
+    const float var = fmaf(-off, off, s_out[1][gl] * inv_n);
+    const float mu = mu0 + off, rstd = rsqrtf((var > 0.f || var != var ? var : 0.f) + eps);
+    if (!live) return;
+    if (mean_out && row == 0 && col * V % q.Cg == 0) {
+        mean_out[b * q.G + c0 / q.Cg + gl] = mu;
+        rstd_out[b * q.G + c0 / q.Cg + gl] = rstd;
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) w[j] *= rstd;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (row + i * R < q.S) {
+            float v[V];
+            r[i].get(v);
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] = act_of<ACT>(fmaf(v[j] - mu, w[j], sh[j]));
+            Raw<T, V>::store(y + base + (int64_t)(row + i * R) * q.C, v);
+        }
+}
+
+template <class T, int V, int ACT, int NT, int NV>
+__global__ __launch_bounds__(NT) void gn_slab_bwd(const T* __restrict__ x, const T* __restrict__ dy,
+                                                  const float* __restrict__ weight, const float* __restrict__ bias,
+                                                  const float* __restrict__ mean, const float* __restrict__ rstd,
+                                                  T* __restrict__ dx, float* __restrict__ chan, Slab q) {
+    __shared__ float s_1[NT * V], s_2[NT * V];
+    __shared__ float s_m[2][NT];
+    const int tid = threadIdx.x;
+    const int R = NT / q.wv, row = tid / q.wv, col = tid - row * q.wv;
+    int slab_id, b;
+    slab_place(q, slab_id, b);
+    const int c0 = slab_id * q.W;
+    const int gl = col * V / q.Cg;
+    const int64_t base = ((int64_t)b * q.S) * q.C + c0 + col * V;
+    const bool live = row < R;
+    // gelu' and silu' cost more arithmetic than the memory leaves time for twice: their dz stays in registers
+    constexpr bool HOLD = ACT == GN_GELU || ACT == GN_SILU;
+    Raw<T, V> rx[NV], rg[NV];
+    float held[HOLD ? NV : 1][V];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (live && row + i * R < q.S) {
+            rx[i].load(x + base + (int64_t)(row + i * R) * q.C);
+            rg[i].load(dy + base + (int64_t)(row + i * R) * q.C);
+        }
+    float w[V], sh[V], a1[V], a2[V];
+    const float mu = live ? mean[b * q.G + c0 / q.Cg + gl] : 0.f, rs = live ? rstd[b * q.G + c0 / q.Cg + gl] : 0.f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        w[j] = live && weight ? weight[c0 + col * V + j] : 1.f;
+        sh[j] = live && bias ? bias[c0 + col * V + j] : 0.f;
+        a1[j] = a2[j] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (live && row + i * R < q.S) {
+            float v[V], g[V];
+            rx[i].get(v);
+            rg[i].get(g);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float h = (v[j] - mu) * rs;
+                const float dz = ACT == GN_NONE ? g[j] : g[j] * dact_of<ACT>(fmaf(h, w[j], sh[j]));
+                if constexpr (HOLD) held[i][j] = dz;
+                a1[j] += dz;
+                a2[j] = fmaf(dz, h, a2[j]);
+            }
+        }
+    if (live) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            s_1[row * q.W + col * V + j] = a1[j];
+            s_2[row * q.W + col * V + j] = a2[j];
+        }
+    }
+    __syncthreads();
+    // per channel: the rows in NT / W parts, then the parts
+    const int parts = NT / q.W < R ? (NT / q.W > 0 ? NT / q.W : 1) : R;
+    for (int i = tid; i < parts * q.W; i += NT) {
+        const int p = i / q.W, c = i - p * q.W;
+        float t1 = 0.f, t2 = 0.f;
+        for (int r = p; r < R; r += parts) {
+            t1 += s_1[r * q.W + c];
+            t2 += s_2[r * q.W + c];
+        }
+        s_1[p * q.W + c] = t1;                              // rows p, p + parts, ...: this thread's alone
+        s_2[p * q.W + c] = t2;
+    }
+    __syncthreads();
+    for (int c = tid; c < q.W; c += NT) {
+        float t1 = s_1[c], t2 = s_2[c];
+        for (int p = 1; p < parts; ++p) {
+            t1 += s_1[p * q.W + c];
+            t2 += s_2[p * q.W + c];
+        }
+        chan[(int64_t)b * 2 * q.C + c0 + c] = t1;
+        chan[(int64_t)b * 2 * q.C + q.C + c0 + c] = t2;
+        const float wc = weight ? weight[c0 + c] : 1.f;
+        s_1[c] = t1 * wc;
+        s_2[c] = t2 * wc;
+    }
+    __syncthreads();
+    const float inv_n = 1.0f / ((float)q.S * (float)q.Cg);
+    by_groups<NT>(q.W / q.Cg, q.L, [&](int g, int l) {
+        const bool on = g < q.W / q.Cg;
+        float t1 = 0.f, t2 = 0.f;
+        if (on)
+            for (int c = l; c < q.Cg; c += q.L) {
+                t1 += s_1[g * q.Cg + c];
+                t2 += s_2[g * q.Cg + c];
+            }
+        t1 = lanes_sum(t1, q.L);
+        t2 = lanes_sum(t2, q.L);
+        if (on && l == 0) {
+            s_m[0][g] = t1 * inv_n;
+            s_m[1][g] = t2 * inv_n;
+        }
+    });
+    __syncthreads();
+    if (!live) return;
+    const float m1 = s_m[0][gl], m2 = s_m[1][gl];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (row + i * R < q.S) {
+            float v[V], g[V];
+            rx[i].get(v);
+            if constexpr (!HOLD) rg[i].get(g);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float h = (v[j] - mu) * rs;
+                float dz;
+                if constexpr (HOLD) dz = held[i][j];
+                else dz = ACT == GN_NONE ? g[j] : g[j] * dact_of<ACT>(fmaf(h, w[j], sh[j]));
+                v[j] = rs * (fmaf(dz, w[j], -m1) - h * m2);
+            }
+            Raw<T, V>::store(dx + base + (int64_t)(row + i * R) * q.C, v);
+        }
 }
 
 // dweight[c] = sum of chan[r][1][c], dbias[c] = sum of chan[r][0][c] over the rows r, in a fixed order: a workgroup takes
@@ -490,6 +781,13 @@ __global__ __launch_bounds__(1024) void gn_bwd_params(const float* __restrict__ 
     }
 }
 
+// lanes to a group so that `threads` serve ng groups at once where they can
+int lanes_of(int threads, int ng) {
+    int L = 64;
+    while (L > 1 && L * ng > threads) L >>= 1;
+    return L;
+}
+
 int vec_of(int esize, int C, bool aligned) {
     const int v = 16 / esize;
     return aligned && C % v == 0 ? v : 1;
@@ -512,6 +810,32 @@ Geometry geometry(int B, int S, int C, int G, int V) {
     if (chunks < 1) chunks = 1;
     q.chunk = (int)((S + chunks - 1) / chunks);
     q.chunks = (S + q.chunk - 1) / q.chunk;
+    q.L = lanes_of(kT, (q.cv * V + q.Cg - 1) / q.Cg + 1);
+    return q;
+}
+
+constexpr int kSlabMost = 16;   // vectors of a thread at most (of x, and of dy again in the backward)
+
+// The one-pass form's cut, or W = 0 where a sample's groups do not fit: as few whole groups as make rows of 128 bytes, of
+// 64 where those do not fit, each vector within one group.  512 threads, or in the forward 1,024 for longer maps (128
+// registers each; the backward holds twice as much).
+Slab slab(int B, int S, int C, int G, int V, int esize, bool backward, int& threads) {
+    Slab q = {S, C, G, C / G, 0, 0, 1, 0};
+    if (V == 1 || q.Cg % V != 0) return q;
+    for (threads = 512; threads <= (backward ? 512 : 1024); threads *= 2)
+        for (const int bytes : {128, 64}) {
+            int k = 1;
+            while (k < G && (k * q.Cg * esize < bytes || G % k != 0)) ++k;
+            const int64_t wv = (int64_t)k * q.Cg / V;
+            if (wv > threads || (int64_t)B * (G / k) > 0x7FFFFFFF) continue;
+            const int R = threads / (int)wv;
+            if (((int64_t)S + R - 1) / R > kSlabMost) continue;
+            q.W = k * q.Cg;
+            q.wv = (int)wv;
+            q.L = lanes_of(threads, k);
+            q.paired = q.W * esize == 64 && (int64_t)B * (G / k) % 16 == 0 && (G / k) % 2 == 0;
+            return q;
+        }
     return q;
 }
 
@@ -528,6 +852,21 @@ hipError_t by_act(int act, F&& f) {
 template <class T, int V>
 hipError_t forward(const T* x, const float* weight, const float* bias, T* y, float* mean, float* rstd, Mom* part, int B,
                    int S, int C, int G, float eps, int act, hipStream_t s) {
+    if constexpr (V > 1) {
+        int threads;
+        const Slab sl = slab(B, S, C, G, V, sizeof(T), false, threads);
+        if (sl.W) {
+            const int R = threads / sl.wv, nv = (S + R - 1) / R;
+            return by_act(act, [&](auto a) {
+                constexpr int A = decltype(a)::value;
+                const dim3 grid(B * (C / sl.W)), block(threads);
+                if (threads == 1024) hipLaunchKernelGGL((gn_slab<T, V, A, 1024, kSlabMost>), grid, block, 0, s, x, weight, bias, y, mean, rstd, sl, eps);
+                else if (nv <= 4) hipLaunchKernelGGL((gn_slab<T, V, A, 512, 4>), grid, block, 0, s, x, weight, bias, y, mean, rstd, sl, eps);
+                else hipLaunchKernelGGL((gn_slab<T, V, A, 512, kSlabMost>), grid, block, 0, s, x, weight, bias, y, mean, rstd, sl, eps);
+                return hipGetLastError();
+            });
+        }
+    }
     const Geometry q = geometry(B, S, C, G, V);
     const dim3 grid(q.chunks, q.slabs, B);
     hipLaunchKernelGGL((gn_moments<T, V>), grid, dim3(kT), 0, s, x, part, q);
@@ -542,6 +881,23 @@ hipError_t forward(const T* x, const float* weight, const float* bias, T* y, flo
 template <class T, int V>
 hipError_t backward(const T* x, const float* weight, const float* bias, const T* dy, const float* mean, const float* rstd,
                     T* dx, float* dweight, float* dbias, float* ws, int B, int S, int C, int G, int act, hipStream_t s) {
+    if constexpr (V > 1) {
+        int threads;
+        const Slab sl = slab(B, S, C, G, V, sizeof(T), true, threads);
+        if (sl.W) {
+            const int R = threads / sl.wv, nv = (S + R - 1) / R;
+            hipError_t e = by_act(act, [&](auto a) {
+                constexpr int A = decltype(a)::value;
+                const dim3 grid(B * (C / sl.W)), block(512);
+                if (nv <= 4) hipLaunchKernelGGL((gn_slab_bwd<T, V, A, 512, 4>), grid, block, 0, s, x, dy, weight, bias, mean, rstd, dx, ws, sl);
+                else hipLaunchKernelGGL((gn_slab_bwd<T, V, A, 512, kSlabMost>), grid, block, 0, s, x, dy, weight, bias, mean, rstd, dx, ws, sl);
+                return hipGetLastError();
+            });
+            if (e != hipSuccess || (!dweight && !dbias)) return e;
+            hipLaunchKernelGGL(gn_bwd_params, dim3((2 * C + 63) / 64), dim3(1024), 0, s, ws, B, C, dweight, dbias);
+            return hipGetLastError();
+        }
+    }
     const Geometry q = geometry(B, S, C, G, V);
     float* chan = ws;
     float* grp = ws + (int64_t)B * q.chunks * 2 * C;

@@ -647,7 +647,8 @@ static int diff_args(const char* name, DiffArgs& a, const void* q, const void* k
     if (!(scale > 0.f) || scale > 3e38f) return fail(VITK_ERR_INVALID, "%s: scale=%g must be positive and finite", name, (double)scale);
     if (nq > (1 << 28) || nk > (1 << 28) || (int64_t)nq * (heads / kv_heads) > (1 << 30) || (int64_t)batch * heads > (1 << 24))
         return fail(VITK_ERR_UNSUPPORTED, "%s: batch=%d nq=%d nk=%d heads=%d", name, batch, nq, nk, heads);
-    if (!aligned16(q) || !aligned16(k) || !aligned16(v)) return fail(VITK_ERR_INVALID, "%s: q, k and v must be 16-byte aligned", name);
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(lam))
+        return fail(VITK_ERR_INVALID, "%s: q, k, v and lam must be 16-byte aligned", name);
     const int per = dtype == VITK_BF16 ? 8 : 4;
     for (int i = 0; i < 11; ++i)
         if (strides[i] < 0 || strides[i] % per != 0)
@@ -678,7 +679,7 @@ int64_t vitk_diff_attention_workspace(int batch, int nq, int nk, int heads, int 
 }
 
 int vitk_diff_attention(const void* q, const void* k, const void* v, const int64_t* strides, const float* lam, int lam_heads,
-                        float lambda_init, float scale, const int* key_lens, int causal, void* out, void* out2, float* lse,
+                        float lambda_init, float scale, const int* key_lens, int causal, void* out, void* out2, float* stats,
                         float* weight, float* workspace, int64_t workspace_floats, int batch, int nq, int nk, int heads,
                         int kv_heads, int d, int dtype, void* stream) {
     const char* name = "vitk_diff_attention";
@@ -687,20 +688,20 @@ int vitk_diff_attention(const void* q, const void* k, const void* v, const int64
                              heads, kv_heads, d, dtype);
     if (rc) return rc;
     if (!out) return fail(VITK_ERR_INVALID, "%s: null pointer", name);
-    if ((out2 != nullptr) != (lse != nullptr) || (out2 != nullptr) != (weight != nullptr))
-        return fail(VITK_ERR_INVALID, "%s: out2, lse and weight come together", name);
+    if ((out2 != nullptr) != (stats != nullptr) || (out2 != nullptr) != (weight != nullptr))
+        return fail(VITK_ERR_INVALID, "%s: out2, stats and weight come together", name);
     if (!aligned16(out) || (out2 && !aligned16(out2))) return fail(VITK_ERR_INVALID, "%s: out and out2 must be 16-byte aligned", name);
     const int64_t need = diff_attention_workspace(a, dtype == VITK_BF16);
     if (workspace_floats < need || (need > 0 && !workspace))
         return fail(VITK_ERR_INVALID, "%s: workspace of %lld floats, %lld needed", name, (long long)workspace_floats, (long long)need);
     if (workspace && !aligned16(workspace)) return fail(VITK_ERR_INVALID, "%s: workspace must be 16-byte aligned", name);
-    hipError_t e = launch_diff_attention(a, DiffOut{out, out2, lse, weight}, workspace, dtype == VITK_BF16, reinterpret_cast<hipStream_t>(stream));
+    hipError_t e = launch_diff_attention(a, DiffOut{out, out2, stats, weight}, workspace, dtype == VITK_BF16, reinterpret_cast<hipStream_t>(stream));
     return launched(e, name);
 }
 
 int vitk_diff_attention_backward(const void* q, const void* k, const void* v, const int64_t* strides, const float* lam,
                                  int lam_heads, float scale, const int* key_lens, int causal, const void* out, const void* out2,
-                                 const float* lse, const float* weight, const void* dout, void* dq, void* dk, void* dv,
+                                 const float* stats, const float* weight, const void* dout, void* dq, void* dk, void* dv,
                                  const int64_t* grad_strides, float* dlam, float* workspace, int64_t workspace_floats, int batch,
                                  int nq, int nk, int heads, int kv_heads, int d, int dtype, void* stream) {
     const char* name = "vitk_diff_attention_backward";
@@ -708,7 +709,7 @@ int vitk_diff_attention_backward(const void* q, const void* k, const void* v, co
     const int rc = diff_args(name, a, q, k, v, strides, lam, lam_heads, 0.f, scale, key_lens, causal, batch, nq, nk, heads,
                              kv_heads, d, dtype);
     if (rc) return rc;
-    if (!out || !out2 || !lse || !weight || !dout || !dq || !dk || !dv || !grad_strides || !workspace)
+    if (!out || !out2 || !stats || !weight || !dout || !dq || !dk || !dv || !grad_strides || !workspace)
         return fail(VITK_ERR_INVALID, "%s: null pointer", name);
     if (!aligned16(out) || !aligned16(out2) || !aligned16(dout) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv))
         return fail(VITK_ERR_INVALID, "%s: pointers must be 16-byte aligned", name);
@@ -720,7 +721,7 @@ int vitk_diff_attention_backward(const void* q, const void* k, const void* v, co
     if (workspace_floats < need) return fail(VITK_ERR_INVALID, "%s: workspace of %lld floats, %lld needed", name, (long long)workspace_floats, (long long)need);
     if (!aligned16(workspace)) return fail(VITK_ERR_INVALID, "%s: workspace must be 16-byte aligned", name);
     DiffGrads g = {};
-    g.out = out; g.out2 = out2; g.dout = dout; g.lse = lse; g.weight = weight; g.dq = dq; g.dk = dk; g.dv = dv; g.dlam = dlam;
+    g.out = out; g.out2 = out2; g.dout = dout; g.stats = stats; g.weight = weight; g.dq = dq; g.dk = dk; g.dv = dv; g.dlam = dlam;
     for (int i = 0; i < 4; ++i) { g.dqs[i] = grad_strides[i]; g.dks[i] = grad_strides[4 + i]; }
     for (int i = 0; i < 3; ++i) g.dvs[i] = grad_strides[8 + i];
     return launched(launch_diff_attention_backward(a, g, workspace, dtype == VITK_BF16, reinterpret_cast<hipStream_t>(stream)), name);

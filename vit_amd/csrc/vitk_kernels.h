@@ -128,18 +128,19 @@ struct DiffArgs {
     int causal;
     float scale, lambda_init;
 };
-// forward: out [batch, nq, heads, 2 d]; for the backward also out2 (the second map's product with V, out's shape), lse
-// f32 [2, batch, heads, nq] and weight f32 [heads], or all three nullptr
+// forward: out [batch, nq, heads, 2 d]; for the backward also out2 (the second map's product with V, out's shape), stats
+// f32 [4, batch, heads, nq] (of both maps the reference point m and 1 / sum of exp2(scale log2(e) s - m)) and weight f32
+// [heads], or all three nullptr
 struct DiffOut {
     void *out, *out2;
-    float *lse, *weight;
+    float *stats, *weight;
 };
 int64_t diff_attention_workspace(const DiffArgs& a, bool bf16);
 hipError_t launch_diff_attention(const DiffArgs& a, const DiffOut& o, float* ws, bool bf16, hipStream_t s);
 // backward: dq, dk, dv with the strides dqs, dks, dvs; dlam f32 [4, lam_heads, d]
 struct DiffGrads {
     const void *out, *out2, *dout;   // [batch, nq, heads, 2 d]
-    const float *lse, *weight;
+    const float *stats, *weight;
     void *dq, *dk, *dv;
     int64_t dqs[4], dks[4], dvs[3];
     float* dlam;

@@ -85,7 +85,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
         return torch.tensor(0.0)
     grads = _ops.GradList(tensors)
     with torch.cuda.device(grads.device):
-        if error_if_nonfinite or not any(grads.size):
+        if error_if_nonfinite or grads.empty:
             partials, norm = _ops.grad_norm(grads, kind)
             if error_if_nonfinite and not math.isfinite(float(norm)):
                 raise _lib.VitkError(f"the gradients' norm is {float(norm)}, so they cannot be clipped (error_if_nonfinite)")
