@@ -77,7 +77,8 @@ def reference(q, k, v, lam, do, kl, lambda_init, scale, causal, dtype):
     edk = torch.stack([fold(edS[m].transpose(-1, -2) @ Q[m].abs()) for m in (0, 1)]) * scale
     res["dk"] = tuple(t.permute(1, 3, 2, 0, 4) for t in (dk, edk * 1.01 + half * dk.abs() + 2.0 ** -20 * edk))
     dv = fold(A.transpose(-1, -2) @ DO)
-    edv = fold((u * A.abs() + r32 * Aabs + EW * p[1]).transpose(-1, -2) @ DO.abs())
+    # the maps' probabilities meet dO apart, each rounded to the type: u P_1 + u |w| P_2
+    edv = fold((u * Aabs + EW * p[1]).transpose(-1, -2) @ DO.abs())
     res["dv"] = tuple(head(t) for t in (dv, edv * 1.01 + half * dv.abs()))
     dw = -(p[1] * dA).sum((0, 2, 3))
     edw = (p[1] * (r32 * dA.abs() + eA)).sum((0, 2, 3))                        # f32 in both types

@@ -147,6 +147,13 @@ __device__ __forceinline__ f32x16 mma_t(const Trans<float, RB>& a, const Slice<f
     return c;
 }
 
+// column sums of the B operand in every element of the accumulator: a product with ones
+__device__ __forceinline__ f32x16 ones_t(const Slice<bf16_t>& b, f32x16 c) {
+    const u32x4 one = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, one), b.v, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 ones_t(const Slice<float>&, f32x16 c) { return c; }
+
 // four neighbouring values to memory
 __device__ __forceinline__ void store4(bf16_t* p, f32x4 v) {
     *reinterpret_cast<u32x2*>(p) = u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
@@ -157,13 +164,14 @@ __device__ __forceinline__ void store4(float* p, f32x4 v) { *reinterpret_cast<f3
 static __device__ __align__(16) const unsigned kZeros[4] = {0, 0, 0, 0};
 
 // The rows of a (sample, key head): row r = query token r / g of query head kh * g + r % g, so that the query heads which
-// share a key head share its tiles.
+// share a key head share its tiles.  The division by g = group is a multiplication by group_mul = 2^(31 + l) / g + 1 with
+// 2^l >= g: n < 2^31 times that, over 2^(31 + l), exceeds n / g by less than 1 / g.
 struct RowPlace {
     int tok, head;
 };
 __device__ __forceinline__ RowPlace row_place(const DiffArgs& a, int kh, int r) {
     if (a.group == 1) return RowPlace{r, kh};
-    const int t = r / a.group;
+    const int t = (int)(__umulhi((unsigned)r, a.group_mul) >> a.group_shift);
     return RowPlace{t, kh * a.group + (r - t * a.group)};
 }
 
@@ -173,6 +181,55 @@ __device__ __forceinline__ int key_limit(const DiffArgs& a, int len, int tok) {
     const int lim = tok + a.nk - a.nq + 1;
     return lim < len ? (lim > 0 ? lim : 0) : len;
 }
+
+constexpr int pow2_below(int n) { return n >= 32 ? 32 : n >= 16 ? 16 : n >= 8 ? 8 : n >= 4 ? 4 : n >= 2 ? 2 : 1; }
+
+// Staging of a chunk of C rows of two tensors side by side, [2 maps x d] and [2 d] (K and V, or Q and dO), through
+// registers into an LDS buffer of two tiles: 4 DPC neighbouring lanes move a row's chunks.  Columns past the head's d are
+// zeroed once in both buffers and left alone; rows past the last one are the last one again (nothing behind it is read),
+// which the caller masks.
+template <class T, int DP, int NT, int C>
+struct Stage {
+    static constexpr int PER = Op<T>::kPer, DPC = DP / PER, RB = row_bytes<T, 2 * DP>(), TILE = C * RB;
+    static constexpr int LANES = 4 * DPC, ROWS = pow2_below(NT / LANES < C ? NT / LANES : C), PASSES = C / ROWS;
+    int row, col;          // within the chunk; chunk of the LDS row
+    bool second, on;
+    int map, e;            // first tensor: map and chunk within it
+    u32x4 held[PASSES];
+    __device__ __forceinline__ void init(int tid, int dc, char* bufs) {
+        row = tid / LANES;
+        const int c = tid - row * LANES;
+        second = c >= 2 * DPC;
+        col = second ? c - 2 * DPC : c;
+        map = !second && col >= DPC ? 1 : 0;
+        e = col - map * DPC;
+        const bool mine = row < ROWS;
+        on = mine && (second ? col < 2 * dc : e < dc);
+        if (mine && !on)
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int i = 0; i < PASSES; ++i) *reinterpret_cast<u32x4*>(bufs + k * 2 * TILE + at(i)) = u32x4{0u, 0u, 0u, 0u};
+    }
+    __device__ __forceinline__ int at(int i) const {
+        const int lr = row + i * ROWS;
+        return (second ? TILE : 0) + lr * RB + ((col ^ swz<RB>(lr)) << 4);
+    }
+    // addr(row): where the row of this lane's tensor, map and chunk lies
+    template <class F>
+    __device__ __forceinline__ void fetch(int row0, int rows, F&& addr) {
+        if (!on) return;
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+            const int r = row0 + row + i * ROWS;
+            held[i] = *reinterpret_cast<const u32x4*>(addr(r < rows ? r : rows - 1));
+        }
+    }
+    __device__ __forceinline__ void put(char* buf) const {
+        if (!on) return;
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) *reinterpret_cast<u32x4*>(buf + at(i)) = held[i];
+    }
+};
 
 // w_h = exp(lam0 . lam1) - exp(lam2 . lam3) + lambda_init; the half-waves share the sums of a lane's head, all loads at once
 template <int DP>

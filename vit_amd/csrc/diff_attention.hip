@@ -2,18 +2,19 @@
 //     P_m = softmax over the visible keys of scale q_m . k_m,  m = 1, 2
 //     out = (P_1 - w P_2) V,    w = exp(lam0 . lam1) - exp(lam2 . lam3) + lambda_init
 //
-// One pass over the keys with a running maximum and sum per map.  The two maps share everything but their scores: a
-// workgroup stages the keys of both maps and V once, and every transposed V fragment feeds the products of both maps.
-// The maps' products with V stay apart until the end because their denominators are known only then.
+// One pass over the keys with a running maximum and sum per map.  The two maps of a head share V and little else, and
+// their products with V stay apart until the end, because their denominators are known only then; so a pair of waves takes
+// 32 query rows, one map each, which halves what a wave holds (its accumulators above all) and doubles the waves that hide
+// each other's waiting.  They meet once, for P_1 V - w P_2 V.
 //
 //     S_m^T[key][row]  = K_m Q_m^T       keys on the matrix row, query rows on the lane
 //     O_m^T[col][row] += V^T P_m^T       the exponentiated accumulators are the B operand as they lie
 //
-// Rows of a (sample, key head) are the tokens of all its query heads (diff_attention.h), 32 to a wave.  Two forms:
-//   many rows:  a workgroup of 4 waves takes 128 rows and walks all their keys in chunks of 32 through two LDS buffers,
+// Rows of a (sample, key head) are the tokens of all its query heads (diff_attention.h).  Two forms:
+//   many rows:  the pairs of a workgroup take 32 rows each and walk all their keys in chunks of 32 through two LDS buffers,
 //               the next chunk on its way to registers while the waves work on the one before;
-//   few rows:   its waves take the same 32 rows and every fourth block of 32 keys, and the keys are split over so many
-//               workgroups that the chip is full; the waves' results are joined in LDS, the workgroups' by a second kernel.
+//   few rows:   the pairs take the same 32 rows and every fourth block of 32 keys, and the keys are split over so many
+//               workgroups that the chip is full; the pairs' results are joined in LDS, the workgroups' by a second kernel.
 #include <type_traits>
 
 #include "diff_attention.h"
@@ -24,10 +25,12 @@ using namespace diff;
 
 namespace {
 
+// pairs of waves in a workgroup
 template <class T, int DP>
-constexpr int keys_waves() { return row_bytes<T, 2 * DP>() == 512 ? 2 : 4; }
+constexpr int keys_pairs() { return row_bytes<T, 2 * DP>() == 512 ? 2 : 4; }
 
-constexpr int pow2_below(int n) { return n >= 16 ? 16 : n >= 8 ? 8 : n >= 4 ? 4 : n >= 2 ? 2 : 1; }
+template <class T, int DP>
+constexpr int rows_pairs() { return sizeof(T) == 4 || DP == 32 ? 4 : 2; }
 
 // index of a 4-column piece of a joined row in LDS: [row][2 maps x DV columns] f32, pieces swizzled by the row
 template <int DV>
@@ -36,23 +39,27 @@ __device__ __forceinline__ int joined(int row, int map, int col) {
     return row * (2 * DV) + ((c ^ (row & 15)) << 2);
 }
 
-template <class T, int DP, int NW, bool KEYS>
-__global__ __launch_bounds__(NW * 64, KEYS || sizeof(T) == 4 ? 1 : 2) void diff_fwd(DiffArgs a, DiffOut o, float* __restrict__ ws, int tiles,
-                                                                  int splits) {
+// OCC: waves to a SIMD that the registers have to allow.  TRAIN: the sums for the backward are written too, and the
+// denominators are added from the probabilities before their rounding to bf16 (16 additions a block and lane); without it
+// the matrix pipe adds the rounded ones, which are what the product with V uses, beside that product.
+template <class T, int DP, int NG, bool KEYS, bool TRAIN, int OCC>
+__global__ __launch_bounds__(NG * 128, OCC) void diff_fwd(DiffArgs a, DiffOut o, float* __restrict__ ws, int tiles, int splits) {
     constexpr int DV = 2 * DP;
+    constexpr int NT = NG * 128;
     constexpr int RB = row_bytes<T, DV>();         // of an LDS row: both maps of a key, or one of V
     constexpr int PER = Op<T>::kPer;
     constexpr int DPC = DP / PER;                  // chunks of one map's key
     constexpr int KT = DPC / 2;                    // products of 2 chunks (one per half-wave) of a score
     constexpr int DB = DV / 32;
-    constexpr int KC = KEYS ? 32 * NW : 32;        // keys of a chunk
+    constexpr int KC = 32 * (KEYS ? NG : 1);       // keys of a chunk; 64 for many rows: 3 to 9 % slower
     constexpr int TILE = KC * RB;
     typedef typename Op<T>::Chunk Chunk;
     __shared__ __align__(16) char bufs[2][2 * TILE];
-    __shared__ float s_ml[KEYS ? NW : 1][4][32];
-    __shared__ float s_w[32];
+    __shared__ float s_ml[KEYS ? NG : 1][4][32];
+    __shared__ float s_w[KEYS ? 32 : 1];
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), map = wave & 1, grp = wave >> 1;
     const int r = lane & 31, hh = lane >> 5;
     const int bks = a.batch * a.kv_heads;
     const int bk = blockIdx.x % bks;               // workgroups of one head lie bks apart: one XCD where 8 divides bks
@@ -61,8 +68,8 @@ __global__ __launch_bounds__(NW * 64, KEYS || sizeof(T) == 4 ? 1 : 2) void diff_
     const int split = KEYS ? rest / tiles : 0;
     const int b = bk / a.kv_heads, kh = bk - b * a.kv_heads;
     const int nrows = a.nq * a.group;
-    const int row0 = KEYS ? tile * 32 : (tile * NW + wave) * 32;
-    const int end = KEYS ? tile * 32 + 32 : (tile + 1) * NW * 32;
+    const int row0 = KEYS ? tile * 32 : (tile * NG + grp) * 32;
+    const int end = KEYS ? tile * 32 + 32 : (tile + 1) * NG * 32;
     int len = a.nk;
     if (a.key_lens) {
         len = a.key_lens[b];
@@ -70,37 +77,13 @@ __global__ __launch_bounds__(NW * 64, KEYS || sizeof(T) == 4 ? 1 : 2) void diff_
     }
     const int kmax = key_limit(a, len, row_place(a, kh, (end < nrows ? end : nrows) - 1).tok);
 
-    // Staging: 4 DPC neighbouring lanes move a key's chunks, both maps of K and then V, ROWS keys at a time; what lies past
-    // the last visible key or past the head's d columns is written as zeros and never read from memory.
-    constexpr int LANES = 4 * DPC;
-    constexpr int ROWS = pow2_below(NW * 64 / LANES);
-    constexpr int PASSES = KC / ROWS;
     const int dc = a.d / PER;
-    const int srow = tid / LANES, scol = tid - srow * LANES;
-    const bool s_v = scol >= 2 * DPC;
-    const int s_c = s_v ? scol - 2 * DPC : scol;                         // chunk of the LDS row
-    const int s_m = !s_v && s_c >= DPC ? 1 : 0, s_e = s_c - s_m * DPC;
-    const bool s_on = srow < ROWS && (s_v ? s_c < 2 * dc : s_e < dc);
-    const int64_t s_step = s_v ? a.vs[1] : a.ks[1];
-    const T* s_src = s_v ? reinterpret_cast<const T*>(a.v) + b * a.vs[0] + kh * a.vs[2] + s_c * PER
-                         : reinterpret_cast<const T*>(a.k) + b * a.ks[0] + kh * a.ks[2] + s_m * a.ks[3] + s_e * PER;
-    u32x4 held[PASSES];
-    auto fetch = [&](int key0) {
-#pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
-            const int key = key0 + srow + i * ROWS;
-            held[i] = u32x4{0u, 0u, 0u, 0u};
-            if (s_on && key < kmax) held[i] = *reinterpret_cast<const u32x4*>(s_src + key * s_step);
-        }
-    };
-    auto put = [&](char* buf) {
-        if (srow >= ROWS) return;
-#pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
-            const int lr = srow + i * ROWS;
-            *reinterpret_cast<u32x4*>(buf + (s_v ? TILE : 0) + lr * RB + ((s_c ^ swz<RB>(lr)) << 4)) = held[i];
-        }
-    };
+    Stage<T, DP, NT, KC> stage;
+    stage.init(tid, dc, bufs[0]);
+    const int64_t s_step = stage.second ? a.vs[1] : a.ks[1];
+    const T* s_src = stage.second ? reinterpret_cast<const T*>(a.v) + b * a.vs[0] + kh * a.vs[2] + stage.col * PER
+                                  : reinterpret_cast<const T*>(a.k) + b * a.ks[0] + kh * a.ks[2] + stage.map * a.ks[3] + stage.e * PER;
+    auto fetch = [&](int key0) { stage.fetch(key0, kmax, [&](int key) { return s_src + key * s_step; }); };
 
     int c0 = 0, c1 = (kmax + KC - 1) / KC;
     if constexpr (KEYS) {
@@ -118,93 +101,87 @@ __global__ __launch_bounds__(NW * 64, KEYS || sizeof(T) == 4 ? 1 : 2) void diff_
     const int wave_min = key_limit(a, len, row_place(a, kh, row0 < nrows ? row0 : nrows - 1).tok);
     const bool active = row0 < nrows;
 
-    Chunk qf[2][KT];
+    Chunk qf[KT];
     {
-        const T* qg = reinterpret_cast<const T*>(a.q) + b * a.qs[0] + place.tok * a.qs[1] + place.head * a.qs[2];
+        const T* qg = reinterpret_cast<const T*>(a.q) + b * a.qs[0] + place.tok * a.qs[1] + place.head * a.qs[2] + map * a.qs[3];
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int t = 0; t < KT; ++t) {
-                const int c = 2 * t + hh;
-                qf[m][t] = *reinterpret_cast<const Chunk*>(c < dc ? (const void*)(qg + m * a.qs[3] + c * PER) : (const void*)kZeros);
-            }
+        for (int t = 0; t < KT; ++t) {
+            const int c = 2 * t + hh;
+            qf[t] = *reinterpret_cast<const Chunk*>(c < dc ? (const void*)(qg + c * PER) : (const void*)kZeros);
+        }
     }
-    const float weight = map_weight<DP>(a, place.head, hh);
+    const float weight = map == 0 ? map_weight<DP>(a, place.head, hh) : 0.f;
 
-    f32x16 acc[2][DB];
-    float m_run[2] = {kNoScore, kNoScore}, l_run[2] = {0.f, 0.f};
+    constexpr bool MSUM = !TRAIN && sizeof(T) == 2;
+    f32x16 acc[DB], l_acc = zero16();
+    float m_run = kNoScore, l_run = 0.f;
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int d = 0; d < DB; ++d) acc[m][d] = zero16();
+    for (int d = 0; d < DB; ++d) acc[d] = zero16();
     const float sc = a.scale * kLog2e;
     constexpr float kLazy = 8.0f;     // the accumulators are rescaled only when a maximum grows by more than 2^8
 
     auto step = [&](const char* kt, const char* vt, int kb, int key0) {
-        f32x16 s[2];
+        f32x16 s = zero16();
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            s[m] = zero16();
-#pragma unroll
-            for (int t = 0; t < KT; ++t) s[m] = Op<T>::mma(chunk_at<T, RB>(kt, kb * 32 + r, m * DPC + 2 * t + hh), qf[m][t], s[m]);
-        }
+        for (int t = 0; t < KT; ++t) s = Op<T>::mma(chunk_at<T, RB>(kt, kb * 32 + r, map * DPC + 2 * t + hh), qf[t], s);
         if (key0 + 32 > wave_min) {
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-                if (key0 + 8 * (i >> 2) + 4 * hh + (i & 3) >= lim) s[0][i] = s[1][i] = -__builtin_inff();
+                if (key0 + 8 * (i >> 2) + 4 * hh + (i & 3) >= lim) s[i] = -__builtin_inff();
         }
+        float mx = fmaxf(s[0], s[1]);
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            float mx = fmaxf(s[m][0], s[m][1]);
+        for (int i = 2; i < 16; i += 2) mx = fmaxf(fmaxf(mx, s[i]), s[i + 1]);
+        mx = both_max(mx) * sc;                                      // scale > 0: the maximum commutes with it
+        if (__any(mx > m_run + kLazy)) {
+            const float m_new = fmaxf(m_run, mx);
+            const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+            m_run = m_new;
+            if constexpr (MSUM) {
 #pragma unroll
-            for (int i = 2; i < 16; i += 2) mx = fmaxf(fmaxf(mx, s[m][i]), s[m][i + 1]);
-            mx = both_max(mx) * sc;                                  // scale > 0: the maximum commutes with it
-            if (__any(mx > m_run[m] + kLazy)) {
-                const float m_new = fmaxf(m_run[m], mx);
-                const float alpha = __builtin_amdgcn_exp2f(m_run[m] - m_new);
-                m_run[m] = m_new;
-                l_run[m] *= alpha;
-#pragma unroll
-                for (int d = 0; d < DB; ++d)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[m][d][i] *= alpha;
+                for (int i = 0; i < 16; ++i) l_acc[i] *= alpha;
+            } else {
+                l_run *= alpha;
             }
-            float sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[m][i] = __builtin_amdgcn_exp2f(fmaf(s[m][i], sc, -m_run[m]));
-                sum += s[m][i];
-            }
-            l_run[m] += sum;
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[d][i] *= alpha;
         }
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], sc, -m_run));
+            if constexpr (!MSUM) sum += s[i];
+        }
+        l_run += sum;
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
-            Slice<T> p1, p2;
-            p1.take(s[0], st);
-            p2.take(s[1], st);
+            Slice<T> p;
+            p.take(s, st);
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
                 Trans<T, RB> v;
                 v.load(vt, kb * 32 + 16 * st, d * 32, lane);
-                acc[0][d] = mma_t(v, p1, acc[0][d]);
-                acc[1][d] = mma_t(v, p2, acc[1][d]);
+                acc[d] = mma_t(v, p, acc[d]);
             }
+            if constexpr (MSUM) l_acc = ones_t(p, l_acc);
         }
     };
-    const int kb = KEYS ? wave : 0;                                  // the wave's block of a chunk
-    if (c0 < c1) put(bufs[0]);
+    if (c0 < c1) stage.put(bufs[0]);
     __syncthreads();
     for (int c = c0; c < c1; ++c) {
         const char* buf = bufs[(c - c0) & 1];
         const bool more = c + 1 < c1;
         if (more) fetch((c + 1) * KC);
-        const int key0 = c * KC + kb * 32;
-        if (active && key0 < wave_max) step(buf, buf + TILE, kb, key0);
-        if (more) put(bufs[(c - c0 + 1) & 1]);
+        const int key0 = c * KC + (KEYS ? grp * 32 : 0);             // few rows: the pair's block of the chunk
+        if (active && key0 < wave_max) step(buf, buf + TILE, KEYS ? grp : 0, key0);
+        if (more) stage.put(bufs[(c - c0 + 1) & 1]);
         __syncthreads();
     }
 
-    const float l_tot[2] = {both_sum(l_run[0]), both_sum(l_run[1])};
+    const float l_tot = MSUM ? l_acc[0] : both_sum(l_run);           // each element of l_acc holds the lane's whole sum
+    const float inv = l_tot > 0.f || l_tot != l_tot ? 1.0f / l_tot : 0.f;
     const int64_t orow = (((int64_t)b * a.nq + place.tok) * a.heads + place.head) * 2 * a.d;
     const int64_t lrow = ((int64_t)b * a.heads + place.head) * a.nq + place.tok;
     const int64_t lmap = (int64_t)a.batch * a.heads * a.nq;
@@ -212,87 +189,89 @@ __global__ __launch_bounds__(NW * 64, KEYS || sizeof(T) == 4 ? 1 : 2) void diff_
     T* out2 = reinterpret_cast<T*>(o.out2);
 
     if constexpr (!KEYS) {
-        if (row >= nrows) return;
-        const float i1 = l_tot[0] > 0.f || l_tot[0] != l_tot[0] ? 1.0f / l_tot[0] : 0.f;
-        const float i2 = l_tot[1] > 0.f || l_tot[1] != l_tot[1] ? 1.0f / l_tot[1] : 0.f;
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int col = d * 32 + 8 * g + 4 * hh;
-                if (col >= 2 * a.d) continue;
-                f32x4 x, y;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    y[j] = acc[1][d][4 * g + j] * i2;
-                    x[j] = fmaf(-weight, y[j], acc[0][d][4 * g + j] * i1);
-                }
-                store4(out + orow + col, x);
-                if (out2) store4(out2 + orow + col, y);
-            }
-        if (out2 && hh == 0) {
-            o.stats[lrow] = l_tot[0] == 0.f ? 0.f : m_run[0];
-            o.stats[lmap + lrow] = l_tot[1] == 0.f ? 0.f : m_run[1];
-            o.stats[2 * lmap + lrow] = i1;
-            o.stats[3 * lmap + lrow] = i2;
-            if (b == 0 && place.tok == 0) o.weight[place.head] = weight;
+        const bool live = row < nrows;
+        if (TRAIN && live && hh == 0) {
+            o.stats[map * lmap + lrow] = l_tot == 0.f ? 0.f : m_run;
+            o.stats[(2 + map) * lmap + lrow] = inv;
+            if (map == 0 && b == 0 && place.tok == 0) o.weight[place.head] = weight;
         }
-    } else {
-        // join the waves' keys
-        if (hh == 0) {
-            s_ml[wave][0][r] = m_run[0];
-            s_ml[wave][1][r] = l_tot[0];
-            s_ml[wave][2][r] = m_run[1];
-            s_ml[wave][3][r] = l_tot[1];
-            if (wave == 0) s_w[r] = weight;
-        }
-        __syncthreads();
-        float top[2], sum[2] = {0.f, 0.f};
+        // the second map's wave hands its sums over, as many 32-column blocks at a time as the buffers hold
+        constexpr int FIT = 4 * TILE / (NG * 4096) < DB ? 4 * TILE / (NG * 4096) : DB;
+        static_assert(FIT >= 1, "one block of columns fits the buffers");
+        f32x4* box = reinterpret_cast<f32x4*>(bufs[0]) + grp * FIT * 256 + hh * 32 + r;
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            top[m] = s_ml[0][2 * m][r];
+        for (int d0 = 0; d0 < DB; d0 += FIT) {
+            if (d0) __syncthreads();
+            if (map == 1) {
 #pragma unroll
-            for (int w = 1; w < NW; ++w) top[m] = fmaxf(top[m], s_ml[w][2 * m][r]);
-#pragma unroll
-            for (int w = 0; w < NW; ++w) sum[m] += s_ml[w][2 * m + 1][r] * __builtin_amdgcn_exp2f(s_ml[w][2 * m][r] - top[m]);
-        }
-        constexpr int HALF = NW / 2;
-        float* mine = reinterpret_cast<float*>(bufs[wave < HALF ? 0 : 1]) + (wave % HALF) * 32 * 2 * DV;
-        static_assert(HALF * 32 * 2 * DV * 4 <= 2 * TILE, "the waves' rows fit the buffers");
-        if (row < nrows) {
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                const float f = __builtin_amdgcn_exp2f(m_run[m] - top[m]);
-#pragma unroll
-                for (int d = 0; d < DB; ++d)
+                for (int d = d0; d < d0 + FIT && d < DB; ++d)
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
+                        const f32x4 y = {acc[d][4 * g] * inv, acc[d][4 * g + 1] * inv, acc[d][4 * g + 2] * inv, acc[d][4 * g + 3] * inv};
+                        box[(d - d0) * 256 + g * 64] = y;
+                        const int col = d * 32 + 8 * g + 4 * hh;
+                        if (TRAIN && live && col < 2 * a.d) store4(out2 + orow + col, y);
+                    }
+            }
+            __syncthreads();
+            if (map == 0 && live) {
+#pragma unroll
+                for (int d = d0; d < d0 + FIT && d < DB; ++d)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const int col = d * 32 + 8 * g + 4 * hh;
+                        if (col >= 2 * a.d) continue;
+                        const f32x4 y = box[(d - d0) * 256 + g * 64];
                         f32x4 x;
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) x[j] = acc[m][d][4 * g + j] * f;
-                        *reinterpret_cast<f32x4*>(mine + joined<DV>(r, m, d * 32 + 8 * g + 4 * hh)) = x;
+                        for (int j = 0; j < 4; ++j) x[j] = fmaf(-weight, y[j], acc[d][4 * g + j] * inv);
+                        store4(out + orow + col, x);
                     }
             }
         }
+    } else {
+        // join the pairs' keys
+        if (hh == 0) {
+            s_ml[grp][2 * map][r] = m_run;
+            s_ml[grp][2 * map + 1][r] = l_tot;
+            if (wave == 0) s_w[r] = weight;
+        }
         __syncthreads();
-        if (wave == 0 && hh == 0) {                                  // the joined maximum and sum take the first wave's place
-            s_ml[0][0][r] = top[0];
-            s_ml[0][1][r] = sum[0];
-            s_ml[0][2][r] = top[1];
-            s_ml[0][3][r] = sum[1];
+        float top = s_ml[0][2 * map][r], sum = 0.f;
+#pragma unroll
+        for (int w = 1; w < NG; ++w) top = fmaxf(top, s_ml[w][2 * map][r]);
+#pragma unroll
+        for (int w = 0; w < NG; ++w) sum += s_ml[w][2 * map + 1][r] * __builtin_amdgcn_exp2f(s_ml[w][2 * map][r] - top);
+        constexpr int HALF = NG / 2;
+        static_assert(HALF * 32 * 2 * DV * 4 <= 2 * TILE, "the pairs' rows fit the buffers");
+        float* mine = reinterpret_cast<float*>(bufs[grp < HALF ? 0 : 1]) + (grp % HALF) * 32 * 2 * DV;
+        if (row < nrows) {
+            const float f = __builtin_amdgcn_exp2f(m_run - top);
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const f32x4 x = {acc[d][4 * g] * f, acc[d][4 * g + 1] * f, acc[d][4 * g + 2] * f, acc[d][4 * g + 3] * f};
+                    *reinterpret_cast<f32x4*>(mine + joined<DV>(r, map, d * 32 + 8 * g + 4 * hh)) = x;
+                }
+        }
+        __syncthreads();
+        if (grp == 0 && hh == 0) {                                   // the joined maximum and sum take the first pair's place
+            s_ml[0][2 * map][r] = top;
+            s_ml[0][2 * map + 1][r] = sum;
         }
         __syncthreads();
         const int live = nrows - row0 < 32 ? nrows - row0 : 32;
         const int64_t part = ((int64_t)bk * tiles + tile) * splits + split;
         float* wo = ws + part * 32 * (2 * DV + 4);
-        for (int i = tid; i < live * (DV / 4); i += NW * 64) {
+        for (int i = tid; i < live * (DV / 4); i += NT) {
             const int rr = i / (DV / 4), col = (i - rr * (DV / 4)) * 4;
             f32x4 x[2];
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
                 x[m] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int w = 0; w < NW; ++w)
+                for (int w = 0; w < NG; ++w)
                     x[m] = x[m] + *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(bufs[w < HALF ? 0 : 1]) +
                                                                   (w % HALF) * 32 * 2 * DV + joined<DV>(rr, m, col));
             }
@@ -311,84 +290,110 @@ __global__ __launch_bounds__(NW * 64, KEYS || sizeof(T) == 4 ? 1 : 2) void diff_
             for (int j = 0; j < 4; ++j) z[j] = fmaf(-w, y[j], x[0][j] * i1);
             const int64_t at = (((int64_t)b * a.nq + pl.tok) * a.heads + pl.head) * 2 * a.d + col;
             store4(out + at, z);
-            if (out2) store4(out2 + at, y);
+            if (TRAIN) store4(out2 + at, y);
         }
-        if (wave == 0 && row < nrows && hh == 0) {
+        if (grp == 0 && row < nrows && hh == 0) {
             if (splits > 1) {
                 float* ml = wo + 32 * 2 * DV + r * 4;
-                ml[0] = top[0];
-                ml[1] = sum[0];
-                ml[2] = top[1];
-                ml[3] = sum[1];
-            } else if (out2) {
-#pragma unroll
-                for (int m = 0; m < 2; ++m) {
-                    o.stats[m * lmap + lrow] = sum[m] == 0.f ? 0.f : top[m];
-                    o.stats[(2 + m) * lmap + lrow] = sum[m] == 0.f ? 0.f : 1.0f / sum[m];
-                }
-                if (b == 0 && place.tok == 0) o.weight[place.head] = weight;
+                ml[2 * map] = top;
+                ml[2 * map + 1] = sum;
+            } else if (TRAIN) {
+                o.stats[map * lmap + lrow] = sum == 0.f ? 0.f : top;
+                o.stats[(2 + map) * lmap + lrow] = sum == 0.f ? 0.f : 1.0f / sum;
+                if (map == 0 && b == 0 && place.tok == 0) o.weight[place.head] = weight;
             }
         }
     }
 }
 
-// The splits of the keys joined: a workgroup per tile of 32 rows.
+// The splits of the keys joined: a workgroup per row, 4 columns to a lane, the splits shared among as many lanes as are
+// left, two maps side by side.
 template <class T, int DV>
 __global__ __launch_bounds__(256) void diff_fwd_join(DiffArgs a, DiffOut o, const float* __restrict__ ws, int tiles,
                                                      int splits) {
-    __shared__ float s_top[2][32], s_inv[2][32], s_w[32];
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int bk = blockIdx.x / tiles, tile = blockIdx.x - bk * tiles;
-    const int b = bk / a.kv_heads, kh = bk - b * a.kv_heads;
-    const int nrows = a.nq * a.group, row0 = tile * 32;
-    const int live = nrows - row0 < 32 ? nrows - row0 : 32;
+    constexpr int CH = DV / 4, NP = 256 / (2 * CH);                  // pieces of a row, lanes that share a piece's splits
     constexpr int STRIDE = 32 * (2 * DV + 4);
+    __shared__ f32x4 s_part[NP][2][CH];
+    __shared__ float s_f[2][128];                                    // what a split's sums are scaled by
+    __shared__ float s_inv[2], s_w;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int nrows = a.nq * a.group;
+    const int bk = blockIdx.x / nrows, row = blockIdx.x - bk * nrows, tile = row >> 5, rr = row & 31;
+    const int b = bk / a.kv_heads, kh = bk - b * a.kv_heads;
+    const RowPlace pl = row_place(a, kh, row);
     const float* base = ws + ((int64_t)bk * tiles + tile) * splits * STRIDE;
-    if (tid < 64) {
-        const int r = lane & 31, hh = lane >> 5;                     // half-wave m joins map m
-        const int rr = r < live ? r : live - 1;
-        const RowPlace pl = row_place(a, kh, row0 + rr);
-        float top = kNoScore, sum = 0.f;
-        for (int s = 0; s < splits; ++s) top = fmaxf(top, base[(int64_t)s * STRIDE + 32 * 2 * DV + rr * 4 + 2 * hh]);
-        for (int s = 0; s < splits; ++s) {
-            const float* ml = base + (int64_t)s * STRIDE + 32 * 2 * DV + rr * 4 + 2 * hh;
-            sum += ml[1] * __builtin_amdgcn_exp2f(ml[0] - top);
+    // the splits' values are on their way while the factors are computed
+    const int m = tid / (CH * NP), c = tid % CH, part = tid / CH % NP;
+    const float* p = base + (int64_t)part * STRIDE + rr * 2 * DV + m * DV + c * 4;
+    f32x4 first = {0.f, 0.f, 0.f, 0.f};
+    if (tid < 2 * CH * NP && part < splits) first = *reinterpret_cast<const f32x4*>(p);
+    if (wave < 2) {                                                  // wave m joins map m's maxima and sums
+        float mx[2], l[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int s = lane + 64 * j;
+            const float* ml = base + (int64_t)s * STRIDE + 32 * 2 * DV + rr * 4 + 2 * wave;
+            mx[j] = s < splits ? ml[0] : kNoScore;
+            l[j] = s < splits ? ml[1] : 0.f;
         }
-        s_top[hh][r] = top;
-        s_inv[hh][r] = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
-        const float w = map_weight<DV / 2>(a, pl.head, hh);
-        if (hh == 0) s_w[r] = w;
-        if (o.out2 && r < live) {
-            const int64_t lmap = (int64_t)a.batch * a.heads * a.nq, at = ((int64_t)b * a.heads + pl.head) * a.nq + pl.tok;
-            o.stats[hh * lmap + at] = sum == 0.f ? 0.f : top;
-            o.stats[(2 + hh) * lmap + at] = s_inv[hh][r];
-            if (b == 0 && pl.tok == 0 && hh == 0) o.weight[pl.head] = w;
+        float top = fmaxf(mx[0], mx[1]);
+#pragma unroll
+        for (int sh = 32; sh > 0; sh >>= 1) top = fmaxf(top, __shfl_xor(top, sh, 64));
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const float f = __builtin_amdgcn_exp2f(mx[j] - top);
+            s_f[wave][lane + 64 * j] = f;
+            sum = fmaf(l[j], f, sum);
+        }
+        sum = wave_sum(sum);
+        const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
+        if (lane == 0) {
+            s_inv[wave] = inv;
+            if (o.out2) {
+                const int64_t lmap = (int64_t)a.batch * a.heads * a.nq, at = ((int64_t)b * a.heads + pl.head) * a.nq + pl.tok;
+                o.stats[wave * lmap + at] = sum == 0.f ? 0.f : top;
+                o.stats[(2 + wave) * lmap + at] = inv;
+            }
+        }
+    } else if (wave == 2) {
+        const float w = map_weight<DV / 2>(a, pl.head, lane >> 5);
+        if (lane == 0) {
+            s_w = w;
+            if (o.out2 && b == 0 && pl.tok == 0) o.weight[pl.head] = w;
         }
     }
     __syncthreads();
-    for (int i = tid; i < live * (DV / 4); i += 256) {
-        const int rr = i / (DV / 4), col = (i - rr * (DV / 4)) * 4;
-        if (col >= 2 * a.d) continue;
-        f32x4 x[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
-        for (int s = 0; s < splits; ++s) {
-            const float* p = base + (int64_t)s * STRIDE;
+    if (tid < 2 * CH * NP) {
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+        if (part < splits) {
+            const float f = s_f[m][part];
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                const float f = __builtin_amdgcn_exp2f(p[32 * 2 * DV + rr * 4 + 2 * m] - s_top[m][rr]);
-                const f32x4 v = *reinterpret_cast<const f32x4*>(p + rr * 2 * DV + m * DV + col);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x[m][j] = fmaf(v[j], f, x[m][j]);
-            }
+            for (int j = 0; j < 4; ++j) x[j] = first[j] * f;
         }
-        const RowPlace pl = row_place(a, kh, row0 + rr);
-        const f32x4 y = x[1] * s_inv[1][rr];
-        f32x4 z;
+        for (int s = part + NP; s < splits; s += NP) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(p + (int64_t)(s - part) * STRIDE);
+            const float f = s_f[m][s];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) z[j] = fmaf(-s_w[rr], y[j], x[0][j] * s_inv[0][rr]);
-        const int64_t at = (((int64_t)b * a.nq + pl.tok) * a.heads + pl.head) * 2 * a.d + col;
-        store4(reinterpret_cast<T*>(o.out) + at, z);
-        if (o.out2) store4(reinterpret_cast<T*>(o.out2) + at, y);
+            for (int j = 0; j < 4; ++j) x[j] = fmaf(v[j], f, x[j]);
+        }
+        s_part[part][m][c] = x;
     }
+    __syncthreads();
+    if (tid >= CH || 4 * tid >= 2 * a.d) return;
+    f32x4 x1 = s_part[0][0][tid], x2 = s_part[0][1][tid];
+#pragma unroll
+    for (int j = 1; j < NP; ++j) {
+        x1 = x1 + s_part[j][0][tid];
+        x2 = x2 + s_part[j][1][tid];
+    }
+    const f32x4 y = x2 * s_inv[1];
+    f32x4 z;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) z[j] = fmaf(-s_w, y[j], x1[j] * s_inv[0]);
+    const int64_t at = (((int64_t)b * a.nq + pl.tok) * a.heads + pl.head) * 2 * a.d + 4 * tid;
+    store4(reinterpret_cast<T*>(o.out) + at, z);
+    if (o.out2) store4(reinterpret_cast<T*>(o.out2) + at, y);
 }
 
 struct Plan {
@@ -396,18 +401,19 @@ struct Plan {
     int tiles, splits;
 };
 
-// Which form, and into how many workgroups.  Few rows (at most 32 to a key head), or so few workgroups of 128 rows that
-// most of the 256 CUs would have none: the waves share the rows and split the keys.
+// Which form, and into how many workgroups.  At most 32 rows to a key head, or at most one block of 32 rows to each of the
+// 256 CUs: the pairs share the rows and split the keys.  Measured, keys split / not: 64 rows, 2048 keys, 128 key heads of
+// size 64 (256 blocks) 50 / 105 us, 256 heads (512 blocks) 105 / 108; 577 rows and keys, 16 heads of 64 (304) 29.2 / 27.4.
 template <class T, int DP>
 Plan plan(const DiffArgs& a) {
     const int64_t nrows = (int64_t)a.nq * a.group, bks = (int64_t)a.batch * a.kv_heads;
     Plan p;
-    const int64_t wide = bks * ((nrows + 127) / 128);
-    p.keys = nrows <= 32 || wide < 128;
-    p.tiles = (int)(p.keys ? (nrows + 31) / 32 : (nrows + 127) / 128);
+    p.keys = nrows <= 32 || bks * ((nrows + 31) / 32) <= 256;
+    constexpr int R = 32 * rows_pairs<T, DP>();
+    p.tiles = (int)(p.keys ? (nrows + 31) / 32 : (nrows + R - 1) / R);
     p.splits = 1;
     if (p.keys) {
-        const int kc = 32 * keys_waves<T, DP>();
+        const int kc = 32 * keys_pairs<T, DP>();
         const int64_t chunks = ((int64_t)a.nk + kc - 1) / kc, blocks = bks * p.tiles;
         int64_t s = (256 + blocks - 1) / blocks;
         if (s > chunks) s = chunks;
@@ -428,12 +434,18 @@ hipError_t launch(const DiffArgs& a, const DiffOut& o, float* ws, hipStream_t s)
     const Plan p = plan<T, DP>(a);
     const int64_t blocks = (int64_t)a.batch * a.kv_heads * p.tiles * p.splits;
     if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
-    constexpr int NK = keys_waves<T, DP>();
-    if (p.keys) hipLaunchKernelGGL((diff_fwd<T, DP, NK, true>), dim3((int)blocks), dim3(NK * 64), 0, s, a, o, ws, p.tiles, p.splits);
-    else hipLaunchKernelGGL((diff_fwd<T, DP, 4, false>), dim3((int)blocks), dim3(256), 0, s, a, o, ws, p.tiles, 1);
+    constexpr int NK = keys_pairs<T, DP>(), OCCK = NK == 4 ? 2 : 1;
+    constexpr int NG = rows_pairs<T, DP>(), OCC = sizeof(T) == 4 ? 2 : DP == 32 ? 4 : 3;
+    const dim3 grid((int)blocks), kb(NK * 128), rb(NG * 128);
+    if (p.keys && o.out2) hipLaunchKernelGGL((diff_fwd<T, DP, NK, true, true, OCCK>), grid, kb, 0, s, a, o, ws, p.tiles, p.splits);
+    else if (p.keys) hipLaunchKernelGGL((diff_fwd<T, DP, NK, true, false, OCCK>), grid, kb, 0, s, a, o, ws, p.tiles, p.splits);
+    else if (o.out2) hipLaunchKernelGGL((diff_fwd<T, DP, NG, false, true, OCC>), grid, rb, 0, s, a, o, ws, p.tiles, 1);
+    else hipLaunchKernelGGL((diff_fwd<T, DP, NG, false, false, OCC>), grid, rb, 0, s, a, o, ws, p.tiles, 1);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits == 1) return e;
-    hipLaunchKernelGGL((diff_fwd_join<T, 2 * DP>), dim3(a.batch * a.kv_heads * p.tiles), dim3(256), 0, s, a, o, ws, p.tiles, p.splits);
+    const int64_t rows = (int64_t)a.batch * a.heads * a.nq;
+    if (rows > 0x7FFFFFFF) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((diff_fwd_join<T, 2 * DP>), dim3((int)rows), dim3(256), 0, s, a, o, ws, p.tiles, p.splits);
     return hipGetLastError();
 }
 

@@ -7,29 +7,20 @@
 //     dQ_m = scale dS_m K_m,  dK_m = scale dS_m^T Q_m,  dV = (P_1 - w P_2)^T dO
 //     dw_h = - sum over the head's rows and keys of P_2 dA
 // Two kernels, so that nothing is added by atomics and results are reproducible: one walks the keys for 128 rows (dQ, and
-// the row's share of dw), one walks the rows for 128 keys (dK, dV; the rows of all query heads of a key head, so that shared
+// the row's share of dw), one walks the rows for 128 keys (64 and 64 in f32: dK, dV; the rows of all query heads of a key head, so that shared
 // heads need no sum of their own).  dw is added from f32 probabilities and f32 accumulators, not from the rounded O_2.
+// As in the forward a pair of waves shares 32 rows or keys, one map each: dA is computed by both, everything else once, and
+// the registers that leaves allow two waves and more to a SIMD, which hide each other's waiting (one wave with both maps
+// took 2.3 times as long at 577 tokens of head size 48, most of it waiting).
 #include <type_traits>
 
 #include "diff_attention.h"
-
-#ifndef KVOCC
-#define KVOCC 1
-#endif
-#ifndef KVRC
-#define KVRC 32
-#endif
 
 namespace vitk {
 
 using namespace diff;
 
 namespace {
-
-constexpr int kNW = 4;                        // waves of a workgroup, 32 rows or keys each
-constexpr int kBlock = 32 * kNW;
-
-constexpr int pow2_below(int n) { return n >= 16 ? 16 : n >= 8 ? 8 : n >= 4 ? 4 : n >= 2 ? 2 : 1; }
 
 __device__ __forceinline__ int sample_len(const DiffArgs& a, int b) {
     if (!a.key_lens) return a.nk;
@@ -45,60 +36,41 @@ __device__ __forceinline__ float dot(typename Op<T>::Chunk x, typename Op<T>::Ch
     return s;
 }
 
-// dQ of 128 rows, their D_m (ws_d [2, batch, heads, nq]) and the workgroup's share of every head's dw (ws_w)
-template <class T, int DP>
-__global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void diff_bwd_q(DiffArgs a, DiffGrads g, float* __restrict__ ws_d,
-                                                                          float* __restrict__ ws_w, int tiles) {
+// dQ of 32 NP rows, their D_m (ws_d [2, batch, heads, nq]) and the workgroup's share of every head's dw (ws_w)
+// NP: pairs of waves in a workgroup, 32 rows each; OCC: waves to a SIMD that the registers have to allow
+template <class T, int DP, int NP, int NB, int OCC>
+__global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_q(DiffArgs a, DiffGrads g, float* __restrict__ ws_d,
+                                                             float* __restrict__ ws_w, int tiles) {
+    constexpr int kThreads = NP * 128, kBlock = NP * 32;
     constexpr int DV = 2 * DP;
     constexpr int RB = row_bytes<T, DV>();
     constexpr int PER = Op<T>::kPer;
     constexpr int DPC = DP / PER, KT = DPC / 2;
     constexpr int EB = (DP + 31) / 32;
-    constexpr int KC = 32, TILE = KC * RB;
+    constexpr int KC = 32 * NB, TILE = KC * RB;                       // KC: keys of a chunk
     typedef typename Op<T>::Chunk Chunk;
     __shared__ __align__(16) char bufs[2][2 * TILE];
     __shared__ float s_dw[kBlock];
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), map = wave & 1, grp = wave >> 1;
     const int r = lane & 31, hh = lane >> 5;
     const int bks = a.batch * a.kv_heads;
     const int bk = blockIdx.x % bks, rest = blockIdx.x / bks;
     const int tile = a.causal ? tiles - 1 - rest : rest;
     const int b = bk / a.kv_heads, kh = bk - b * a.kv_heads;
     const int nrows = a.nq * a.group;
-    const int row0 = tile * kBlock + wave * 32, end = (tile + 1) * kBlock;
+    const int row0 = tile * kBlock + grp * 32, end = (tile + 1) * kBlock;
     const int len = sample_len(a, b);
     const int kmax = key_limit(a, len, row_place(a, kh, (end < nrows ? end : nrows) - 1).tok);
 
-    constexpr int LANES = 4 * DPC;
-    constexpr int ROWS = pow2_below(256 / LANES);
-    constexpr int PASSES = KC / ROWS;
     const int dc = a.d / PER;
-    const int srow = tid / LANES, scol = tid - srow * LANES;
-    const bool s_v = scol >= 2 * DPC;
-    const int s_c = s_v ? scol - 2 * DPC : scol;
-    const int s_m = !s_v && s_c >= DPC ? 1 : 0, s_e = s_c - s_m * DPC;
-    const bool s_on = srow < ROWS && (s_v ? s_c < 2 * dc : s_e < dc);
-    const int64_t s_step = s_v ? a.vs[1] : a.ks[1];
-    const T* s_src = s_v ? reinterpret_cast<const T*>(a.v) + b * a.vs[0] + kh * a.vs[2] + s_c * PER
-                         : reinterpret_cast<const T*>(a.k) + b * a.ks[0] + kh * a.ks[2] + s_m * a.ks[3] + s_e * PER;
-    u32x4 held[PASSES];
-    auto fetch = [&](int key0) {
-#pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
-            const int key = key0 + srow + i * ROWS;
-            held[i] = u32x4{0u, 0u, 0u, 0u};
-            if (s_on && key < kmax) held[i] = *reinterpret_cast<const u32x4*>(s_src + key * s_step);
-        }
-    };
-    auto put = [&](char* buf) {
-        if (srow >= ROWS) return;
-#pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
-            const int lr = srow + i * ROWS;
-            *reinterpret_cast<u32x4*>(buf + (s_v ? TILE : 0) + lr * RB + ((s_c ^ swz<RB>(lr)) << 4)) = held[i];
-        }
-    };
+    Stage<T, DP, kThreads, KC> stage;
+    stage.init(tid, dc, bufs[0]);
+    const int64_t s_step = stage.second ? a.vs[1] : a.ks[1];
+    const T* s_src = stage.second ? reinterpret_cast<const T*>(a.v) + b * a.vs[0] + kh * a.vs[2] + stage.col * PER
+                                  : reinterpret_cast<const T*>(a.k) + b * a.ks[0] + kh * a.ks[2] + stage.map * a.ks[3] + stage.e * PER;
+    auto fetch = [&](int key0) { stage.fetch(key0, kmax, [&](int key) { return s_src + key * s_step; }); };
     const int c1 = (kmax + KC - 1) / KC;
     if (c1 > 0) fetch(0);
 
@@ -111,20 +83,17 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void diff_bwd_q(DiffAr
     const int64_t lrow = ((int64_t)b * a.heads + place.head) * a.nq + place.tok;
     const int64_t lmap = (int64_t)a.batch * a.heads * a.nq;
     const float weight = g.weight[place.head];
-    const float ref[2] = {g.stats[lrow], g.stats[lmap + lrow]};
-    const float inv[2] = {g.stats[2 * lmap + lrow], g.stats[3 * lmap + lrow]};
+    const float ref = g.stats[map * lmap + lrow], inv = g.stats[(2 + map) * lmap + lrow];
 
-    Chunk qf[2][KT], of[2 * KT];
-    float dd[2];
+    Chunk qf[KT], of[2 * KT];
+    float dd;
     {
-        const T* qg = reinterpret_cast<const T*>(a.q) + b * a.qs[0] + place.tok * a.qs[1] + place.head * a.qs[2];
+        const T* qg = reinterpret_cast<const T*>(a.q) + b * a.qs[0] + place.tok * a.qs[1] + place.head * a.qs[2] + map * a.qs[3];
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int t = 0; t < KT; ++t) {
-                const int c = 2 * t + hh;
-                qf[m][t] = *reinterpret_cast<const Chunk*>(c < dc ? (const void*)(qg + m * a.qs[3] + c * PER) : (const void*)kZeros);
-            }
+        for (int t = 0; t < KT; ++t) {
+            const int c = 2 * t + hh;
+            qf[t] = *reinterpret_cast<const Chunk*>(c < dc ? (const void*)(qg + c * PER) : (const void*)kZeros);
+        }
         const int64_t orow = (((int64_t)b * a.nq + place.tok) * a.heads + place.head) * 2 * a.d;
         float d0 = 0.f, d2 = 0.f;
 #pragma unroll
@@ -135,78 +104,67 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void diff_bwd_q(DiffAr
                 return *reinterpret_cast<const Chunk*>(on ? (const void*)(reinterpret_cast<const T*>(p) + orow + c * PER) : (const void*)kZeros);
             };
             of[t] = at(g.dout);
-            d0 += dot<T>(of[t], at(g.out));
             d2 += dot<T>(of[t], at(g.out2));
+            if (map == 0) d0 += dot<T>(of[t], at(g.out));
         }
-        dd[1] = both_sum(d2);
-        dd[0] = fmaf(weight, dd[1], both_sum(d0));
-        if (row < nrows && hh == 0) {
-            ws_d[lrow] = dd[0];
-            ws_d[lmap + lrow] = dd[1];
-        }
+        dd = both_sum(d2);
+        if (map == 0) dd = fmaf(weight, dd, both_sum(d0));
+        if (row < nrows && hh == 0) ws_d[map * lmap + lrow] = dd;
     }
 
-    f32x16 dq[2][EB];
+    f32x16 dq[EB];
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int e = 0; e < EB; ++e) dq[m][e] = zero16();
+    for (int e = 0; e < EB; ++e) dq[e] = zero16();
     float dw = 0.f;
     const float sc = a.scale * kLog2e;
 
-    if (c1 > 0) put(bufs[0]);
+    if (c1 > 0) stage.put(bufs[0]);
     __syncthreads();
     for (int c = 0; c < c1; ++c) {
         const char* kt = bufs[c & 1];
         const char* vt = kt + TILE;
         const bool more = c + 1 < c1;
         if (more) fetch((c + 1) * KC);
-        const int key0 = c * KC;
-        if (active && key0 < wave_max) {
-            f32x16 s[2], da = zero16();
+#pragma unroll 2
+        for (int kb = 0; kb < KC; kb += 32) {
+            const int key0 = c * KC + kb;
+            if (!active || key0 >= wave_max) break;
+            f32x16 s = zero16(), da = zero16();
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                s[m] = zero16();
+            for (int t = 0; t < KT; ++t) s = Op<T>::mma(chunk_at<T, RB>(kt, kb + r, map * DPC + 2 * t + hh), qf[t], s);
 #pragma unroll
-                for (int t = 0; t < KT; ++t) s[m] = Op<T>::mma(chunk_at<T, RB>(kt, r, m * DPC + 2 * t + hh), qf[m][t], s[m]);
-            }
-#pragma unroll
-            for (int t = 0; t < 2 * KT; ++t) da = Op<T>::mma(chunk_at<T, RB>(vt, r, 2 * t + hh), of[t], da);
+            for (int t = 0; t < 2 * KT; ++t) da = Op<T>::mma(chunk_at<T, RB>(vt, kb + r, 2 * t + hh), of[t], da);
             if (key0 + 32 > wave_min) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (key0 + 8 * (i >> 2) + 4 * hh + (i & 3) >= lim) s[0][i] = s[1][i] = -__builtin_inff();
+                    if (key0 + 8 * (i >> 2) + 4 * hh + (i & 3) >= lim) s[i] = -__builtin_inff();
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const float p1 = __builtin_amdgcn_exp2f(fmaf(s[0][i], sc, -ref[0]));       // times 1 / l at the end
-                const float p2 = __builtin_amdgcn_exp2f(fmaf(s[1][i], sc, -ref[1]));
-                dw = fmaf(p2, da[i], dw);
-                s[0][i] = p1 * (da[i] - dd[0]);
-                s[1][i] = p2 * (da[i] - dd[1]);
+                const float p = __builtin_amdgcn_exp2f(fmaf(s[i], sc, -ref));     // times 1 / l at the end
+                dw = fmaf(p, da[i], dw);
+                s[i] = p * (da[i] - dd);
             }
 #pragma unroll
-            for (int st = 0; st < 2; ++st)
+            for (int st = 0; st < 2; ++st) {
+                Slice<T> ds;
+                ds.take(s, st);
 #pragma unroll
-                for (int m = 0; m < 2; ++m) {
-                    Slice<T> ds;
-                    ds.take(s[m], st);
-#pragma unroll
-                    for (int e = 0; e < EB; ++e) {
-                        Trans<T, RB> k;
-                        k.load(kt, 16 * st, m * DP + e * 32, lane);
-                        dq[m][e] = mma_t(k, ds, dq[m][e]);
-                    }
+                for (int e = 0; e < EB; ++e) {
+                    Trans<T, RB> k;
+                    k.load(kt, kb + 16 * st, map * DP + e * 32, lane);
+                    dq[e] = mma_t(k, ds, dq[e]);
                 }
+            }
         }
-        if (more) put(bufs[(c + 1) & 1]);
+        if (more) stage.put(bufs[(c + 1) & 1]);
         __syncthreads();
     }
 
-    dw = both_sum(dw) * inv[1];
-    if (hh == 0) s_dw[wave * 32 + r] = row < nrows ? -dw : 0.f;
+    dw = both_sum(dw) * inv;
+    if (map == 1 && hh == 0) s_dw[grp * 32 + r] = row < nrows ? -dw : 0.f;
     __syncthreads();
-    for (int h = tid; h < a.group; h += 256) {
+    for (int h = tid; h < a.group; h += kThreads) {
         // rows of the workgroup that belong to the group's head h
         const int first = tile * kBlock;
         float t = 0.f;
@@ -214,44 +172,46 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void diff_bwd_q(DiffAr
         ws_w[((int64_t)bk * tiles + tile) * a.group + h] = t;
     }
     if (row >= nrows) return;
-    T* out = reinterpret_cast<T*>(g.dq) + b * g.dqs[0] + place.tok * g.dqs[1] + place.head * g.dqs[2];
+    T* out = reinterpret_cast<T*>(g.dq) + b * g.dqs[0] + place.tok * g.dqs[1] + place.head * g.dqs[2] + map * g.dqs[3];
+    const float f = map == 0 ? inv * a.scale : -weight * inv * a.scale;
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
-        const float f = m == 0 ? inv[0] * a.scale : -weight * inv[1] * a.scale;
+    for (int e = 0; e < EB; ++e)
 #pragma unroll
-        for (int e = 0; e < EB; ++e)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int col = e * 32 + 8 * q + 4 * hh;
-                if (col >= a.d) continue;
-                store4(out + m * g.dqs[3] + col,
-                       f32x4{dq[m][e][4 * q] * f, dq[m][e][4 * q + 1] * f, dq[m][e][4 * q + 2] * f, dq[m][e][4 * q + 3] * f});
-            }
-    }
+        for (int q = 0; q < 4; ++q) {
+            const int col = e * 32 + 8 * q + 4 * hh;
+            if (col >= a.d) continue;
+            store4(out + col, f32x4{dq[e][4 * q] * f, dq[e][4 * q + 1] * f, dq[e][4 * q + 2] * f, dq[e][4 * q + 3] * f});
+        }
 }
 
-// dK and dV of 128 keys
-template <class T, int DP, int RC>
-__global__ __launch_bounds__(256, KVOCC) void diff_bwd_kv(DiffArgs a, DiffGrads g, const float* __restrict__ ws_d, int tiles) {
+// dK and dV of 32 NP keys.  What a row contributes beside its Q and dO is folded into the products' initial accumulators:
+//     S_m starts at -lse_m / (scale log2 e), so that P_m = exp2(scale log2(e) S_m);  dA starts at -D_m.
+// ONE: one query head to a key head, so that w is the workgroup's and can wait until the end (else the rows bring theirs).
+template <class T, int DP, bool ONE, int NP, int NB, int OCC>
+__global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_kv(DiffArgs a, DiffGrads g, const float* __restrict__ ws_d, int tiles) {
+    constexpr int kThreads = NP * 128, kBlock = NP * 32;
     constexpr int DV = 2 * DP;
     constexpr int RB = row_bytes<T, DV>();
     constexpr int PER = Op<T>::kPer;
     constexpr int DPC = DP / PER, KT = DPC / 2;
     constexpr int DB = DV / 32, EB = (DP + 31) / 32;
-    constexpr int TILE = RC * RB;                                     // RC: rows of a chunk
+    constexpr int RC = 32 * NB, TILE = RC * RB;                       // RC: rows of a chunk
+    constexpr int NS = ONE ? 4 : 5;
     typedef typename Op<T>::Chunk Chunk;
     __shared__ __align__(16) char bufs[2][2 * TILE];                  // Q of both maps, dO
-    __shared__ __align__(16) float s_row[2][6][RC];                   // m_1, m_2, 1 / l_1, w / l_2, D_1, D_2 of the rows
+    __shared__ __align__(16) float s_row[2][NS][RC];                  // -lse_1 / sc, -lse_2 / sc, -D_1, -D_2, w
     __shared__ __align__(16) int s_lim[2][RC];
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), map = wave & 1, grp = wave >> 1;
     const int r = lane & 31, hh = lane >> 5;
     const int bks = a.batch * a.kv_heads;
-    const int bk = blockIdx.x % bks, tile = blockIdx.x / bks;
+    const int bk = blockIdx.x % bks, tile = blockIdx.x / bks;        // causal: the first keys have the most rows
     const int b = bk / a.kv_heads, kh = bk - b * a.kv_heads;
     const int nrows = a.nq * a.group;
     const int len = sample_len(a, b);
-    const int block0 = tile * kBlock, key0 = block0 + wave * 32, key = key0 + r;
+    const int block0 = tile * kBlock, key0 = block0 + grp * 32, key = key0 + r;
+    const float sc = a.scale * kLog2e, rsc = 1.0f / sc;
     // rows from the first one that sees a key of this workgroup
     int first = 0;
     if (a.causal) {
@@ -260,78 +220,60 @@ __global__ __launch_bounds__(256, KVOCC) void diff_bwd_kv(DiffArgs a, DiffGrads 
     }
     const int c1 = block0 < len ? (nrows + RC - 1) / RC : 0;
 
-    constexpr int LANES = 4 * DPC;
-    constexpr int ROWS = pow2_below(256 / LANES);
-    constexpr int PASSES = RC / ROWS;
     const int dc = a.d / PER;
-    const int srow = tid / LANES, scol = tid - srow * LANES;
-    const bool s_o = scol >= 2 * DPC;
-    const int s_c = s_o ? scol - 2 * DPC : scol;
-    const int s_m = !s_o && s_c >= DPC ? 1 : 0, s_e = s_c - s_m * DPC;
-    const bool s_on = srow < ROWS && (s_o ? s_c < 2 * dc : s_e < dc);
-    const T* qg = reinterpret_cast<const T*>(a.q) + b * a.qs[0] + s_m * a.qs[3] + s_e * PER;
-    const T* og = reinterpret_cast<const T*>(g.dout) + (int64_t)b * a.nq * a.heads * 2 * a.d + s_c * PER;
+    Stage<T, DP, kThreads, RC> stage;
+    stage.init(tid, dc, bufs[0]);
+    const int64_t s_tok = stage.second ? (int64_t)a.heads * 2 * a.d : a.qs[1], s_head = stage.second ? 2 * a.d : a.qs[2];
+    const T* s_src = stage.second ? reinterpret_cast<const T*>(g.dout) + (int64_t)b * a.nq * a.heads * 2 * a.d + stage.col * PER
+                                  : reinterpret_cast<const T*>(a.q) + b * a.qs[0] + stage.map * a.qs[3] + stage.e * PER;
+    if (ONE) s_src += kh * s_head;
     const int64_t lmap = (int64_t)a.batch * a.heads * a.nq;
-    u32x4 held[PASSES];
-    float held_r[6];
+    float held_r[NS];
     int held_l = 0;
     auto fetch = [&](int c) {
-#pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
-            const int row = c * RC + srow + i * ROWS;
-            held[i] = u32x4{0u, 0u, 0u, 0u};
-            if (s_on && row < nrows) {
-                const RowPlace pl = row_place(a, kh, row);
-                const T* src = s_o ? og + ((int64_t)pl.tok * a.heads + pl.head) * 2 * a.d : qg + pl.tok * a.qs[1] + pl.head * a.qs[2];
-                held[i] = *reinterpret_cast<const u32x4*>(src);
-            }
-        }
+        stage.fetch(c * RC, nrows, [&](int row) {
+            if constexpr (ONE) return s_src + row * s_tok;
+            const RowPlace pl = row_place(a, kh, row);
+            return s_src + pl.tok * s_tok + pl.head * s_head;
+        });
         if (tid < RC) {
             const int row = c * RC + tid;
             held_l = 0;
-#pragma unroll
-            for (int j = 0; j < 6; ++j) held_r[j] = 0.f;
+            held_r[0] = held_r[1] = -__builtin_inff();                // a row past the last one: P = 0
+            held_r[2] = held_r[3] = 0.f;
+            if constexpr (!ONE) held_r[4] = 0.f;
             if (row < nrows) {
-                const RowPlace pl = row_place(a, kh, row);
+                const RowPlace pl = ONE ? RowPlace{row, kh} : row_place(a, kh, row);
                 const int64_t at = ((int64_t)b * a.heads + pl.head) * a.nq + pl.tok;
-                held_r[0] = g.stats[at];
-                held_r[1] = g.stats[lmap + at];
-                held_r[2] = g.stats[2 * lmap + at];
-                held_r[3] = g.stats[3 * lmap + at] * g.weight[pl.head];
-                held_r[4] = ws_d[at];
-                held_r[5] = ws_d[lmap + at];
+                held_r[0] = (__builtin_amdgcn_logf(g.stats[2 * lmap + at]) - g.stats[at]) * rsc;
+                held_r[1] = (__builtin_amdgcn_logf(g.stats[3 * lmap + at]) - g.stats[lmap + at]) * rsc;
+                held_r[2] = -ws_d[at];
+                held_r[3] = -ws_d[lmap + at];
+                if constexpr (!ONE) held_r[4] = g.weight[pl.head];
                 held_l = key_limit(a, len, pl.tok);
             }
         }
     };
     auto put = [&](int k) {
-        if (srow < ROWS) {
-#pragma unroll
-            for (int i = 0; i < PASSES; ++i) {
-                const int lr = srow + i * ROWS;
-                *reinterpret_cast<u32x4*>(bufs[k] + (s_o ? TILE : 0) + lr * RB + ((s_c ^ swz<RB>(lr)) << 4)) = held[i];
-            }
-        }
+        stage.put(bufs[k]);
         if (tid < RC) {
 #pragma unroll
-            for (int j = 0; j < 6; ++j) s_row[k][j][tid] = held_r[j];
+            for (int j = 0; j < NS; ++j) s_row[k][j][tid] = held_r[j];
             s_lim[k][tid] = held_l;
         }
     };
     if (first < c1) fetch(first);
 
-    Chunk kf[2][KT], vf[2 * KT];
+    Chunk kf[KT], vf[2 * KT];
     {
         const bool on = key < len;
-        const T* kg = reinterpret_cast<const T*>(a.k) + b * a.ks[0] + kh * a.ks[2] + (int64_t)(on ? key : 0) * a.ks[1];
+        const T* kg = reinterpret_cast<const T*>(a.k) + b * a.ks[0] + kh * a.ks[2] + map * a.ks[3] + (int64_t)(on ? key : 0) * a.ks[1];
         const T* vg = reinterpret_cast<const T*>(a.v) + b * a.vs[0] + kh * a.vs[2] + (int64_t)(on ? key : 0) * a.vs[1];
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int t = 0; t < KT; ++t) {
-                const int c = 2 * t + hh;
-                kf[m][t] = *reinterpret_cast<const Chunk*>(on && c < dc ? (const void*)(kg + m * a.ks[3] + c * PER) : (const void*)kZeros);
-            }
+        for (int t = 0; t < KT; ++t) {
+            const int c = 2 * t + hh;
+            kf[t] = *reinterpret_cast<const Chunk*>(on && c < dc ? (const void*)(kg + c * PER) : (const void*)kZeros);
+        }
 #pragma unroll
         for (int t = 0; t < 2 * KT; ++t) {
             const int c = 2 * t + hh;
@@ -339,64 +281,12 @@ __global__ __launch_bounds__(256, KVOCC) void diff_bwd_kv(DiffArgs a, DiffGrads 
         }
     }
 
-    f32x16 dk[2][EB], dv[DB];
+    f32x16 dk[EB], dv[DB];
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int e = 0; e < EB; ++e) dk[m][e] = zero16();
+    for (int e = 0; e < EB; ++e) dk[e] = zero16();
 #pragma unroll
     for (int d = 0; d < DB; ++d) dv[d] = zero16();
-    const float sc = a.scale * kLog2e;
 
-    auto work = [&](const char* qt, const char* ot, int k, int rb, bool masked) {
-                    f32x16 s[2], da = zero16();
-        #pragma unroll
-                    for (int m = 0; m < 2; ++m) {
-                        s[m] = zero16();
-        #pragma unroll
-                        for (int t = 0; t < KT; ++t) s[m] = Op<T>::mma(chunk_at<T, RB>(qt, rb + r, m * DPC + 2 * t + hh), kf[m][t], s[m]);
-                    }
-        #pragma unroll
-                    for (int t = 0; t < 2 * KT; ++t) da = Op<T>::mma(chunk_at<T, RB>(ot, rb + r, 2 * t + hh), vf[t], da);
-                    f32x16 pa;
-        #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const int at = rb + 8 * q + 4 * hh;
-                        auto row4 = [&](int j) { return *reinterpret_cast<const f32x4*>(&s_row[k][j][at]); };
-                        const f32x4 m1 = row4(0), m2 = row4(1), i1 = row4(2), w2 = row4(3), d1 = row4(4), d2 = row4(5);
-        #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int i = 4 * q + j;
-                            float p1 = __builtin_amdgcn_exp2f(fmaf(s[0][i], sc, -m1[j])) * i1[j];
-                            float wp2 = __builtin_amdgcn_exp2f(fmaf(s[1][i], sc, -m2[j])) * w2[j];
-                            if (masked && key >= s_lim[k][at + j]) p1 = wp2 = 0.f;
-                            pa[i] = p1 - wp2;
-                            s[0][i] = p1 * (da[i] - d1[j]);
-                            s[1][i] = wp2 * (d2[j] - da[i]);
-                        }
-                    }
-        #pragma unroll
-                    for (int st = 0; st < 2; ++st) {
-                        Slice<T> p, d0, d1;
-                        p.take(pa, st);
-                        d0.take(s[0], st);
-                        d1.take(s[1], st);
-        #pragma unroll
-                        for (int d = 0; d < DB; ++d) {
-                            Trans<T, RB> o;
-                            o.load(ot, rb + 16 * st, d * 32, lane);
-                            dv[d] = mma_t(o, p, dv[d]);
-                        }
-        #pragma unroll
-                        for (int e = 0; e < EB; ++e) {
-                            Trans<T, RB> q0, q1;
-                            q0.load(qt, rb + 16 * st, e * 32, lane);
-                            q1.load(qt, rb + 16 * st, DP + e * 32, lane);
-                            dk[0][e] = mma_t(q0, d0, dk[0][e]);
-                            dk[1][e] = mma_t(q1, d1, dk[1][e]);
-                        }
-                    }
-    };
     if (first < c1) put(0);
     __syncthreads();
     for (int c = first; c < c1; ++c) {
@@ -405,40 +295,104 @@ __global__ __launch_bounds__(256, KVOCC) void diff_bwd_kv(DiffArgs a, DiffGrads 
         const char* ot = qt + TILE;
         const bool more = c + 1 < c1;
         if (more) fetch(c + 1);
-#pragma unroll
+        // what the chunk's rows see grows with the row: nothing to do where a block's last one sees none of the wave's keys
+#pragma unroll 1
         for (int rb = 0; rb < RC; rb += 32) {
-            // the block's last row sees most: nothing to do where that is below the wave's keys
             const int at0 = c * RC + rb, last = at0 + 32 < nrows ? at0 + 32 : nrows;
-            const int most = at0 < nrows ? key_limit(a, len, row_place(a, kh, last - 1).tok) : 0;
-            const int least = at0 < nrows ? key_limit(a, len, row_place(a, kh, at0).tok) : 0;
-            if (key0 < most) work(qt, ot, k, rb, key0 + 32 > least);
+            if (at0 >= nrows) break;
+            if (key0 >= key_limit(a, len, row_place(a, kh, last - 1).tok)) continue;
+            auto rows16 = [&](int j) {                                // row values in the accumulators' layout
+                f32x16 v;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const f32x4 x = *reinterpret_cast<const f32x4*>(&s_row[k][j][rb + 8 * q + 4 * hh]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[4 * q + i] = x[i];
+                }
+                return v;
+            };
+            f32x16 s = rows16(map), da = rows16(2 + map);
+#pragma unroll
+            for (int t = 0; t < KT; ++t) s = Op<T>::mma(chunk_at<T, RB>(qt, rb + r, map * DPC + 2 * t + hh), kf[t], s);
+#pragma unroll
+            for (int t = 0; t < 2 * KT; ++t) da = Op<T>::mma(chunk_at<T, RB>(ot, rb + r, 2 * t + hh), vf[t], da);
+            if (key0 + 32 > key_limit(a, len, row_place(a, kh, at0).tok)) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (key >= s_lim[k][rb + 8 * (i >> 2) + 4 * hh + (i & 3)]) s[i] = -__builtin_inff();
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i] * sc);
+            if constexpr (!ONE) {
+                if (map == 1) s = s * rows16(NS - 1);
+            }
+#pragma unroll
+            for (int st = 0; st < 2; ++st) {
+                Slice<T> p, ds;
+                p.take(s, st);
+                f32x16 x;
+#pragma unroll
+                for (int i = 8 * st; i < 8 * st + 8; ++i) x[i] = s[i] * da[i];
+                ds.take(x, st);
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    Trans<T, RB> o;
+                    o.load(ot, rb + 16 * st, d * 32, lane);
+                    dv[d] = mma_t(o, p, dv[d]);
+                }
+#pragma unroll
+                for (int e = 0; e < EB; ++e) {
+                    Trans<T, RB> q;
+                    q.load(qt, rb + 16 * st, map * DP + e * 32, lane);
+                    dk[e] = mma_t(q, ds, dk[e]);
+                }
+            }
         }
         if (more) put(k ^ 1);
         __syncthreads();
     }
 
-    if (key >= a.nk) return;
-    T* ko = reinterpret_cast<T*>(g.dk) + b * g.dks[0] + (int64_t)key * g.dks[1] + kh * g.dks[2];
-    T* vo = reinterpret_cast<T*>(g.dv) + b * g.dvs[0] + (int64_t)key * g.dvs[1] + kh * g.dvs[2];
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
+    const bool live = key < a.nk;
+    const float f = map == 0 ? 1.f : ONE ? -g.weight[kh] : -1.f;      // the second map's part
+    if (live) {
+        T* ko = reinterpret_cast<T*>(g.dk) + b * g.dks[0] + (int64_t)key * g.dks[1] + kh * g.dks[2] + map * g.dks[3];
+        const float fk = f * a.scale;
 #pragma unroll
         for (int e = 0; e < EB; ++e)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int col = e * 32 + 8 * q + 4 * hh;
                 if (col >= a.d) continue;
-                store4(ko + m * g.dks[3] + col, f32x4{dk[m][e][4 * q] * a.scale, dk[m][e][4 * q + 1] * a.scale,
-                                                      dk[m][e][4 * q + 2] * a.scale, dk[m][e][4 * q + 3] * a.scale});
+                store4(ko + col, f32x4{dk[e][4 * q] * fk, dk[e][4 * q + 1] * fk, dk[e][4 * q + 2] * fk, dk[e][4 * q + 3] * fk});
             }
+    }
+    T* vo = reinterpret_cast<T*>(g.dv) + b * g.dvs[0] + (int64_t)key * g.dvs[1] + kh * g.dvs[2];
+    constexpr int FIT = 4 * TILE / (NP * 4096) < DB ? 4 * TILE / (NP * 4096) : DB;
+    static_assert(FIT >= 1, "one block of columns fits the buffers");
+    f32x4* box = reinterpret_cast<f32x4*>(bufs[0]) + grp * FIT * 256 + hh * 32 + r;
 #pragma unroll
-    for (int d = 0; d < DB; ++d)
+    for (int d0 = 0; d0 < DB; d0 += FIT) {
+        if (d0) __syncthreads();
+        if (map == 1) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int col = d * 32 + 8 * q + 4 * hh;
-            if (col >= 2 * a.d) continue;
-            store4(vo + col, f32x4{dv[d][4 * q], dv[d][4 * q + 1], dv[d][4 * q + 2], dv[d][4 * q + 3]});
+            for (int d = d0; d < d0 + FIT && d < DB; ++d)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    box[(d - d0) * 256 + q * 64] = f32x4{dv[d][4 * q] * f, dv[d][4 * q + 1] * f, dv[d][4 * q + 2] * f, dv[d][4 * q + 3] * f};
         }
+        __syncthreads();
+        if (map == 0 && live) {
+#pragma unroll
+            for (int d = d0; d < d0 + FIT && d < DB; ++d)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int col = d * 32 + 8 * q + 4 * hh;
+                    if (col >= 2 * a.d) continue;
+                    const f32x4 y = box[(d - d0) * 256 + q * 64];
+                    store4(vo + col, f32x4{dv[d][4 * q] + y[0], dv[d][4 * q + 1] + y[1], dv[d][4 * q + 2] + y[2], dv[d][4 * q + 3] + y[3]});
+                }
+        }
+    }
 }
 
 // dlam of one lam head from the workgroups' shares of dw: dlam_0 = dw e_1 lam_1, dlam_1 = dw e_1 lam_0, and the second
@@ -481,29 +435,42 @@ __global__ __launch_bounds__(256) void diff_bwd_lam(DiffArgs a, const float* __r
     }
 }
 
+// Pairs of a workgroup: four share the staged tiles in bf16; in f32 a lane holds twice the bytes, and two pairs leave it
+// all 512 registers.
+template <class T>
+constexpr int pairs() { return sizeof(T) == 4 ? 2 : 4; }
+
+int64_t row_tiles(const DiffArgs& a, int np) { return ((int64_t)a.nq * a.group + 32 * np - 1) / (32 * np); }
+
 template <class T, int DP>
 hipError_t launch(const DiffArgs& a, const DiffGrads& g, float* ws, hipStream_t s) {
+    constexpr int NP = pairs<T>(), OCC = sizeof(T) == 4 && DP > 32 ? 1 : 2;
+    // blocks of 32 that are staged between two barriers, each side measured at 577 causal rows of head size 48 (batch 8, 6
+    // heads), at 4096 causal ones of 48 (16 heads, 4 key heads) and in f32 at 301 of 40 (batch 4, 12 heads): dQ with one 104.7 / 193 / 80.6 us, with
+    // two 94.7 / 168 / 81;  dK and dV with one 102.8 / 454 / 93, with two 100.8 / 542 / 85
+    constexpr int NBQ = sizeof(T) == 4 ? 1 : 2, NBK = sizeof(T) == 4 ? 2 : 1;
     const int64_t bks = (int64_t)a.batch * a.kv_heads;
-    const int qt = (int)(((int64_t)a.nq * a.group + kBlock - 1) / kBlock), kt = (a.nk + kBlock - 1) / kBlock;
+    const int64_t qt = row_tiles(a, NP), kt = ((int64_t)a.nk + 32 * NP - 1) / (32 * NP);
     if (bks * qt > 0x7FFFFFFF || bks * kt > 0x7FFFFFFF) return hipErrorInvalidValue;
     float* ws_d = ws;
     float* ws_w = ws + 2 * (int64_t)a.batch * a.heads * a.nq;
-    hipLaunchKernelGGL((diff_bwd_q<T, DP>), dim3((int)(bks * qt)), dim3(256), 0, s, a, g, ws_d, ws_w, qt);
+    hipLaunchKernelGGL((diff_bwd_q<T, DP, NP, NBQ, OCC>), dim3((int)(bks * qt)), dim3(NP * 128), 0, s, a, g, ws_d, ws_w, (int)qt);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((diff_bwd_kv<T, DP, KVRC>), dim3((int)(bks * kt)), dim3(256), 0, s, a, g, ws_d, kt);
+    const dim3 grid((int)(bks * kt)), block(NP * 128);
+    if (a.group == 1) hipLaunchKernelGGL((diff_bwd_kv<T, DP, true, NP, NBK, OCC>), grid, block, 0, s, a, g, ws_d, (int)kt);
+    else hipLaunchKernelGGL((diff_bwd_kv<T, DP, false, NP, NBK, OCC>), grid, block, 0, s, a, g, ws_d, (int)kt);
     e = hipGetLastError();
     if (e != hipSuccess || !g.dlam) return e;
-    hipLaunchKernelGGL(diff_bwd_lam, dim3(a.lam_heads), dim3(256), 0, s, a, ws_w, qt, g.dlam);
+    hipLaunchKernelGGL(diff_bwd_lam, dim3(a.lam_heads), dim3(256), 0, s, a, ws_w, (int)qt, g.dlam);
     return hipGetLastError();
 }
 
 }  // namespace
 
 // f32 values of scratch of the backward
-int64_t diff_attention_bwd_workspace(const DiffArgs& a, bool) {
-    const int64_t rows = (int64_t)a.nq * a.group;
-    return 2 * (int64_t)a.batch * a.heads * a.nq + (int64_t)a.batch * a.kv_heads * ((rows + kBlock - 1) / kBlock) * a.group;
+int64_t diff_attention_bwd_workspace(const DiffArgs& a) {
+    return 2 * (int64_t)a.batch * a.heads * a.nq + (int64_t)a.batch * a.heads * row_tiles(a, 2);
 }
 
 hipError_t launch_diff_attention_backward(const DiffArgs& a, const DiffGrads& g, float* ws, bool bf16, hipStream_t s) {

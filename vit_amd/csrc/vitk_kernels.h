@@ -126,6 +126,7 @@ struct DiffArgs {
     const int* key_lens;          // [batch] or nullptr
     int batch, nq, nk, heads, kv_heads, group, d, lam_heads;   // group = heads / kv_heads
     int causal;
+    unsigned group_mul, group_shift;   // division by group (diff_attention.h)
     float scale, lambda_init;
 };
 // forward: out [batch, nq, heads, 2 d]; for the backward also out2 (the second map's product with V, out's shape), stats
@@ -145,7 +146,7 @@ struct DiffGrads {
     int64_t dqs[4], dks[4], dvs[3];
     float* dlam;
 };
-int64_t diff_attention_bwd_workspace(const DiffArgs& a, bool bf16);
+int64_t diff_attention_bwd_workspace(const DiffArgs& a);
 hipError_t launch_diff_attention_backward(const DiffArgs& a, const DiffGrads& g, float* ws, bool bf16, hipStream_t s);
 
 }  // namespace vitk
