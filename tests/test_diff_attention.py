@@ -262,6 +262,40 @@ def test_layouts(dtype):
 
 
 @gpu
+def test_gradients_that_arrive_in_any_layout():
+    """A gradient at an odd address, transposed, or broadcast: copied first, with the same values after."""
+    q, k, v, lam, do, _ = _inputs(2, 40, 50, 4, 2, 16, H16)
+    leaves = [t.cuda().requires_grad_(True) for t in (q, k, v, lam)]
+    do = do.cuda()
+    out = vit_amd.diff_attention(*leaves)
+    want = torch.autograd.grad(out, leaves, do, retain_graph=True)
+    odd = torch.empty(do.numel() + 1, dtype=do.dtype, device="cuda")
+    odd[1:] = do.reshape(-1)
+    for g in (odd[1:].view(do.shape), do.transpose(1, 2).contiguous().transpose(1, 2)):
+        for a, b in zip(torch.autograd.grad(out, leaves, g, retain_graph=True), want):
+            assert torch.equal(a, b)
+    ones = torch.autograd.grad(out, leaves, torch.ones_like(out), retain_graph=True)
+    for a, b in zip(torch.autograd.grad(out.sum(), leaves), ones):
+        assert torch.equal(a, b)
+
+
+@gpu
+def test_broadcast_inputs():
+    """Keys that all samples share by a stride of 0: their gradient is the sum over the samples, each rounded to the type."""
+    q, k, v, lam, do, _ = _inputs(3, 20, 33, 2, 2, 32, F)
+    q, lam, do = q.cuda(), lam.cuda(), do.cuda()
+    k1, v1 = k[:1].cuda().requires_grad_(True), v[:1].cuda().requires_grad_(True)
+    out = vit_amd.diff_attention(q, k1.expand(3, -1, -1, -1, -1), v1.expand(3, -1, -1, -1), lam)
+    dk, dv = torch.autograd.grad(out, (k1, v1), do)
+    kf, vf = (t.detach().repeat(3, *[1] * (t.dim() - 1)).requires_grad_(True) for t in (k1, v1))
+    full = vit_amd.diff_attention(q, kf, vf, lam)
+    assert torch.equal(out, full)
+    for a, b in zip((dk, dv), torch.autograd.grad(full, (kf, vf), do)):
+        s = b.double().sum(0, keepdim=True)
+        assert ((a.double() - s).abs() <= 3 * 2.0 ** -24 * b.double().abs().sum(0, keepdim=True)).all()
+
+
+@gpu
 def test_offsets_past_32_bits():
     """A sample that lies more than 2^32 bytes (and 2^31 elements) behind the first one."""
     far = (1 << 31) + 1024

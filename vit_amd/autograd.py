@@ -318,8 +318,11 @@ class DiffAttentionFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, g):
         q, k, v, lam, key_lens, out, out2, stats, weight = ctx.saved_tensors
+        g = g.contiguous()
+        if g.data_ptr() % 16:                        # a view into something larger
+            g = g.clone()
         dq, dk, dv, dlam = ops.diff_attention_backward(q, k, v, lam, ctx.scale, key_lens, ctx.causal, out, out2, stats, weight,
-                                                       g.contiguous(), lam_grad=ctx.needs_input_grad[3])
+                                                       g, lam_grad=ctx.needs_input_grad[3], checked=True)
         return dq, dk, dv, dlam, None, None, None, None
 
 
@@ -329,18 +332,18 @@ class GroupNormFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, num_groups, eps, activation):
-        y, mean, rstd = ops.group_norm(x, num_groups, weight, bias, eps, activation, stats=True)
-        ctx.save_for_backward(x, weight, bias, mean, rstd)
+        y, stats = ops.group_norm(x, num_groups, weight, bias, eps, activation, want_stats=True)
+        ctx.save_for_backward(x, weight, bias, stats)
         ctx.num_groups, ctx.activation = num_groups, activation
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        x, weight, bias, mean, rstd = ctx.saved_tensors
+        x, weight, bias, stats = ctx.saved_tensors
         want_w, want_b = weight is not None and ctx.needs_input_grad[1], bias is not None and ctx.needs_input_grad[2]
-        dx, dw, db = ops.group_norm_backward(x, ctx.num_groups, weight, bias, g.contiguous(), mean, rstd, ctx.activation,
-                                             param_grads=want_w or want_b)
+        dx, dw, db = ops.group_norm_backward(x, ctx.num_groups, weight, bias, g.contiguous(), stats, ctx.activation,
+                                             param_grads=want_w or want_b, checked=True)
         return dx, dw.view(weight.shape) if want_w else None, db.view(bias.shape) if want_b else None, None, None, None
 
 

@@ -684,22 +684,27 @@ def _grad_like(t):
     return g if g.stride(-1) == 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
-def diff_attention_backward(q, k, v, lam, scale, key_lens, causal, out, out2, stats, weight, dout, lam_grad=True):
-    """(dq, dk, dv, dlam) of diff_attention(); dlam None without `lam_grad`."""
-    B, nq, nk, H, K, d, code = _diff_sizes(q, k, v, lam, key_lens)
+def diff_attention_backward(q, k, v, lam, scale, key_lens, causal, out, out2, stats, weight, dout, lam_grad=True, checked=False):
+    """(dq, dk, dv, dlam) of diff_attention(); dlam None without `lam_grad`.  `checked`: the tensors are as diff_attention()
+    took and made them, and dout is contiguous and of out's shape and type."""
+    if checked:
+        (B, nq, H, _, d), nk, K, code = q.shape, k.shape[1], k.shape[2], _DTYPE_CODES[q.dtype]
+    else:
+        B, nq, nk, H, K, d, code = _diff_sizes(q, k, v, lam, key_lens)
     dq, dk, dv = _grad_like(q), _grad_like(k), _grad_like(v)
     dlam = torch.empty_like(lam) if lam_grad else None
     if q.numel() == 0 or k.numel() == 0:
         return dq.zero_(), dk.zero_(), dv.zero_(), None if dlam is None else dlam.zero_()
     L = _lib.load()
-    for n, t in (("out", out), ("out2", out2), ("dout", dout)):
-        _chk(t, q.dtype, n)
-        if tuple(t.shape) != (B, nq, H, 2 * d):
-            raise _lib.VitkError(f"diff_attention_backward: {n} {tuple(t.shape)} vs [{B},{nq},{H},{2 * d}]")
-    _chk(stats, torch.float32, "stats")
-    _chk(weight, torch.float32, "weight")
-    if stats.numel() != 4 * B * H * nq or weight.numel() != H:
-        raise _lib.VitkError(f"diff_attention_backward: stats {tuple(stats.shape)}, weight {tuple(weight.shape)}")
+    if not checked:
+        for n, t in (("out", out), ("out2", out2), ("dout", dout)):
+            _chk(t, q.dtype, n)
+            if tuple(t.shape) != (B, nq, H, 2 * d):
+                raise _lib.VitkError(f"diff_attention_backward: {n} {tuple(t.shape)} vs [{B},{nq},{H},{2 * d}]")
+        _chk(stats, torch.float32, "stats")
+        _chk(weight, torch.float32, "weight")
+        if stats.numel() != 4 * B * H * nq or weight.numel() != H:
+            raise _lib.VitkError(f"diff_attention_backward: stats {tuple(stats.shape)}, weight {tuple(weight.shape)}")
     n = L.vitk_diff_attention_workspace(B, nq, nk, H, K, d, code, 1)
     if n < 0:
         raise _lib.VitkError(f"diff_attention_backward: unsupported sizes q {tuple(q.shape)}, k {tuple(k.shape)}")
@@ -736,39 +741,42 @@ def _gn_sizes(x, num_groups, weight, bias, activation):
     return B, (x.numel() // (B * C) if B * C else 0), C
 
 
-def group_norm(x, num_groups, weight, bias, eps, activation="none", stats=False):
-    """(y, mean, rstd): y = act(GroupNorm(x)) for x bf16 / f32 [batch, ..., channels]; mean, rstd f32 [batch, groups]
-    with `stats`, else None."""
+def group_norm(x, num_groups, weight, bias, eps, activation="none", want_stats=False):
+    """(y, stats): y = act(GroupNorm(x)) for x bf16 / f32 [batch, ..., channels]; stats f32 [2, batch, groups] the means
+    and the reciprocal deviations with `want_stats`, else None."""
     L = _lib.load()
     B, S, C = _gn_sizes(x, num_groups, weight, bias, activation)
     y = torch.empty_like(x)
-    mean = rstd = None
-    if stats:
-        mean, rstd = torch.empty(2, B, num_groups, dtype=torch.float32, device=x.device).unbind(0)
+    stats = torch.empty(2, B, num_groups, dtype=torch.float32, device=x.device) if want_stats else None
     if x.numel() == 0:
-        return y, mean, rstd
+        return y, stats
     code = _DTYPE_CODES[x.dtype]
     n = L.vitk_group_norm_workspace(B, S, C, num_groups, code, 0)
     if n < 0:
         _lib.check(_lib.VITK_ERR_UNSUPPORTED, L)
     ws = _scratch(n, x.device)
+    mean = _ptr(stats)
     with _span("group_norm"):
-        _lib.check(L.vitk_group_norm(_ptr(x), _ptr(weight), _ptr(bias), _ptr(y), _ptr(mean), _ptr(rstd), _ptr(ws), n, B, S, C,
-                                     num_groups, float(eps), _lib.GROUP_NORM_ACTS[activation], code, _stream()), L)
-    return y, mean, rstd
+        _lib.check(L.vitk_group_norm(_ptr(x), _ptr(weight), _ptr(bias), _ptr(y), mean, mean and mean + 4 * B * num_groups, _ptr(ws),
+                                     n, B, S, C, num_groups, float(eps), _lib.GROUP_NORM_ACTS[activation], code, _stream()), L)
+    return y, stats
 
 
-def group_norm_backward(x, num_groups, weight, bias, dy, mean, rstd, activation="none", param_grads=True):
-    """(dx, dweight, dbias) of group_norm(); dweight and dbias f32 [channels], or None without `param_grads`."""
+def group_norm_backward(x, num_groups, weight, bias, dy, stats, activation="none", param_grads=True, checked=False):
+    """(dx, dweight, dbias) of group_norm() with its `stats`; dweight and dbias f32 [channels], or None without
+    `param_grads`.  `checked`: x, weight and bias are as group_norm() took them, and dy is of x's shape and type."""
     L = _lib.load()
-    B, S, C = _gn_sizes(x, num_groups, weight, bias, activation)
-    _chk(dy, x.dtype, "dy")
-    if dy.shape != x.shape:
-        raise _lib.VitkError(f"group_norm_backward: dy {tuple(dy.shape)} vs x {tuple(x.shape)}")
-    for n, t in (("mean", mean), ("rstd", rstd)):
-        _chk(t, torch.float32, n)
-        if t.numel() != B * num_groups:
-            raise _lib.VitkError(f"group_norm_backward: {n} has {t.numel()} elements, expected {B * num_groups}")
+    if checked:
+        B, C = x.shape[0], x.shape[-1]
+        S = x.numel() // (B * C) if B * C else 0
+    else:
+        B, S, C = _gn_sizes(x, num_groups, weight, bias, activation)
+        _chk(dy, x.dtype, "dy")
+        if dy.shape != x.shape:
+            raise _lib.VitkError(f"group_norm_backward: dy {tuple(dy.shape)} vs x {tuple(x.shape)}")
+        _chk(stats, torch.float32, "stats")
+        if stats.numel() != 2 * B * num_groups:
+            raise _lib.VitkError(f"group_norm_backward: stats has {stats.numel()} elements, expected {2 * B * num_groups}")
     dx = torch.empty_like(x)
     dw = db = None
     if param_grads:
@@ -780,9 +788,10 @@ def group_norm_backward(x, num_groups, weight, bias, dy, mean, rstd, activation=
     if n < 0:
         _lib.check(_lib.VITK_ERR_UNSUPPORTED, L)
     ws = _scratch(n, x.device)
+    mean = stats.data_ptr()
     with _span("group_norm_backward"):
-        _lib.check(L.vitk_group_norm_backward(_ptr(x), _ptr(weight), _ptr(bias), _ptr(dy), _ptr(mean), _ptr(rstd), _ptr(dx),
-                                              _ptr(dw), _ptr(db), _ptr(ws), n, B, S, C, num_groups,
+        _lib.check(L.vitk_group_norm_backward(_ptr(x), _ptr(weight), _ptr(bias), _ptr(dy), mean, mean + 4 * B * num_groups,
+                                              _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), n, B, S, C, num_groups,
                                               _lib.GROUP_NORM_ACTS[activation], code, _stream()), L)
     return dx, dw, db
 
@@ -804,17 +813,21 @@ class GradList:
     one device."""
 
     def __init__(self, tensors):
+        # one attribute at a time through the unbound getters: half the time of a loop over the tensors
         dev = tensors[0].get_device()
-        for t in tensors:
-            if t.layout is not torch.strided or t.get_device() != dev or dev < 0 or not (t.is_contiguous() or _dense(t)):
-                self._refuse(t, tensors[0])
-        kind = [_DTYPE_CODES.get(t.dtype, -1) for t in tensors]
-        if -1 in kind:
-            self._refuse(tensors[kind.index(-1)], tensors[0])
+        try:
+            addr = list(map(torch.Tensor.data_ptr, tensors))            # raises for tensors without strided memory
+            dense = all(map(torch.Tensor.is_contiguous, tensors)) or all(map(_dense, tensors))
+        except RuntimeError:
+            dense = False
+        kind = list(map(_DTYPE_CODES.get, map(torch.Tensor.dtype.__get__, tensors)))
+        if not dense or dev < 0 or None in kind or set(map(torch.Tensor.get_device, tensors)) != {dev}:
+            for t in tensors:
+                if t.layout is not torch.strided or t.dtype not in _DTYPE_CODES or t.get_device() != dev or dev < 0 or not _dense(t):
+                    self._refuse(t, tensors[0])
         n = self.n = len(tensors)
         # array.array copies a list of ints several times faster than a ctypes array does
-        self._held = (array.array("Q", [t.data_ptr() for t in tensors]), array.array("q", [t.numel() for t in tensors]),
-                      array.array("i", kind))
+        self._held = (array.array("Q", addr), array.array("q", map(torch.Tensor.numel, tensors)), array.array("i", kind))
         self.addr, self.size, self.kind = (a.buffer_info()[0] for a in self._held)
         self.empty = not any(self._held[1])
         self.device = tensors[0].device

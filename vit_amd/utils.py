@@ -76,7 +76,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     Gradients of bf16 or f32, dense, on one device, no two sharing memory.  A norm of NaN makes every gradient NaN and one of inf
     makes them 0 (NaN where they are infinite), as in torch."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
-    tensors = [p.grad for p in parameters if p.grad is not None]
+    tensors = [g for p in parameters if (g := p.grad) is not None]
     kind = _norm_kind(norm_type)
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
