@@ -344,7 +344,11 @@ class GroupNormFn(torch.autograd.Function):
         want_w, want_b = weight is not None and ctx.needs_input_grad[1], bias is not None and ctx.needs_input_grad[2]
         dx, dw, db = ops.group_norm_backward(x, ctx.num_groups, weight, bias, g.contiguous(), stats, ctx.activation,
                                              param_grads=want_w or want_b, checked=True)
-        return dx, dw.view(weight.shape) if want_w else None, db.view(bias.shape) if want_b else None, None, None, None
+        if want_w and weight.dim() != 1:
+            dw = dw.view(weight.shape)
+        if want_b and bias.dim() != 1:
+            db = db.view(bias.shape)
+        return dx, dw if want_w else None, db if want_b else None, None, None, None
 
 
 class PatchEmbedFn(torch.autograd.Function):

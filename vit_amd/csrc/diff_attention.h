@@ -175,6 +175,10 @@ __device__ __forceinline__ RowPlace row_place(const DiffArgs& a, int kh, int r) 
     return RowPlace{t, kh * a.group + (r - t * a.group)};
 }
 
+// Waits for every load so far.  Before a loop that loads ahead: what was loaded before it and is used in it would otherwise be
+// waited for inside, and the loop's own loads with it.
+__device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0F70); }       // vmcnt(0), other counters free
+
 // keys that a query token sees: those below the result
 __device__ __forceinline__ int key_limit(const DiffArgs& a, int len, int tok) {
     if (!a.causal) return len;

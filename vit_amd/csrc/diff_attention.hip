@@ -169,6 +169,7 @@ __global__ __launch_bounds__(NG * 128, OCC) void diff_fwd(DiffArgs a, DiffOut o,
         }
     };
     if (c0 < c1) stage.put(bufs[0]);
+    loads_done();
     __syncthreads();
     for (int c = c0; c < c1; ++c) {
         const char* buf = bufs[(c - c0) & 1];

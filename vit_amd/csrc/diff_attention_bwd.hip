@@ -119,6 +119,7 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_q(DiffArgs a, DiffGrad
     const float sc = a.scale * kLog2e;
 
     if (c1 > 0) stage.put(bufs[0]);
+    loads_done();
     __syncthreads();
     for (int c = 0; c < c1; ++c) {
         const char* kt = bufs[c & 1];
@@ -188,7 +189,8 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_q(DiffArgs a, DiffGrad
 //     S_m starts at -lse_m / (scale log2 e), so that P_m = exp2(scale log2(e) S_m);  dA starts at -D_m.
 // ONE: one query head to a key head, so that w is the workgroup's and can wait until the end (else the rows bring theirs).
 template <class T, int DP, bool ONE, int NP, int NB, int OCC>
-__global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_kv(DiffArgs a, DiffGrads g, const float* __restrict__ ws_d, int tiles) {
+__global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_kv(DiffArgs a, DiffGrads g, const float* __restrict__ ws_d,
+                                                             float* __restrict__ parts, int splits) {
     constexpr int kThreads = NP * 128, kBlock = NP * 32;
     constexpr int DV = 2 * DP;
     constexpr int RB = row_bytes<T, DV>();
@@ -206,7 +208,7 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_kv(DiffArgs a, DiffGra
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), map = wave & 1, grp = wave >> 1;
     const int r = lane & 31, hh = lane >> 5;
     const int bks = a.batch * a.kv_heads;
-    const int bk = blockIdx.x % bks, tile = blockIdx.x / bks;        // causal: the first keys have the most rows
+    const int bk = blockIdx.x % bks, rest = blockIdx.x / bks, tile = rest / splits;      // causal: the first keys have the most rows
     const int b = bk / a.kv_heads, kh = bk - b * a.kv_heads;
     const int nrows = a.nq * a.group;
     const int len = sample_len(a, b);
@@ -218,7 +220,12 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_kv(DiffArgs a, DiffGra
         const int t = block0 - (a.nk - a.nq);
         first = t > 0 ? t * a.group / RC : 0;
     }
-    const int c1 = block0 < len ? (nrows + RC - 1) / RC : 0;
+    int c1 = block0 < len ? (nrows + RC - 1) / RC : 0;
+    if (splits > 1) {                                                 // this workgroup's share of them
+        const int per = (c1 - first + splits - 1) / splits;
+        first += (rest - tile * splits) * per;
+        c1 = first + per < c1 ? first + per : c1;
+    }
 
     const int dc = a.d / PER;
     Stage<T, DP, kThreads, RC> stage;
@@ -228,39 +235,34 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_kv(DiffArgs a, DiffGra
                                   : reinterpret_cast<const T*>(a.q) + b * a.qs[0] + stage.map * a.qs[3] + stage.e * PER;
     if (ONE) s_src += kh * s_head;
     const int64_t lmap = (int64_t)a.batch * a.heads * a.nq;
-    float held_r[NS];
-    int held_l = 0;
+    static_assert(4 * RC <= kThreads, "four values of a row have a thread each");
+    // the rows' values: a thread brings one to four of them, raw; what is computed from them waits until they are put
+    const int role = tid / RC, s_at = tid % RC;                       // 0, 1: -lse of a map;  2, 3: -D of a map
+    const float* s_from = role < 2 ? g.stats + role * lmap : ws_d + (role - 2) * lmap;
+    float held0 = 0.f, held1 = 0.f, held_w = 0.f;
     auto fetch = [&](int c) {
         stage.fetch(c * RC, nrows, [&](int row) {
             if constexpr (ONE) return s_src + row * s_tok;
             const RowPlace pl = row_place(a, kh, row);
             return s_src + pl.tok * s_tok + pl.head * s_head;
         });
-        if (tid < RC) {
-            const int row = c * RC + tid;
-            held_l = 0;
-            held_r[0] = held_r[1] = -__builtin_inff();                // a row past the last one: P = 0
-            held_r[2] = held_r[3] = 0.f;
-            if constexpr (!ONE) held_r[4] = 0.f;
-            if (row < nrows) {
-                const RowPlace pl = ONE ? RowPlace{row, kh} : row_place(a, kh, row);
-                const int64_t at = ((int64_t)b * a.heads + pl.head) * a.nq + pl.tok;
-                held_r[0] = (__builtin_amdgcn_logf(g.stats[2 * lmap + at]) - g.stats[at]) * rsc;
-                held_r[1] = (__builtin_amdgcn_logf(g.stats[3 * lmap + at]) - g.stats[lmap + at]) * rsc;
-                held_r[2] = -ws_d[at];
-                held_r[3] = -ws_d[lmap + at];
-                if constexpr (!ONE) held_r[4] = g.weight[pl.head];
-                held_l = key_limit(a, len, pl.tok);
-            }
+        const int row = c * RC + s_at;
+        if (role < 4 && row < nrows) {
+            const RowPlace pl = ONE ? RowPlace{row, kh} : row_place(a, kh, row);
+            const int64_t at = ((int64_t)b * a.heads + pl.head) * a.nq + pl.tok;
+            held0 = s_from[at];
+            if (role < 2) held1 = s_from[2 * lmap + at];
+            if (!ONE && role == 1) held_w = g.weight[pl.head];
         }
     };
-    auto put = [&](int k) {
+    auto put = [&](int k, int c) {
         stage.put(bufs[k]);
-        if (tid < RC) {
-#pragma unroll
-            for (int j = 0; j < NS; ++j) s_row[k][j][tid] = held_r[j];
-            s_lim[k][tid] = held_l;
-        }
+        if (role >= 4) return;
+        const int row = c * RC + s_at;
+        const bool on = row < nrows;                                  // a row past the last one: P = 0
+        s_row[k][role][s_at] = role < 2 ? (on ? (__builtin_amdgcn_logf(held1) - held0) * rsc : -__builtin_inff()) : on ? -held0 : 0.f;
+        if (!ONE && role == 1) s_row[k][NS - 1][s_at] = on ? held_w : 0.f;
+        if (role == 0) s_lim[k][s_at] = on ? key_limit(a, len, ONE ? row : row_place(a, kh, row).tok) : 0;
     };
     if (first < c1) fetch(first);
 
@@ -287,7 +289,8 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_kv(DiffArgs a, DiffGra
 #pragma unroll
     for (int d = 0; d < DB; ++d) dv[d] = zero16();
 
-    if (first < c1) put(0);
+    if (first < c1) put(0, first);
+    loads_done();
     __syncthreads();
     for (int c = first; c < c1; ++c) {
         const int k = (c - first) & 1;
@@ -348,12 +351,14 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_kv(DiffArgs a, DiffGra
                 }
             }
         }
-        if (more) put(k ^ 1);
+        if (more) put(k ^ 1, c + 1);
         __syncthreads();
     }
 
     const bool live = key < a.nk;
     const float f = map == 0 ? 1.f : ONE ? -g.weight[kh] : -1.f;      // the second map's part
+    // [split][sample, key head][key][dK of both maps, dV]
+    float* part = splits > 1 ? parts + (((int64_t)(rest - tile * splits) * bks + bk) * a.nk + key) * 4 * a.d : nullptr;
     if (live) {
         T* ko = reinterpret_cast<T*>(g.dk) + b * g.dks[0] + (int64_t)key * g.dks[1] + kh * g.dks[2] + map * g.dks[3];
         const float fk = f * a.scale;
@@ -363,7 +368,9 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_kv(DiffArgs a, DiffGra
             for (int q = 0; q < 4; ++q) {
                 const int col = e * 32 + 8 * q + 4 * hh;
                 if (col >= a.d) continue;
-                store4(ko + col, f32x4{dk[e][4 * q] * fk, dk[e][4 * q + 1] * fk, dk[e][4 * q + 2] * fk, dk[e][4 * q + 3] * fk});
+                const f32x4 x = {dk[e][4 * q] * fk, dk[e][4 * q + 1] * fk, dk[e][4 * q + 2] * fk, dk[e][4 * q + 3] * fk};
+                if (part) *reinterpret_cast<f32x4*>(part + map * a.d + col) = x;
+                else store4(ko + col, x);
             }
     }
     T* vo = reinterpret_cast<T*>(g.dv) + b * g.dvs[0] + (int64_t)key * g.dvs[1] + kh * g.dvs[2];
@@ -389,10 +396,29 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_kv(DiffArgs a, DiffGra
                     const int col = d * 32 + 8 * q + 4 * hh;
                     if (col >= 2 * a.d) continue;
                     const f32x4 y = box[(d - d0) * 256 + q * 64];
-                    store4(vo + col, f32x4{dv[d][4 * q] + y[0], dv[d][4 * q + 1] + y[1], dv[d][4 * q + 2] + y[2], dv[d][4 * q + 3] + y[3]});
+                    const f32x4 x = {dv[d][4 * q] + y[0], dv[d][4 * q + 1] + y[1], dv[d][4 * q + 2] + y[2], dv[d][4 * q + 3] + y[3]};
+                    if (part) *reinterpret_cast<f32x4*>(part + 2 * a.d + col) = x;
+                    else store4(vo + col, x);
                 }
         }
     }
+}
+
+// The row splits' dK and dV added, four columns of a key to a lane.
+template <class T>
+__global__ __launch_bounds__(256) void diff_bwd_join(DiffArgs a, DiffGrads g, const float* __restrict__ parts, int splits) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, keys = (int64_t)a.batch * a.kv_heads * a.nk;
+    const int64_t row = i / a.d;
+    if (row >= keys) return;
+    const int col = (int)(i - row * a.d) * 4;
+    const float* p = parts + row * 4 * a.d + col;
+    f32x4 x = *reinterpret_cast<const f32x4*>(p);
+    for (int s = 1; s < splits; ++s) x = x + *reinterpret_cast<const f32x4*>(p + s * keys * 4 * a.d);
+    const int64_t bk = row / a.nk, key = row - bk * a.nk, b = bk / a.kv_heads, kh = bk - b * a.kv_heads;
+    const int map = col >= a.d;
+    T* to = col < 2 * a.d ? reinterpret_cast<T*>(g.dk) + b * g.dks[0] + key * g.dks[1] + kh * g.dks[2] + map * g.dks[3] + col - map * a.d
+                          : reinterpret_cast<T*>(g.dv) + b * g.dvs[0] + key * g.dvs[1] + kh * g.dvs[2] + col - 2 * a.d;
+    store4(to, x);
 }
 
 // dlam of one lam head from the workgroups' shares of dw: dlam_0 = dw e_1 lam_1, dlam_1 = dw e_1 lam_0, and the second
@@ -441,27 +467,54 @@ template <class T>
 constexpr int pairs() { return sizeof(T) == 4 ? 2 : 4; }
 
 int64_t row_tiles(const DiffArgs& a, int np) { return ((int64_t)a.nq * a.group + 32 * np - 1) / (32 * np); }
+int64_t key_tiles(const DiffArgs& a, int np) { return ((int64_t)a.nk + 32 * np - 1) / (32 * np); }
+
+// Into how many parts the rows of a key tile are split: so many that there are two workgroups to a CU, where most CUs would
+// have none, or where the rows are long enough to pay for adding the parts (under a causal mask the first keys' workgroups
+// have twice the average work).  Measured with / without, the addition included: 10000 causal rows, 20 workgroups 66 / 621
+// us; 1800, 45: 31 / 95; 600, 80: 27 / 30; 8192, 256: 305 / 452;  1500 unmasked rows, 384 workgroups 183 / 183, 1200 causal
+// ones, 240: 64 / 55.
+int row_splits(const DiffArgs& a, int np) {
+    const int64_t blocks = (int64_t)a.batch * a.kv_heads * key_tiles(a, np), rows = (int64_t)a.nq * a.group;
+    if (blocks >= 128 && rows < 2048) return 1;
+    int64_t s = 511 / blocks + 1, most = rows / 256;
+    s = s < most ? s : most;
+    return (int)(s < 1 ? 1 : s > 16 ? 16 : s);
+}
+
+int64_t parts_floats(const DiffArgs& a, int np) {
+    const int s = row_splits(a, np);
+    return s > 1 ? (int64_t)s * a.batch * a.kv_heads * a.nk * 4 * a.d : 0;
+}
 
 template <class T, int DP>
 hipError_t launch(const DiffArgs& a, const DiffGrads& g, float* ws, hipStream_t s) {
     constexpr int NP = pairs<T>(), OCC = sizeof(T) == 4 && DP > 32 ? 1 : 2;
-    // blocks of 32 that are staged between two barriers, each side measured at 577 causal rows of head size 48 (batch 8, 6
-    // heads), at 4096 causal ones of 48 (16 heads, 4 key heads) and in f32 at 301 of 40 (batch 4, 12 heads): dQ with one 104.7 / 193 / 80.6 us, with
-    // two 94.7 / 168 / 81;  dK and dV with one 102.8 / 454 / 93, with two 100.8 / 542 / 85
+    // blocks of 32 that are staged between two barriers, measured with one / two:  dQ at 577 tokens (batch 16, 8 heads of
+    // 48) 104.7 / 94.7 us, at 4096 causal ones (2, 8 heads of 64, 4 key heads) 193 / 168, in f32 at 257 (4, 16 heads of 40)
+    // 80.6 / 81;  dK and dV 102.8 / 100.8, 454 / 542, 93 / 85
     constexpr int NBQ = sizeof(T) == 4 ? 1 : 2, NBK = sizeof(T) == 4 ? 2 : 1;
     const int64_t bks = (int64_t)a.batch * a.kv_heads;
-    const int64_t qt = row_tiles(a, NP), kt = ((int64_t)a.nk + 32 * NP - 1) / (32 * NP);
-    if (bks * qt > 0x7FFFFFFF || bks * kt > 0x7FFFFFFF) return hipErrorInvalidValue;
-    float* ws_d = ws;
-    float* ws_w = ws + 2 * (int64_t)a.batch * a.heads * a.nq;
+    const int64_t qt = row_tiles(a, NP), kt = key_tiles(a, NP), keys = (int64_t)a.batch * a.kv_heads * a.nk;
+    const int splits = row_splits(a, NP);
+    if (bks * qt > 0x7FFFFFFF || bks * kt * splits > 0x7FFFFFFF || keys * a.d / 256 > 0x7FFFFFF0) return hipErrorInvalidValue;
+    float* parts = ws;
+    float* ws_d = ws + parts_floats(a, NP);
+    float* ws_w = ws_d + 2 * (int64_t)a.batch * a.heads * a.nq;
     hipLaunchKernelGGL((diff_bwd_q<T, DP, NP, NBQ, OCC>), dim3((int)(bks * qt)), dim3(NP * 128), 0, s, a, g, ws_d, ws_w, (int)qt);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const dim3 grid((int)(bks * kt)), block(NP * 128);
-    if (a.group == 1) hipLaunchKernelGGL((diff_bwd_kv<T, DP, true, NP, NBK, OCC>), grid, block, 0, s, a, g, ws_d, (int)kt);
-    else hipLaunchKernelGGL((diff_bwd_kv<T, DP, false, NP, NBK, OCC>), grid, block, 0, s, a, g, ws_d, (int)kt);
+    const dim3 grid((int)(bks * kt * splits)), block(NP * 128);
+    if (a.group == 1) hipLaunchKernelGGL((diff_bwd_kv<T, DP, true, NP, NBK, OCC>), grid, block, 0, s, a, g, ws_d, parts, splits);
+    else hipLaunchKernelGGL((diff_bwd_kv<T, DP, false, NP, NBK, OCC>), grid, block, 0, s, a, g, ws_d, parts, splits);
     e = hipGetLastError();
-    if (e != hipSuccess || !g.dlam) return e;
+    if (e != hipSuccess) return e;
+    if (splits > 1) {
+        hipLaunchKernelGGL((diff_bwd_join<T>), dim3((int)((keys * a.d + 255) / 256)), dim3(256), 0, s, a, g, parts, splits);
+        e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    if (!g.dlam) return hipSuccess;
     hipLaunchKernelGGL(diff_bwd_lam, dim3(a.lam_heads), dim3(256), 0, s, a, ws_w, (int)qt, g.dlam);
     return hipGetLastError();
 }
@@ -469,8 +522,9 @@ hipError_t launch(const DiffArgs& a, const DiffGrads& g, float* ws, hipStream_t 
 }  // namespace
 
 // f32 values of scratch of the backward
-int64_t diff_attention_bwd_workspace(const DiffArgs& a) {
-    return 2 * (int64_t)a.batch * a.heads * a.nq + (int64_t)a.batch * a.heads * row_tiles(a, 2);
+int64_t diff_attention_bwd_workspace(const DiffArgs& a, bool bf16) {
+    const int np = bf16 ? pairs<bf16_t>() : pairs<float>();
+    return parts_floats(a, np) + 2 * (int64_t)a.batch * a.heads * a.nq + (int64_t)a.batch * a.heads * row_tiles(a, np);
 }
 
 hipError_t launch_diff_attention_backward(const DiffArgs& a, const DiffGrads& g, float* ws, bool bf16, hipStream_t s) {

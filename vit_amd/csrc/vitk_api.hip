@@ -678,7 +678,7 @@ int64_t vitk_diff_attention_workspace(int batch, int nq, int nk, int heads, int 
         (dtype != VITK_F32 && dtype != VITK_BF16))
         return -1;
     const DiffArgs a = diff_sizes(batch, nq, nk, heads, kv_heads, d);
-    return backward ? diff_attention_bwd_workspace(a) : diff_attention_workspace(a, dtype == VITK_BF16);
+    return backward ? diff_attention_bwd_workspace(a, dtype == VITK_BF16) : diff_attention_workspace(a, dtype == VITK_BF16);
 }
 
 int vitk_diff_attention(const void* q, const void* k, const void* v, const int64_t* strides, const float* lam, int lam_heads,
@@ -720,7 +720,7 @@ int vitk_diff_attention_backward(const void* q, const void* k, const void* v, co
     for (int i = 0; i < 11; ++i)
         if (grad_strides[i] < 0 || grad_strides[i] % per != 0)
             return fail(VITK_ERR_INVALID, "%s: gradient stride %lld is not a multiple of 16 bytes", name, (long long)grad_strides[i]);
-    const int64_t need = diff_attention_bwd_workspace(a);
+    const int64_t need = diff_attention_bwd_workspace(a, dtype == VITK_BF16);
     if (workspace_floats < need) return fail(VITK_ERR_INVALID, "%s: workspace of %lld floats, %lld needed", name, (long long)workspace_floats, (long long)need);
     if (!aligned16(workspace)) return fail(VITK_ERR_INVALID, "%s: workspace must be 16-byte aligned", name);
     DiffGrads g = {};

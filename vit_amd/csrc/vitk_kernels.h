@@ -146,7 +146,7 @@ struct DiffGrads {
     int64_t dqs[4], dks[4], dvs[3];
     float* dlam;
 };
-int64_t diff_attention_bwd_workspace(const DiffArgs& a);
+int64_t diff_attention_bwd_workspace(const DiffArgs& a, bool bf16);
 hipError_t launch_diff_attention_backward(const DiffArgs& a, const DiffGrads& g, float* ws, bool bf16, hipStream_t s);
 
 }  // namespace vitk

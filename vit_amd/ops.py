@@ -780,7 +780,7 @@ def group_norm_backward(x, num_groups, weight, bias, dy, stats, activation="none
     dx = torch.empty_like(x)
     dw = db = None
     if param_grads:
-        dw, db = torch.empty(2, C, dtype=torch.float32, device=x.device).unbind(0)
+        dw, db = (torch.empty(C, dtype=torch.float32, device=x.device) for _ in range(2))
     if x.numel() == 0:
         return dx, dw if dw is None else dw.zero_(), db if db is None else db.zero_()
     code = _DTYPE_CODES[x.dtype]
