@@ -160,24 +160,58 @@ __device__ __forceinline__ void store4(bf16_t* p, f32x4 v) {
 }
 __device__ __forceinline__ void store4(float* p, f32x4 v) { *reinterpret_cast<f32x4*>(p) = v; }
 
-// 16 zero bytes to stage from where there is nothing: rows past the last visible key, columns past the head
-static __device__ __align__(16) const unsigned kZeros[4] = {0, 0, 0, 0};
+// Columns col0 + 8 g + 4 hh ... of a row (a) and the same 8 further (b), as an accumulator's elements hold them, if they lie
+// below `limit` (a multiple of 8) and the row is live.  In bf16 the half-waves exchange fours, so that each stores 16 bytes.
+__device__ __forceinline__ void store_pair(bf16_t* row, int col, int hh, int limit, bool live, f32x4 a, f32x4 b) {
+    const auto s0 = __builtin_amdgcn_permlane32_swap(pack_bf16(a[0], a[1]), pack_bf16(b[0], b[1]), false, false);
+    const auto s1 = __builtin_amdgcn_permlane32_swap(pack_bf16(a[2], a[3]), pack_bf16(b[2], b[3]), false, false);
+    const u32x4 x = {s0[0], s1[0], s0[1], s1[1]};
+    col += 8 * hh;
+    if (live && col < limit) *reinterpret_cast<u32x4*>(row + col) = x;
+}
+__device__ __forceinline__ void store_pair(float* row, int col, int hh, int limit, bool live, f32x4 a, f32x4 b) {
+    col += 4 * hh;
+    if (live && col < limit) store4(row + col, a);
+    if (live && col + 8 < limit) store4(row + col + 8, b);
+}
+__device__ __forceinline__ f32x4 four(const f32x16& v, int g, float f) {
+    return f32x4{v[4 * g] * f, v[4 * g + 1] * f, v[4 * g + 2] * f, v[4 * g + 3] * f};
+}
+
+// Chunk c of a row, or zeros (columns past the head, rows past the last one): `row` is always one that can be read
+template <class T>
+__device__ __forceinline__ typename Op<T>::Chunk chunk_or_zero(const T* row, int c, bool on) {
+    typename Op<T>::Chunk x = *reinterpret_cast<const typename Op<T>::Chunk*>(row + (on ? c * Op<T>::kPer : 0));
+#pragma unroll
+    for (int j = 0; j < Op<T>::kPer; ++j) x[j] = on ? x[j] : (T)0.f;
+    return x;
+}
+
+__device__ __forceinline__ int quotient(int n, Divisor d) { return d.mul ? (int)(__umulhi((unsigned)n, d.mul) >> d.shift) : n; }
 
 // The rows of a (sample, key head): row r = query token r / g of query head kh * g + r % g, so that the query heads which
-// share a key head share its tiles.  The division by g = group is a multiplication by group_mul = 2^(31 + l) / g + 1 with
-// 2^l >= g: n < 2^31 times that, over 2^(31 + l), exceeds n / g by less than 1 / g.
+// share a key head share its tiles.
 struct RowPlace {
     int tok, head;
 };
 __device__ __forceinline__ RowPlace row_place(const DiffArgs& a, int kh, int r) {
     if (a.group == 1) return RowPlace{r, kh};
-    const int t = (int)(__umulhi((unsigned)r, a.group_mul) >> a.group_shift);
+    const int t = quotient(r, a.by_group);
     return RowPlace{t, kh * a.group + (r - t * a.group)};
 }
 
 // Waits for every load so far.  Before a loop that loads ahead: what was loaded before it and is used in it would otherwise be
 // waited for inside, and the loop's own loads with it.
 __device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0F70); }       // vmcnt(0), other counters free
+
+// Loads what every workgroup needs of the arguments at once: left to the compiler, each block of the prologue loads and waits
+// for its own.
+__device__ __forceinline__ void arguments(const DiffArgs& a) {
+    asm volatile("" ::"s"(a.q), "s"(a.k), "s"(a.v), "s"(a.qs[0]), "s"(a.qs[1]), "s"(a.qs[2]), "s"(a.qs[3]), "s"(a.ks[0]), "s"(a.ks[1]),
+                 "s"(a.ks[2]), "s"(a.ks[3]), "s"(a.vs[0]), "s"(a.vs[1]), "s"(a.vs[2]), "s"(a.lam), "s"(a.key_lens), "s"(a.batch),
+                 "s"(a.nq), "s"(a.nk), "s"(a.heads), "s"(a.kv_heads), "s"(a.group), "s"(a.d), "s"(a.lam_heads), "s"(a.causal),
+                 "s"(a.by_group.mul), "s"(a.by_kv_heads.mul), "s"(a.by_bks.mul), "s"(a.by_bks.shift), "s"(a.scale));
+}
 
 // keys that a query token sees: those below the result
 __device__ __forceinline__ int key_limit(const DiffArgs& a, int len, int tok) {
@@ -186,25 +220,32 @@ __device__ __forceinline__ int key_limit(const DiffArgs& a, int len, int tok) {
     return lim < len ? (lim > 0 ? lim : 0) : len;
 }
 
+// Which element of a column's 16 scores is key first + 8 (i >> 2) + 4 hh + (i & 3): those at `seen` and behind are hidden
+__device__ __forceinline__ void hide(f32x16& s, int seen) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = 8 * (i >> 2) + (i & 3) < seen ? s[i] : -__builtin_inff();
+}
+
 constexpr int pow2_below(int n) { return n >= 32 ? 32 : n >= 16 ? 16 : n >= 8 ? 8 : n >= 4 ? 4 : n >= 2 ? 2 : 1; }
 
 // Staging of a chunk of C rows of two tensors side by side, [2 maps x d] and [2 d] (K and V, or Q and dO), through
-// registers into an LDS buffer of two tiles: 4 DPC neighbouring lanes move a row's chunks.  Columns past the head's d are
-// zeroed once in both buffers and left alone; rows past the last one are the last one again (nothing behind it is read),
-// which the caller masks.
+// registers into an LDS buffer of two tiles: the first half of the threads moves the first tensor, 2 DPC neighbouring lanes a
+// row's chunks.  Columns past the head's d are zeroed once in both buffers and left alone; rows past the last one are the
+// last one again (nothing behind it is read), which the caller masks.
 template <class T, int DP, int NT, int C>
 struct Stage {
     static constexpr int PER = Op<T>::kPer, DPC = DP / PER, RB = row_bytes<T, 2 * DP>(), TILE = C * RB;
-    static constexpr int LANES = 4 * DPC, ROWS = pow2_below(NT / LANES < C ? NT / LANES : C), PASSES = C / ROWS;
+    static constexpr int LANES = 2 * DPC, HALF = NT / 2, ROWS = pow2_below(HALF / LANES < C ? HALF / LANES : C), PASSES = C / ROWS;
+    static_assert(HALF % 64 == 0, "a wave moves one tensor");
     int row, col;          // within the chunk; chunk of the LDS row
-    bool second, on;
+    bool second, on;       // second: wave-uniform
     int map, e;            // first tensor: map and chunk within it
     u32x4 held[PASSES];
-    __device__ __forceinline__ void init(int tid, int dc, char* bufs) {
-        row = tid / LANES;
-        const int c = tid - row * LANES;
-        second = c >= 2 * DPC;
-        col = second ? c - 2 * DPC : c;
+    __device__ __forceinline__ void init(int tid, int dc, char* bufs, int buf_bytes) {
+        second = __builtin_amdgcn_readfirstlane(tid >= HALF);
+        const int t = second ? tid - HALF : tid;
+        row = t / LANES;
+        col = t - row * LANES;
         map = !second && col >= DPC ? 1 : 0;
         e = col - map * DPC;
         const bool mine = row < ROWS;
@@ -212,16 +253,23 @@ struct Stage {
         if (mine && !on)
             for (int k = 0; k < 2; ++k)
 #pragma unroll
-                for (int i = 0; i < PASSES; ++i) *reinterpret_cast<u32x4*>(bufs + k * 2 * TILE + at(i)) = u32x4{0u, 0u, 0u, 0u};
+                for (int i = 0; i < PASSES; ++i) *reinterpret_cast<u32x4*>(bufs + k * buf_bytes + at(i)) = u32x4{0u, 0u, 0u, 0u};
     }
     __device__ __forceinline__ int at(int i) const {
         const int lr = row + i * ROWS;
         return (second ? TILE : 0) + lr * RB + ((col ^ swz<RB>(lr)) << 4);
     }
-    // addr(row): where the row of this lane's tensor, map and chunk lies
+    // Whole chunks: row0 + the thread's row lies (row0 >> shift) `step` behind src (wave-uniform: one addition a load).  addr(r):
+    // where row r of this lane's tensor, map and chunk lies, for the last chunk, and for all where shift < 0.
     template <class F>
-    __device__ __forceinline__ void fetch(int row0, int rows, F&& addr) {
+    __device__ __forceinline__ void fetch(int row0, int rows, const T* src, int64_t step, int shift, F&& addr) {
         if (!on) return;
+        if (shift >= 0 && row0 + C <= rows) {
+#pragma unroll
+            for (int i = 0; i < PASSES; ++i)
+                held[i] = *reinterpret_cast<const u32x4*>(src + ((row0 + i * ROWS) >> shift) * step);
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
             const int r = row0 + row + i * ROWS;
@@ -235,26 +283,46 @@ struct Stage {
     }
 };
 
-// w_h = exp(lam0 . lam1) - exp(lam2 . lam3) + lambda_init; the half-waves share the sums of a lane's head, all loads at once
+// w_h = exp(lam0 . lam1) - exp(lam2 . lam3) + lambda_init, all loads at once.  Where all lanes want the same head the first
+// half-wave adds the first product, a column to a lane, and the second the other; else the half-waves share the sums of a
+// lane's own head.
 template <int DP>
-__device__ __forceinline__ float map_weight(const DiffArgs& a, int head, int hh) {
-    const float* p = a.lam + (a.lam_heads == 1 ? 0 : (int64_t)head * a.d);
+__device__ __forceinline__ float map_weight(const DiffArgs& a, int head, int lane) {
+    const int hh = lane >> 5, col = lane & 31;
     const int64_t vs = (int64_t)a.lam_heads * a.d;
-    float s1 = 0.f, s2 = 0.f;
+    float s1, s2;
+    if (a.group == 1 || a.lam_heads == 1) {
+        const float* p = a.lam + (a.lam_heads == 1 ? 0 : (int64_t)__builtin_amdgcn_readfirstlane(head) * a.d) + 2 * hh * vs;
+        const int e = col < a.d ? col : 0, e2 = DP > 32 && col + 32 < a.d ? col + 32 : 0;
+        const float x = p[e], y = p[vs + e], x2 = p[e2], y2 = p[vs + e2];
+        float s = col < a.d ? x * y : 0.f;
+        if (DP > 32 && col + 32 < a.d) s = fmaf(x2, y2, s);
 #pragma unroll
-    for (int t = 0; t < DP / 8; ++t) {
-        if (8 * t >= a.d) break;
-        const f32x4* e = reinterpret_cast<const f32x4*>(p + 8 * t + 4 * hh);
-        const f32x4 x = e[0], y = *reinterpret_cast<const f32x4*>(p + vs + 8 * t + 4 * hh);
-        const f32x4 z = *reinterpret_cast<const f32x4*>(p + 2 * vs + 8 * t + 4 * hh);
-        const f32x4 u = *reinterpret_cast<const f32x4*>(p + 3 * vs + 8 * t + 4 * hh);
+        for (int o = 1; o < 32; o <<= 1) s += __shfl_xor(s, o, 64);
+        const unsigned u = __builtin_bit_cast(unsigned, s);
+        const auto sw = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+        const unsigned lo = sw[0], hi = sw[1];
+        s1 = __builtin_bit_cast(float, lo);
+        s2 = __builtin_bit_cast(float, hi);
+    } else {
+        const float* p = a.lam + (int64_t)head * a.d;
+        s1 = s2 = 0.f;
+        f32x4 v[4][DP / 8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            s1 = fmaf(x[j], y[j], s1);
-            s2 = fmaf(z[j], u[j], s2);
-        }
+        for (int t = 0; t < DP / 8; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i][t] = *reinterpret_cast<const f32x4*>(p + i * vs + (8 * t < a.d ? 8 * t + 4 * hh : 0));
+#pragma unroll
+        for (int t = 0; t < DP / 8; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                s1 = 8 * t < a.d ? fmaf(v[0][t][j], v[1][t][j], s1) : s1;
+                s2 = 8 * t < a.d ? fmaf(v[2][t][j], v[3][t][j], s2) : s2;
+            }
+        s1 = both_sum(s1);
+        s2 = both_sum(s2);
     }
-    return expf(both_sum(s1)) - expf(both_sum(s2)) + a.lambda_init;
+    return expf(s1) - expf(s2) + a.lambda_init;
 }
 
 }  // namespace diff

@@ -54,19 +54,21 @@ __global__ __launch_bounds__(NG * 128, OCC) void diff_fwd(DiffArgs a, DiffOut o,
     constexpr int KC = 32 * (KEYS ? NG : 1);       // keys of a chunk; 64 for many rows: 3 to 9 % slower
     constexpr int TILE = KC * RB;
     typedef typename Op<T>::Chunk Chunk;
-    __shared__ __align__(16) char bufs[2][2 * TILE];
+    constexpr int BUF = KEYS || 2 * TILE > NG * DB * 2048 ? 2 * TILE : NG * DB * 2048;      // many rows: DB sums of a pair fit
+    __shared__ __align__(16) char bufs[2][BUF];
     __shared__ float s_ml[KEYS ? NG : 1][4][32];
     __shared__ float s_w[KEYS ? 32 : 1];
 
+    arguments(a);
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), map = wave & 1, grp = wave >> 1;
     const int r = lane & 31, hh = lane >> 5;
     const int bks = a.batch * a.kv_heads;
-    const int bk = blockIdx.x % bks;               // workgroups of one head lie bks apart: one XCD where 8 divides bks
-    const int rest = blockIdx.x / bks;
-    const int tile = KEYS ? rest % tiles : (a.causal ? tiles - 1 - rest : rest);     // causal: the longest rows first
+    const int rest = quotient(blockIdx.x, a.by_bks);
+    const int bk = blockIdx.x - rest * bks;        // workgroups of one head lie bks apart: one XCD where 8 divides bks
     const int split = KEYS ? rest / tiles : 0;
-    const int b = bk / a.kv_heads, kh = bk - b * a.kv_heads;
+    const int tile = KEYS ? rest - split * tiles : (a.causal ? tiles - 1 - rest : rest);     // causal: the longest rows first
+    const int b = quotient(bk, a.by_kv_heads), kh = bk - b * a.kv_heads;
     const int nrows = a.nq * a.group;
     const int row0 = KEYS ? tile * 32 : (tile * NG + grp) * 32;
     const int end = KEYS ? tile * 32 + 32 : (tile + 1) * NG * 32;
@@ -79,11 +81,11 @@ __global__ __launch_bounds__(NG * 128, OCC) void diff_fwd(DiffArgs a, DiffOut o,
 
     const int dc = a.d / PER;
     Stage<T, DP, NT, KC> stage;
-    stage.init(tid, dc, bufs[0]);
+    stage.init(tid, dc, bufs[0], BUF);
     const int64_t s_step = stage.second ? a.vs[1] : a.ks[1];
-    const T* s_src = stage.second ? reinterpret_cast<const T*>(a.v) + b * a.vs[0] + kh * a.vs[2] + stage.col * PER
-                                  : reinterpret_cast<const T*>(a.k) + b * a.ks[0] + kh * a.ks[2] + stage.map * a.ks[3] + stage.e * PER;
-    auto fetch = [&](int key0) { stage.fetch(key0, kmax, [&](int key) { return s_src + key * s_step; }); };
+    const T* s_src = stage.row * s_step + (stage.second ? reinterpret_cast<const T*>(a.v) + b * a.vs[0] + kh * a.vs[2] + stage.col * PER
+                                                        : reinterpret_cast<const T*>(a.k) + b * a.ks[0] + kh * a.ks[2] + stage.map * a.ks[3] + stage.e * PER);
+    auto fetch = [&](int key0) { stage.fetch(key0, kmax, s_src, s_step, 0, [&](int key) { return s_src + (key - stage.row) * s_step; }); };
 
     int c0 = 0, c1 = (kmax + KC - 1) / KC;
     if constexpr (KEYS) {
@@ -107,10 +109,10 @@ __global__ __launch_bounds__(NG * 128, OCC) void diff_fwd(DiffArgs a, DiffOut o,
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
             const int c = 2 * t + hh;
-            qf[t] = *reinterpret_cast<const Chunk*>(c < dc ? (const void*)(qg + c * PER) : (const void*)kZeros);
+            qf[t] = chunk_or_zero<T>(qg, c, c < dc);
         }
     }
-    const float weight = map == 0 ? map_weight<DP>(a, place.head, hh) : 0.f;
+    const float weight = KEYS && map ? 0.f : map_weight<DP>(a, place.head, lane);
 
     constexpr bool MSUM = !TRAIN && sizeof(T) == 2;
     f32x16 acc[DB], l_acc = zero16();
@@ -120,15 +122,11 @@ __global__ __launch_bounds__(NG * 128, OCC) void diff_fwd(DiffArgs a, DiffOut o,
     const float sc = a.scale * kLog2e;
     constexpr float kLazy = 8.0f;     // the accumulators are rescaled only when a maximum grows by more than 2^8
 
-    auto step = [&](const char* kt, const char* vt, int kb, int key0) {
+    auto step = [&](const char* kt, const char* vt, int kb, int key0, bool fresh) __attribute__((always_inline)) {
         f32x16 s = zero16();
 #pragma unroll
         for (int t = 0; t < KT; ++t) s = Op<T>::mma(chunk_at<T, RB>(kt, kb * 32 + r, map * DPC + 2 * t + hh), qf[t], s);
-        if (key0 + 32 > wave_min) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (key0 + 8 * (i >> 2) + 4 * hh + (i & 3) >= lim) s[i] = -__builtin_inff();
-        }
+        if (key0 + 32 > wave_min) hide(s, lim - key0 - 4 * hh);
         float mx = fmaxf(s[0], s[1]);
 #pragma unroll
         for (int i = 2; i < 16; i += 2) mx = fmaxf(fmaxf(mx, s[i]), s[i + 1]);
@@ -137,16 +135,18 @@ __global__ __launch_bounds__(NG * 128, OCC) void diff_fwd(DiffArgs a, DiffOut o,
             const float m_new = fmaxf(m_run, mx);
             const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
             m_run = m_new;
-            if constexpr (MSUM) {
+            if (!fresh) {                                            // nothing to rescale before the first block
+                if constexpr (MSUM) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) l_acc[i] *= alpha;
-            } else {
-                l_run *= alpha;
+                    for (int i = 0; i < 16; ++i) l_acc[i] *= alpha;
+                } else {
+                    l_run *= alpha;
+                }
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[d][i] *= alpha;
             }
-#pragma unroll
-            for (int d = 0; d < DB; ++d)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) acc[d][i] *= alpha;
         }
         float sum = 0.f;
 #pragma unroll
@@ -171,14 +171,18 @@ __global__ __launch_bounds__(NG * 128, OCC) void diff_fwd(DiffArgs a, DiffOut o,
     if (c0 < c1) stage.put(bufs[0]);
     loads_done();
     __syncthreads();
-    for (int c = c0; c < c1; ++c) {
-        const char* buf = bufs[(c - c0) & 1];
+    auto chunk = [&](int c, auto which) __attribute__((always_inline)) {                            // the buffer is known when compiled: no address arithmetic
+        const char* buf = bufs[decltype(which)::value];
         const bool more = c + 1 < c1;
         if (more) fetch((c + 1) * KC);
         const int key0 = c * KC + (KEYS ? grp * 32 : 0);             // few rows: the pair's block of the chunk
-        if (active && key0 < wave_max) step(buf, buf + TILE, KEYS ? grp : 0, key0);
-        if (more) stage.put(bufs[(c - c0 + 1) & 1]);
+        if (active && key0 < wave_max) step(buf, buf + TILE, KEYS ? grp : 0, key0, c == c0);
+        if (more) stage.put(bufs[decltype(which)::value ^ 1]);
         __syncthreads();
+    };
+    for (int c = c0; c < c1; c += 2) {
+        chunk(c, std::integral_constant<int, 0>{});
+        if (c + 1 < c1) chunk(c + 1, std::integral_constant<int, 1>{});
     }
 
     const float l_tot = MSUM ? l_acc[0] : both_sum(l_run);           // each element of l_acc holds the lane's whole sum
@@ -196,38 +200,31 @@ __global__ __launch_bounds__(NG * 128, OCC) void diff_fwd(DiffArgs a, DiffOut o,
             o.stats[(2 + map) * lmap + lrow] = inv;
             if (map == 0 && b == 0 && place.tok == 0) o.weight[place.head] = weight;
         }
-        // the second map's wave hands its sums over, as many 32-column blocks at a time as the buffers hold
-        constexpr int FIT = 4 * TILE / (NG * 4096) < DB ? 4 * TILE / (NG * 4096) : DB;
-        static_assert(FIT >= 1, "one block of columns fits the buffers");
-        f32x4* box = reinterpret_cast<f32x4*>(bufs[0]) + grp * FIT * 256 + hh * 32 + r;
+        // the pair's waves exchange sums: the first finishes the first D0 blocks of 32 columns, the second the others
+        constexpr int D0 = (DB + 1) / 2;
+        f32x4* box = reinterpret_cast<f32x4*>(bufs[0]) + grp * DB * 256 + lane;
 #pragma unroll
-        for (int d0 = 0; d0 < DB; d0 += FIT) {
-            if (d0) __syncthreads();
-            if (map == 1) {
+        for (int d = 0; d < DB; ++d) {
+            if ((d < D0) == (map == 0)) continue;
 #pragma unroll
-                for (int d = d0; d < d0 + FIT && d < DB; ++d)
+            for (int g = 0; g < 4; ++g) box[d * 256 + g * 64] = four(acc[d], g, inv);
+        }
+        __syncthreads();
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const f32x4 y = {acc[d][4 * g] * inv, acc[d][4 * g + 1] * inv, acc[d][4 * g + 2] * inv, acc[d][4 * g + 3] * inv};
-                        box[(d - d0) * 256 + g * 64] = y;
-                        const int col = d * 32 + 8 * g + 4 * hh;
-                        if (TRAIN && live && col < 2 * a.d) store4(out2 + orow + col, y);
-                    }
-            }
-            __syncthreads();
-            if (map == 0 && live) {
+        for (int d = 0; d < DB; ++d) {
+            if ((d < D0) != (map == 0)) continue;
 #pragma unroll
-                for (int d = d0; d < d0 + FIT && d < DB; ++d)
+            for (int g = 0; g < 4; g += 2) {
+                f32x4 x[2], y[2];
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const int col = d * 32 + 8 * g + 4 * hh;
-                        if (col >= 2 * a.d) continue;
-                        const f32x4 y = box[(d - d0) * 256 + g * 64];
-                        f32x4 x;
+                for (int i = 0; i < 2; ++i) {
+                    const f32x4 mine = four(acc[d], g + i, inv), other = box[d * 256 + (g + i) * 64];
+                    y[i] = map ? mine : other;
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) x[j] = fmaf(-weight, y[j], acc[d][4 * g + j] * inv);
-                        store4(out + orow + col, x);
-                    }
+                    for (int j = 0; j < 4; ++j) x[i][j] = fmaf(-weight, y[i][j], map ? other[j] : mine[j]);
+                }
+                store_pair(out + orow, d * 32 + 8 * g, hh, 2 * a.d, live, x[0], x[1]);
+                if (TRAIN) store_pair(out2 + orow, d * 32 + 8 * g, hh, 2 * a.d, live, y[0], y[1]);
             }
         }
     } else {
@@ -320,7 +317,7 @@ __global__ __launch_bounds__(256) void diff_fwd_join(DiffArgs a, DiffOut o, cons
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int nrows = a.nq * a.group;
     const int bk = blockIdx.x / nrows, row = blockIdx.x - bk * nrows, tile = row >> 5, rr = row & 31;
-    const int b = bk / a.kv_heads, kh = bk - b * a.kv_heads;
+    const int b = quotient(bk, a.by_kv_heads), kh = bk - b * a.kv_heads;
     const RowPlace pl = row_place(a, kh, row);
     const float* base = ws + ((int64_t)bk * tiles + tile) * splits * STRIDE;
     // the splits' values are on their way while the factors are computed
@@ -358,7 +355,7 @@ __global__ __launch_bounds__(256) void diff_fwd_join(DiffArgs a, DiffOut o, cons
             }
         }
     } else if (wave == 2) {
-        const float w = map_weight<DV / 2>(a, pl.head, lane >> 5);
+        const float w = map_weight<DV / 2>(a, pl.head, lane);
         if (lane == 0) {
             s_w = w;
             if (o.out2 && b == 0 && pl.tok == 0) o.weight[pl.head] = w;

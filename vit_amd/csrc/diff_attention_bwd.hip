@@ -56,9 +56,9 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_q(DiffArgs a, DiffGrad
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), map = wave & 1, grp = wave >> 1;
     const int r = lane & 31, hh = lane >> 5;
     const int bks = a.batch * a.kv_heads;
-    const int bk = blockIdx.x % bks, rest = blockIdx.x / bks;
+    const int rest = quotient(blockIdx.x, a.by_bks), bk = blockIdx.x - rest * bks;
     const int tile = a.causal ? tiles - 1 - rest : rest;
-    const int b = bk / a.kv_heads, kh = bk - b * a.kv_heads;
+    const int b = quotient(bk, a.by_kv_heads), kh = bk - b * a.kv_heads;
     const int nrows = a.nq * a.group;
     const int row0 = tile * kBlock + grp * 32, end = (tile + 1) * kBlock;
     const int len = sample_len(a, b);
@@ -66,11 +66,11 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_q(DiffArgs a, DiffGrad
 
     const int dc = a.d / PER;
     Stage<T, DP, kThreads, KC> stage;
-    stage.init(tid, dc, bufs[0]);
+    stage.init(tid, dc, bufs[0], 2 * TILE);
     const int64_t s_step = stage.second ? a.vs[1] : a.ks[1];
-    const T* s_src = stage.second ? reinterpret_cast<const T*>(a.v) + b * a.vs[0] + kh * a.vs[2] + stage.col * PER
-                                  : reinterpret_cast<const T*>(a.k) + b * a.ks[0] + kh * a.ks[2] + stage.map * a.ks[3] + stage.e * PER;
-    auto fetch = [&](int key0) { stage.fetch(key0, kmax, [&](int key) { return s_src + key * s_step; }); };
+    const T* s_src = stage.row * s_step + (stage.second ? reinterpret_cast<const T*>(a.v) + b * a.vs[0] + kh * a.vs[2] + stage.col * PER
+                                                        : reinterpret_cast<const T*>(a.k) + b * a.ks[0] + kh * a.ks[2] + stage.map * a.ks[3] + stage.e * PER);
+    auto fetch = [&](int key0) { stage.fetch(key0, kmax, s_src, s_step, 0, [&](int key) { return s_src + (key - stage.row) * s_step; }); };
     const int c1 = (kmax + KC - 1) / KC;
     if (c1 > 0) fetch(0);
 
@@ -92,7 +92,7 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_q(DiffArgs a, DiffGrad
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
             const int c = 2 * t + hh;
-            qf[t] = *reinterpret_cast<const Chunk*>(c < dc ? (const void*)(qg + c * PER) : (const void*)kZeros);
+            qf[t] = chunk_or_zero<T>(qg, c, c < dc);
         }
         const int64_t orow = (((int64_t)b * a.nq + place.tok) * a.heads + place.head) * 2 * a.d;
         float d0 = 0.f, d2 = 0.f;
@@ -101,7 +101,7 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_q(DiffArgs a, DiffGrad
             const int c = 2 * t + hh;
             const bool on = c < 2 * dc;
             auto at = [&](const void* p) {
-                return *reinterpret_cast<const Chunk*>(on ? (const void*)(reinterpret_cast<const T*>(p) + orow + c * PER) : (const void*)kZeros);
+                return chunk_or_zero<T>(reinterpret_cast<const T*>(p) + orow, c, on);
             };
             of[t] = at(g.dout);
             d2 += dot<T>(of[t], at(g.out2));
@@ -121,25 +121,21 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_q(DiffArgs a, DiffGrad
     if (c1 > 0) stage.put(bufs[0]);
     loads_done();
     __syncthreads();
-    for (int c = 0; c < c1; ++c) {
-        const char* kt = bufs[c & 1];
+    auto chunk = [&](int c, auto which) __attribute__((always_inline)) {                            // the buffer is known when compiled: no address arithmetic
+        const char* kt = bufs[decltype(which)::value];
         const char* vt = kt + TILE;
         const bool more = c + 1 < c1;
         if (more) fetch((c + 1) * KC);
-#pragma unroll 2
+#pragma unroll
         for (int kb = 0; kb < KC; kb += 32) {
             const int key0 = c * KC + kb;
-            if (!active || key0 >= wave_max) break;
+            if (!active || key0 >= wave_max) continue;
             f32x16 s = zero16(), da = zero16();
 #pragma unroll
             for (int t = 0; t < KT; ++t) s = Op<T>::mma(chunk_at<T, RB>(kt, kb + r, map * DPC + 2 * t + hh), qf[t], s);
 #pragma unroll
             for (int t = 0; t < 2 * KT; ++t) da = Op<T>::mma(chunk_at<T, RB>(vt, kb + r, 2 * t + hh), of[t], da);
-            if (key0 + 32 > wave_min) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (key0 + 8 * (i >> 2) + 4 * hh + (i & 3) >= lim) s[i] = -__builtin_inff();
-            }
+            if (key0 + 32 > wave_min) hide(s, lim - key0 - 4 * hh);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const float p = __builtin_amdgcn_exp2f(fmaf(s[i], sc, -ref));     // times 1 / l at the end
@@ -158,8 +154,12 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_q(DiffArgs a, DiffGrad
                 }
             }
         }
-        if (more) stage.put(bufs[(c + 1) & 1]);
+        if (more) stage.put(bufs[decltype(which)::value ^ 1]);
         __syncthreads();
+    };
+    for (int c = 0; c < c1; c += 2) {
+        chunk(c, std::integral_constant<int, 0>{});
+        if (c + 1 < c1) chunk(c + 1, std::integral_constant<int, 1>{});
     }
 
     dw = both_sum(dw) * inv;
@@ -172,17 +172,13 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_q(DiffArgs a, DiffGrad
         for (int i = (h - first % a.group + a.group) % a.group; i < kBlock; i += a.group) t += s_dw[i];
         ws_w[((int64_t)bk * tiles + tile) * a.group + h] = t;
     }
-    if (row >= nrows) return;
     T* out = reinterpret_cast<T*>(g.dq) + b * g.dqs[0] + place.tok * g.dqs[1] + place.head * g.dqs[2] + map * g.dqs[3];
     const float f = map == 0 ? inv * a.scale : -weight * inv * a.scale;
 #pragma unroll
     for (int e = 0; e < EB; ++e)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int col = e * 32 + 8 * q + 4 * hh;
-            if (col >= a.d) continue;
-            store4(out + col, f32x4{dq[e][4 * q] * f, dq[e][4 * q + 1] * f, dq[e][4 * q + 2] * f, dq[e][4 * q + 3] * f});
-        }
+        for (int q = 0; q < 4; q += 2)
+            store_pair(out, e * 32 + 8 * q, hh, a.d, row < nrows, four(dq[e], q, f), four(dq[e], q + 1, f));
 }
 
 // dK and dV of 32 NP keys.  What a row contributes beside its Q and dO is folded into the products' initial accumulators:
@@ -200,7 +196,8 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_kv(DiffArgs a, DiffGra
     constexpr int RC = 32 * NB, TILE = RC * RB;                       // RC: rows of a chunk
     constexpr int NS = ONE ? 4 : 5;
     typedef typename Op<T>::Chunk Chunk;
-    __shared__ __align__(16) char bufs[2][2 * TILE];                  // Q of both maps, dO
+    constexpr int BUF = 2 * TILE > NP * DB * 2048 ? 2 * TILE : NP * DB * 2048;              // DB sums of a pair fit
+    __shared__ __align__(16) char bufs[2][BUF];                       // Q of both maps, dO
     __shared__ __align__(16) float s_row[2][NS][RC];                  // -lse_1 / sc, -lse_2 / sc, -D_1, -D_2, w
     __shared__ __align__(16) int s_lim[2][RC];
 
@@ -208,8 +205,8 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_kv(DiffArgs a, DiffGra
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), map = wave & 1, grp = wave >> 1;
     const int r = lane & 31, hh = lane >> 5;
     const int bks = a.batch * a.kv_heads;
-    const int bk = blockIdx.x % bks, rest = blockIdx.x / bks, tile = rest / splits;      // causal: the first keys have the most rows
-    const int b = bk / a.kv_heads, kh = bk - b * a.kv_heads;
+    const int rest = quotient(blockIdx.x, a.by_bks), bk = blockIdx.x - rest * bks, tile = rest / splits;      // causal: the first keys have the most rows
+    const int b = quotient(bk, a.by_kv_heads), kh = bk - b * a.kv_heads;
     const int nrows = a.nq * a.group;
     const int len = sample_len(a, b);
     const int block0 = tile * kBlock, key0 = block0 + grp * 32, key = key0 + r;
@@ -229,11 +226,17 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_kv(DiffArgs a, DiffGra
 
     const int dc = a.d / PER;
     Stage<T, DP, kThreads, RC> stage;
-    stage.init(tid, dc, bufs[0]);
+    stage.init(tid, dc, bufs[0], BUF);
     const int64_t s_tok = stage.second ? (int64_t)a.heads * 2 * a.d : a.qs[1], s_head = stage.second ? 2 * a.d : a.qs[2];
-    const T* s_src = stage.second ? reinterpret_cast<const T*>(g.dout) + (int64_t)b * a.nq * a.heads * 2 * a.d + stage.col * PER
-                                  : reinterpret_cast<const T*>(a.q) + b * a.qs[0] + stage.map * a.qs[3] + stage.e * PER;
-    if (ONE) s_src += kh * s_head;
+    const T* s_base = stage.second ? reinterpret_cast<const T*>(g.dout) + (int64_t)b * a.nq * a.heads * 2 * a.d + stage.col * PER
+                                   : reinterpret_cast<const T*>(a.q) + b * a.qs[0] + stage.map * a.qs[3] + stage.e * PER;
+    auto addr = [&](int row) {
+        const RowPlace pl = ONE ? RowPlace{row, kh} : row_place(a, kh, row);
+        return s_base + pl.tok * s_tok + pl.head * s_head;
+    };
+    // a group of heads that divides the rows of a pass: the token moves on alike for all of them
+    const int s_shift = ONE ? 0 : (a.group & (a.group - 1)) == 0 && a.group <= stage.ROWS ? 31 - __builtin_clz(a.group) : -1;
+    const T* s_src = addr(stage.row);
     const int64_t lmap = (int64_t)a.batch * a.heads * a.nq;
     static_assert(4 * RC <= kThreads, "four values of a row have a thread each");
     // the rows' values: a thread brings one to four of them, raw; what is computed from them waits until they are put
@@ -241,11 +244,7 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_kv(DiffArgs a, DiffGra
     const float* s_from = role < 2 ? g.stats + role * lmap : ws_d + (role - 2) * lmap;
     float held0 = 0.f, held1 = 0.f, held_w = 0.f;
     auto fetch = [&](int c) {
-        stage.fetch(c * RC, nrows, [&](int row) {
-            if constexpr (ONE) return s_src + row * s_tok;
-            const RowPlace pl = row_place(a, kh, row);
-            return s_src + pl.tok * s_tok + pl.head * s_head;
-        });
+        stage.fetch(c * RC, nrows, s_src, s_tok, s_shift, addr);
         const int row = c * RC + s_at;
         if (role < 4 && row < nrows) {
             const RowPlace pl = ONE ? RowPlace{row, kh} : row_place(a, kh, row);
@@ -274,12 +273,12 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_kv(DiffArgs a, DiffGra
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
             const int c = 2 * t + hh;
-            kf[t] = *reinterpret_cast<const Chunk*>(on && c < dc ? (const void*)(kg + c * PER) : (const void*)kZeros);
+            kf[t] = chunk_or_zero<T>(kg, c, on && c < dc);
         }
 #pragma unroll
         for (int t = 0; t < 2 * KT; ++t) {
             const int c = 2 * t + hh;
-            vf[t] = *reinterpret_cast<const Chunk*>(on && c < 2 * dc ? (const void*)(vg + c * PER) : (const void*)kZeros);
+            vf[t] = chunk_or_zero<T>(vg, c, on && c < 2 * dc);
         }
     }
 
@@ -292,8 +291,8 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_kv(DiffArgs a, DiffGra
     if (first < c1) put(0, first);
     loads_done();
     __syncthreads();
-    for (int c = first; c < c1; ++c) {
-        const int k = (c - first) & 1;
+    auto chunk = [&](int c, auto which) __attribute__((always_inline)) {
+        const int k = which;
         const char* qt = bufs[k];
         const char* ot = qt + TILE;
         const bool more = c + 1 < c1;
@@ -302,7 +301,7 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_kv(DiffArgs a, DiffGra
 #pragma unroll 1
         for (int rb = 0; rb < RC; rb += 32) {
             const int at0 = c * RC + rb, last = at0 + 32 < nrows ? at0 + 32 : nrows;
-            if (at0 >= nrows) break;
+            if (at0 >= nrows) continue;
             if (key0 >= key_limit(a, len, row_place(a, kh, last - 1).tok)) continue;
             auto rows16 = [&](int j) {                                // row values in the accumulators' layout
                 f32x16 v;
@@ -353,53 +352,51 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_kv(DiffArgs a, DiffGra
         }
         if (more) put(k ^ 1, c + 1);
         __syncthreads();
+    };
+    if constexpr (sizeof(T) == 4) {                                   // twice the body costs f32 more than the addresses: 97 / 83 us
+        for (int c = first; c < c1; ++c) chunk(c, (c - first) & 1);
+    } else {
+        for (int c = first; c < c1; c += 2) {
+            chunk(c, std::integral_constant<int, 0>{});
+            if (c + 1 < c1) chunk(c + 1, std::integral_constant<int, 1>{});
+        }
     }
 
     const bool live = key < a.nk;
     const float f = map == 0 ? 1.f : ONE ? -g.weight[kh] : -1.f;      // the second map's part
     // [split][sample, key head][key][dK of both maps, dV]
     float* part = splits > 1 ? parts + (((int64_t)(rest - tile * splits) * bks + bk) * a.nk + key) * 4 * a.d : nullptr;
-    if (live) {
+    {
         T* ko = reinterpret_cast<T*>(g.dk) + b * g.dks[0] + (int64_t)key * g.dks[1] + kh * g.dks[2] + map * g.dks[3];
         const float fk = f * a.scale;
 #pragma unroll
         for (int e = 0; e < EB; ++e)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int col = e * 32 + 8 * q + 4 * hh;
-                if (col >= a.d) continue;
-                const f32x4 x = {dk[e][4 * q] * fk, dk[e][4 * q + 1] * fk, dk[e][4 * q + 2] * fk, dk[e][4 * q + 3] * fk};
-                if (part) *reinterpret_cast<f32x4*>(part + map * a.d + col) = x;
-                else store4(ko + col, x);
+            for (int q = 0; q < 4; q += 2) {
+                const f32x4 x = four(dk[e], q, fk), y = four(dk[e], q + 1, fk);
+                if (part) store_pair(part + map * a.d, e * 32 + 8 * q, hh, a.d, live, x, y);
+                else store_pair(ko, e * 32 + 8 * q, hh, a.d, live, x, y);
             }
     }
+    // the pair's waves exchange their parts of dV: the first finishes the first D0 blocks of 32 columns, the second the others
     T* vo = reinterpret_cast<T*>(g.dv) + b * g.dvs[0] + (int64_t)key * g.dvs[1] + kh * g.dvs[2];
-    constexpr int FIT = 4 * TILE / (NP * 4096) < DB ? 4 * TILE / (NP * 4096) : DB;
-    static_assert(FIT >= 1, "one block of columns fits the buffers");
-    f32x4* box = reinterpret_cast<f32x4*>(bufs[0]) + grp * FIT * 256 + hh * 32 + r;
+    constexpr int D0 = (DB + 1) / 2;
+    f32x4* box = reinterpret_cast<f32x4*>(bufs[0]) + grp * DB * 256 + lane;
 #pragma unroll
-    for (int d0 = 0; d0 < DB; d0 += FIT) {
-        if (d0) __syncthreads();
-        if (map == 1) {
+    for (int d = 0; d < DB; ++d) {
+        if ((d < D0) == (map == 0)) continue;
 #pragma unroll
-            for (int d = d0; d < d0 + FIT && d < DB; ++d)
+        for (int q = 0; q < 4; ++q) box[d * 256 + q * 64] = four(dv[d], q, f);
+    }
+    __syncthreads();
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    box[(d - d0) * 256 + q * 64] = f32x4{dv[d][4 * q] * f, dv[d][4 * q + 1] * f, dv[d][4 * q + 2] * f, dv[d][4 * q + 3] * f};
-        }
-        __syncthreads();
-        if (map == 0 && live) {
+    for (int d = 0; d < DB; ++d) {
+        if ((d < D0) != (map == 0)) continue;
 #pragma unroll
-            for (int d = d0; d < d0 + FIT && d < DB; ++d)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int col = d * 32 + 8 * q + 4 * hh;
-                    if (col >= 2 * a.d) continue;
-                    const f32x4 y = box[(d - d0) * 256 + q * 64];
-                    const f32x4 x = {dv[d][4 * q] + y[0], dv[d][4 * q + 1] + y[1], dv[d][4 * q + 2] + y[2], dv[d][4 * q + 3] + y[3]};
-                    if (part) *reinterpret_cast<f32x4*>(part + 2 * a.d + col) = x;
-                    else store4(vo + col, x);
-                }
+        for (int q = 0; q < 4; q += 2) {
+            const f32x4 x = four(dv[d], q, f) + box[d * 256 + q * 64], y = four(dv[d], q + 1, f) + box[d * 256 + (q + 1) * 64];
+            if (part) store_pair(part + 2 * a.d, d * 32 + 8 * q, hh, 2 * a.d, live, x, y);
+            else store_pair(vo, d * 32 + 8 * q, hh, 2 * a.d, live, x, y);
         }
     }
 }
@@ -465,6 +462,7 @@ __global__ __launch_bounds__(256) void diff_bwd_lam(DiffArgs a, const float* __r
 // all 512 registers.
 template <class T>
 constexpr int pairs() { return sizeof(T) == 4 ? 2 : 4; }
+constexpr int kRowPairs = 2;
 
 int64_t row_tiles(const DiffArgs& a, int np) { return ((int64_t)a.nq * a.group + 32 * np - 1) / (32 * np); }
 int64_t key_tiles(const DiffArgs& a, int np) { return ((int64_t)a.nk + 32 * np - 1) / (32 * np); }
@@ -495,13 +493,13 @@ hipError_t launch(const DiffArgs& a, const DiffGrads& g, float* ws, hipStream_t 
     // 80.6 / 81;  dK and dV 102.8 / 100.8, 454 / 542, 93 / 85
     constexpr int NBQ = sizeof(T) == 4 ? 1 : 2, NBK = sizeof(T) == 4 ? 2 : 1;
     const int64_t bks = (int64_t)a.batch * a.kv_heads;
-    const int64_t qt = row_tiles(a, NP), kt = key_tiles(a, NP), keys = (int64_t)a.batch * a.kv_heads * a.nk;
+    const int64_t qt = row_tiles(a, kRowPairs), kt = key_tiles(a, NP), keys = (int64_t)a.batch * a.kv_heads * a.nk;
     const int splits = row_splits(a, NP);
     if (bks * qt > 0x7FFFFFFF || bks * kt * splits > 0x7FFFFFFF || keys * a.d / 256 > 0x7FFFFFF0) return hipErrorInvalidValue;
     float* parts = ws;
     float* ws_d = ws + parts_floats(a, NP);
     float* ws_w = ws_d + 2 * (int64_t)a.batch * a.heads * a.nq;
-    hipLaunchKernelGGL((diff_bwd_q<T, DP, NP, NBQ, OCC>), dim3((int)(bks * qt)), dim3(NP * 128), 0, s, a, g, ws_d, ws_w, (int)qt);
+    hipLaunchKernelGGL((diff_bwd_q<T, DP, kRowPairs, NBQ, OCC>), dim3((int)(bks * qt)), dim3(kRowPairs * 128), 0, s, a, g, ws_d, ws_w, (int)qt);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const dim3 grid((int)(bks * kt * splits)), block(NP * 128);
@@ -524,7 +522,7 @@ hipError_t launch(const DiffArgs& a, const DiffGrads& g, float* ws, hipStream_t 
 // f32 values of scratch of the backward
 int64_t diff_attention_bwd_workspace(const DiffArgs& a, bool bf16) {
     const int np = bf16 ? pairs<bf16_t>() : pairs<float>();
-    return parts_floats(a, np) + 2 * (int64_t)a.batch * a.heads * a.nq + (int64_t)a.batch * a.heads * row_tiles(a, np);
+    return parts_floats(a, np) + 2 * (int64_t)a.batch * a.heads * a.nq + (int64_t)a.batch * a.heads * row_tiles(a, kRowPairs);
 }
 
 hipError_t launch_diff_attention_backward(const DiffArgs& a, const DiffGrads& g, float* ws, bool bf16, hipStream_t s) {

@@ -634,6 +634,11 @@ int vitk_group_norm_backward(const void* x, const float* weight, const float* bi
 
 // ---- differential attention ------------------------------------------------------------------------
 
+static Divisor divisor(int d) {
+    const int l = ilog2(d);
+    return d > 1 ? Divisor{(unsigned)(((uint64_t)1 << (31 + l)) / (unsigned)d + 1), (unsigned)l - 1} : Divisor{0, 0};
+}
+
 static int diff_args(const char* name, DiffArgs& a, const void* q, const void* k, const void* v, const int64_t* strides,
                      const float* lam, int lam_heads, float lambda_init, float scale, const int* key_lens, int causal,
                      int batch, int nq, int nk, int heads, int kv_heads, int d, int dtype) {
@@ -659,9 +664,7 @@ static int diff_args(const char* name, DiffArgs& a, const void* q, const void* k
     for (int i = 0; i < 3; ++i) a.vs[i] = strides[8 + i];
     a.lam = lam; a.key_lens = key_lens;
     a.batch = batch; a.nq = nq; a.nk = nk; a.heads = heads; a.kv_heads = kv_heads; a.group = heads / kv_heads;
-    int l = ilog2(a.group);
-    a.group_shift = l > 0 ? l - 1 : 0;
-    a.group_mul = l > 0 ? (unsigned)(((uint64_t)1 << (31 + l)) / (unsigned)a.group + 1) : 0;
+    a.by_group = divisor(a.group); a.by_kv_heads = divisor(kv_heads); a.by_bks = divisor(batch * kv_heads);
     a.d = d; a.lam_heads = lam_heads; a.causal = causal != 0; a.scale = scale; a.lambda_init = lambda_init;
     return VITK_OK;
 }

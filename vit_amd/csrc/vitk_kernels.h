@@ -119,6 +119,12 @@ hipError_t launch_grad_scale(const uint64_t* addr, const int64_t* size, const in
                              const double* partials, int npartials, double max_norm, float* norm, hipStream_t s);
 
 // differential attention (diff_attention.hip, diff_attention_bwd.hip); strides in elements, the last dimension dense
+// Division of n < 2^31 by d: n mul >> (32 + shift) with mul = 2^(31 + l) / d + 1, 2^l >= d, shift = l - 1: n mul / 2^(31 + l)
+// exceeds n / d by less than 1 / d.  mul = 0: d is 1.
+struct Divisor {
+    unsigned mul, shift;
+};
+
 struct DiffArgs {
     const void *q, *k, *v;        // [batch, nq, heads, 2, d], [batch, nk, kv_heads, 2, d], [batch, nk, kv_heads, 2 d]
     int64_t qs[4], ks[4], vs[3];  // strides: sample, token, head, map (v: sample, token, head)
@@ -126,7 +132,7 @@ struct DiffArgs {
     const int* key_lens;          // [batch] or nullptr
     int batch, nq, nk, heads, kv_heads, group, d, lam_heads;   // group = heads / kv_heads
     int causal;
-    unsigned group_mul, group_shift;   // division by group (diff_attention.h)
+    Divisor by_group, by_kv_heads, by_bks;   // bks = batch kv_heads
     float scale, lambda_init;
 };
 // forward: out [batch, nq, heads, 2 d]; for the backward also out2 (the second map's product with V, out's shape), stats
