@@ -50,8 +50,9 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_q(DiffArgs a, DiffGrad
     constexpr int KC = 32 * NB, TILE = KC * RB;                       // KC: keys of a chunk
     typedef typename Op<T>::Chunk Chunk;
     __shared__ __align__(16) char bufs[2][2 * TILE];
-    __shared__ float s_dw[kBlock];
+    __shared__ float s_dw[kBlock], s_dot[NP][2][32];
 
+    arguments(a);
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), map = wave & 1, grp = wave >> 1;
     const int r = lane & 31, hh = lane >> 5;
@@ -86,7 +87,6 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_q(DiffArgs a, DiffGrad
     const float ref = g.stats[map * lmap + lrow], inv = g.stats[(2 + map) * lmap + lrow];
 
     Chunk qf[KT], of[2 * KT];
-    float dd;
     {
         const T* qg = reinterpret_cast<const T*>(a.q) + b * a.qs[0] + place.tok * a.qs[1] + place.head * a.qs[2] + map * a.qs[3];
 #pragma unroll
@@ -94,22 +94,19 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_q(DiffArgs a, DiffGrad
             const int c = 2 * t + hh;
             qf[t] = chunk_or_zero<T>(qg, c, c < dc);
         }
+        // dO . O by the first map's wave, dO . O_2 by the second's, all loads at once
         const int64_t orow = (((int64_t)b * a.nq + place.tok) * a.heads + place.head) * 2 * a.d;
-        float d0 = 0.f, d2 = 0.f;
+        const T* og = reinterpret_cast<const T*>(map ? g.out2 : g.out) + orow;
+        Chunk o[2 * KT];
 #pragma unroll
-        for (int t = 0; t < 2 * KT; ++t) {
-            const int c = 2 * t + hh;
-            const bool on = c < 2 * dc;
-            auto at = [&](const void* p) {
-                return chunk_or_zero<T>(reinterpret_cast<const T*>(p) + orow, c, on);
-            };
-            of[t] = at(g.dout);
-            d2 += dot<T>(of[t], at(g.out2));
-            if (map == 0) d0 += dot<T>(of[t], at(g.out));
-        }
-        dd = both_sum(d2);
-        if (map == 0) dd = fmaf(weight, dd, both_sum(d0));
-        if (row < nrows && hh == 0) ws_d[map * lmap + lrow] = dd;
+        for (int t = 0; t < 2 * KT; ++t) of[t] = chunk_or_zero<T>(reinterpret_cast<const T*>(g.dout) + orow, 2 * t + hh, 2 * t + hh < 2 * dc);
+#pragma unroll
+        for (int t = 0; t < 2 * KT; ++t) o[t] = chunk_or_zero<T>(og, 2 * t + hh, 2 * t + hh < 2 * dc);
+        float s = 0.f;
+#pragma unroll
+        for (int t = 0; t < 2 * KT; ++t) s += dot<T>(of[t], o[t]);
+        s = both_sum(s);
+        if (hh == 0) s_dot[grp][map][r] = s;
     }
 
     f32x16 dq[EB];
@@ -121,6 +118,8 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_q(DiffArgs a, DiffGrad
     if (c1 > 0) stage.put(bufs[0]);
     loads_done();
     __syncthreads();
+    const float dd = map ? s_dot[grp][1][r] : fmaf(weight, s_dot[grp][1][r], s_dot[grp][0][r]);
+    if (row < nrows && hh == 0) ws_d[map * lmap + lrow] = dd;
     auto chunk = [&](int c, auto which) __attribute__((always_inline)) {                            // the buffer is known when compiled: no address arithmetic
         const char* kt = bufs[decltype(which)::value];
         const char* vt = kt + TILE;
@@ -201,6 +200,7 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_kv(DiffArgs a, DiffGra
     __shared__ __align__(16) float s_row[2][NS][RC];                  // -lse_1 / sc, -lse_2 / sc, -D_1, -D_2, w
     __shared__ __align__(16) int s_lim[2][RC];
 
+    arguments(a);
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), map = wave & 1, grp = wave >> 1;
     const int r = lane & 31, hh = lane >> 5;
