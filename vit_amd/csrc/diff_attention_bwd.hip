@@ -182,6 +182,8 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_q(DiffArgs a, DiffGrad
 
 // dK and dV of 32 NP keys.  What a row contributes beside its Q and dO is folded into the products' initial accumulators:
 //     S_m starts at -lse_m / (scale log2 e), so that P_m = exp2(scale log2(e) S_m);  dA starts at -D_m.
+// In f32 it starts at the reference point alone and 1 / l_m is multiplied on: lse is the larger number, and its rounding
+// would be most of the probability's error (1.1e-6 against 5e-7 in dV at 257 tokens).
 // ONE: one query head to a key head, so that w is the workgroup's and can wait until the end (else the rows bring theirs).
 template <class T, int DP, bool ONE, int NP, int NB, int OCC>
 __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_kv(DiffArgs a, DiffGrads g, const float* __restrict__ ws_d,
@@ -193,11 +195,12 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_kv(DiffArgs a, DiffGra
     constexpr int DPC = DP / PER, KT = DPC / 2;
     constexpr int DB = DV / 32, EB = (DP + 31) / 32;
     constexpr int RC = 32 * NB, TILE = RC * RB;                       // RC: rows of a chunk
-    constexpr int NS = ONE ? 4 : 5;
+    constexpr bool APART = sizeof(T) == 4;                            // 1 / l apart from the exponent
+    constexpr int NS = 4 + (APART ? 2 : 0) + (ONE ? 0 : 1);
     typedef typename Op<T>::Chunk Chunk;
     constexpr int BUF = 2 * TILE > NP * DB * 2048 ? 2 * TILE : NP * DB * 2048;              // DB sums of a pair fit
     __shared__ __align__(16) char bufs[2][BUF];                       // Q of both maps, dO
-    __shared__ __align__(16) float s_row[2][NS][RC];                  // -lse_1 / sc, -lse_2 / sc, -D_1, -D_2, w
+    __shared__ __align__(16) float s_row[2][NS][RC];                  // -lse_1 / sc, -lse_2 / sc, -D_1, -D_2, 1 / l_1, 1 / l_2, w
     __shared__ __align__(16) int s_lim[2][RC];
 
     arguments(a);
@@ -259,7 +262,10 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_kv(DiffArgs a, DiffGra
         if (role >= 4) return;
         const int row = c * RC + s_at;
         const bool on = row < nrows;                                  // a row past the last one: P = 0
-        s_row[k][role][s_at] = role < 2 ? (on ? (__builtin_amdgcn_logf(held1) - held0) * rsc : -__builtin_inff()) : on ? -held0 : 0.f;
+        float x = role < 2 ? -__builtin_inff() : 0.f;
+        if (on) x = role >= 2 ? -held0 : APART ? -held0 * rsc : (__builtin_amdgcn_logf(held1) - held0) * rsc;
+        s_row[k][role][s_at] = x;
+        if (APART && role < 2) s_row[k][4 + role][s_at] = on ? held1 : 0.f;
         if (!ONE && role == 1) s_row[k][NS - 1][s_at] = on ? held_w : 0.f;
         if (role == 0) s_lim[k][s_at] = on ? key_limit(a, len, ONE ? row : row_place(a, kh, row).tok) : 0;
     };
@@ -325,6 +331,7 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_kv(DiffArgs a, DiffGra
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i] * sc);
+            if constexpr (APART) s = s * rows16(4 + map);
             if constexpr (!ONE) {
                 if (map == 1) s = s * rows16(NS - 1);
             }
