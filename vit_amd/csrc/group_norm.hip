@@ -194,17 +194,21 @@ __global__ __launch_bounds__(kT) void gn_moments(const T* __restrict__ x, Mom* _
         const bool on = g <= g1;
         const int lo = on ? max(g * q.Cg - c0, 0) : 0, hi = on ? min((g + 1) * q.Cg - c0, wc) : 0;
         const int live = min(rows, len);                             // rows that hold a pixel
+        // lanes over the channels first, over the rows with what is left of them (groups of few channels have many rows)
+        int sh = 0;
+        while ((1 << sh) < q.L && (1 << sh) < hi - lo) ++sh;
+        const int cl = l & ((1 << sh) - 1), cs = 1 << sh, r0 = l >> sh, rs = q.L >> sh;
         const float m0 = s_mean[lo], total = (float)len * (float)(hi - lo);
         float t = 0.f;
-        for (int r = 0; r < live; ++r) {
+        for (int r = r0; r < live; r += rs) {
             const float n = (float)((len - r + rows - 1) / rows);
-            for (int c = lo + l; c < hi; c += q.L) t = fmaf(n, s_mean[r * wc + c] - m0, t);
+            for (int c = lo + cl; c < hi; c += cs) t = fmaf(n, s_mean[r * wc + c] - m0, t);
         }
         const float mean = m0 + lanes_sum(t, q.L) / total;
         t = 0.f;
-        for (int r = 0; r < live; ++r) {
+        for (int r = r0; r < live; r += rs) {
             const float n = (float)((len - r + rows - 1) / rows);
-            for (int c = lo + l; c < hi; c += q.L) {
+            for (int c = lo + cl; c < hi; c += cs) {
                 const float d = s_mean[r * wc + c] - mean;
                 t += fmaf(n * d, d, s_m2[r * wc + c]);
             }
@@ -380,9 +384,25 @@ __global__ __launch_bounds__(kT) void gn_bwd_sums(const T* __restrict__ x, const
     }
     __syncthreads();
     float* o1 = chan + ((int64_t)b * q.chunks + blockIdx.x) * 2 * q.C + c0;
+    // per channel: the rows in kT / wc parts, then the parts
+    const int parts = min(max(kT / wc, 1), rows);
+    if (parts > 1) {
+        for (int i = tid; i < parts * wc; i += kT) {
+            const int p = i / wc, c = i - p * wc;
+            float t1 = 0.f, t2 = 0.f;
+            for (int r = p; r < rows; r += parts) {
+                t1 += s_1[r * wc + c];
+                t2 += s_2[r * wc + c];
+            }
+            s_1[p * wc + c] = t1;                          // rows p, p + parts, ...: this thread's alone
+            s_2[p * wc + c] = t2;
+        }
+        __syncthreads();
+    }
+    const int left = parts > 1 ? parts : rows;
     for (int c = tid; c < wc; c += kT) {
         float t1 = s_1[c], t2 = s_2[c];
-        for (int r = 1; r < rows; ++r) {
+        for (int r = 1; r < left; ++r) {
             t1 += s_1[r * wc + c];
             t2 += s_2[r * wc + c];
         }
