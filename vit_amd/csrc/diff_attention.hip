@@ -123,9 +123,13 @@ __global__ __launch_bounds__(NG * 128, OCC) void diff_fwd(DiffArgs a, DiffOut o,
     constexpr float kLazy = 8.0f;     // the accumulators are rescaled only when a maximum grows by more than 2^8
 
     auto step = [&](const char* kt, const char* vt, int kb, int key0, bool fresh) __attribute__((always_inline)) {
+        // A wave at its products goes first, so that the others of its SIMD fall behind it and compute while it multiplies:
+        // 7 % at head size 64 (1500 tokens 84.4 -> 78.1 us), nothing at 32
         f32x16 s = zero16();
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int t = 0; t < KT; ++t) s = Op<T>::mma(chunk_at<T, RB>(kt, kb * 32 + r, map * DPC + 2 * t + hh), qf[t], s);
+        __builtin_amdgcn_s_setprio(0);
         if (key0 + 32 > wave_min) hide(s, lim - key0 - 4 * hh);
         float mx = fmaxf(s[0], s[1]);
 #pragma unroll
@@ -155,6 +159,7 @@ __global__ __launch_bounds__(NG * 128, OCC) void diff_fwd(DiffArgs a, DiffOut o,
             if constexpr (!MSUM) sum += s[i];
         }
         l_run += sum;
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
             Slice<T> p;
@@ -167,6 +172,7 @@ __global__ __launch_bounds__(NG * 128, OCC) void diff_fwd(DiffArgs a, DiffOut o,
             }
             if constexpr (MSUM) l_acc = ones_t(p, l_acc);
         }
+        __builtin_amdgcn_s_setprio(0);
     };
     if (c0 < c1) stage.put(bufs[0]);
     loads_done();

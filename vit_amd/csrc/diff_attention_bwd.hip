@@ -495,10 +495,11 @@ int64_t parts_floats(const DiffArgs& a, int np) {
 template <class T, int DP>
 hipError_t launch(const DiffArgs& a, const DiffGrads& g, float* ws, hipStream_t s) {
     constexpr int NP = pairs<T>(), OCC = sizeof(T) == 4 && DP > 32 ? 1 : 2;
-    // blocks of 32 that are staged between two barriers, measured with one / two:  dQ at 577 tokens (batch 16, 8 heads of
-    // 48) 104.7 / 94.7 us, at 4096 causal ones (2, 8 heads of 64, 4 key heads) 193 / 168, in f32 at 257 (4, 16 heads of 40)
-    // 80.6 / 81;  dK and dV 102.8 / 100.8, 454 / 542, 93 / 85
-    constexpr int NBQ = sizeof(T) == 4 ? 1 : 2, NBK = sizeof(T) == 4 ? 2 : 1;
+    // blocks of 32 that are staged between two barriers, measured with one / two.  dQ at 577 tokens (batch 16, 8 heads of 48)
+    // 70 / 81 us, at 197 (64, 12 of 32) 55 / 59: the smaller buffers leave room for a third workgroup on a CU;  at 4096
+    // causal ones (2, 8 heads of 64, 4 key heads) 195 / 192, at 1500 (2, 16 of 64) 119 / 115: there the registers do not.
+    // dK and dV 100 / 102, 75 / -, 280 / 319;  in f32 at 257 tokens (4, 16 heads of 40) 93 / 85.
+    constexpr int NBQ = sizeof(T) == 2 && DP == 64 ? 2 : 1, NBK = sizeof(T) == 4 ? 2 : 1;
     const int64_t bks = (int64_t)a.batch * a.kv_heads;
     const int64_t qt = row_tiles(a, kRowPairs), kt = key_tiles(a, NP), keys = (int64_t)a.batch * a.kv_heads * a.nk;
     const int splits = row_splits(a, NP);
