@@ -32,7 +32,7 @@ def main():
     def step():
         loss = crit(model(x), t)
         loss.backward()
-        torch.nn.utils.clip_grad_norm_(model.parameters(), 1.0)
+        vit_amd.clip_grad_norm_(model.parameters(), 1.0)
         opt.step()
         opt.zero_grad(set_to_none=True)
 
