@@ -484,3 +484,14 @@ def test_refusals():
                 dict(q=q[..., :12], k=k[..., :12], v=v[..., :24], lam=lam[..., :12].contiguous())):
         with pytest.raises(VitkError):
             vit_amd.diff_attention(**{**ok, **bad})
+
+
+@gpu
+def test_sizes_beyond_the_counters_are_refused():
+    q = torch.zeros(1, 1, 1, 2, 8, device="cuda", dtype=H16)
+    k = q.expand(1, 2 ** 32 + 8, 1, 2, 8)
+    v = torch.zeros(1, 1, 1, 16, device="cuda", dtype=H16).expand(1, 2 ** 32 + 8, 1, 16)
+    with pytest.raises(VitkError, match="too large"):
+        vit_amd.diff_attention(q, k, v, torch.zeros(4, 8, device="cuda"))
+    with pytest.raises(VitkError):                                             # fits the counter, not the kernels
+        vit_amd.diff_attention(q, k[:, :2 ** 28 + 1], v[:, :2 ** 28 + 1], torch.zeros(4, 8, device="cuda"))

@@ -278,3 +278,12 @@ def test_refusals():
     for t in (x.half(), x.double(), x.permute(0, 3, 1, 2), x[..., ::2], torch.ones(8, device="cuda")):
         with pytest.raises(VitkError):
             vit_amd.group_norm(t, 2)
+
+
+@gpu
+def test_sizes_beyond_the_counters_are_refused():
+    x = torch.empty(1, 2 ** 32 + 8, 1, device="cuda", dtype=torch.bfloat16)    # 8 GiB, not read
+    with pytest.raises(VitkError, match="too large"):
+        vit_amd.group_norm(x, 1)
+    with pytest.raises(VitkError):
+        vit_amd.group_norm(x[:, :2 ** 30 + 1], 1)

@@ -907,6 +907,7 @@ hipError_t forward(const T* x, const float* weight, const float* bias, T* y, flo
             const int R = threads / sl.wv, nv = (S + R - 1) / R;
             return by_act(act, [&](auto a) {
                 constexpr int A = decltype(a)::value;
+                if ((int64_t)B * (C / sl.W) > 0x7FFFFFFF) return hipErrorInvalidValue;
                 const dim3 grid(B * (C / sl.W)), block(threads);
                 if (threads == 1024) hipLaunchKernelGGL((gn_slab<T, V, A, 1024, kSlabMost>), grid, block, 0, s, x, weight, bias, y, mean, rstd, sl, eps);
                 else if (nv <= 4) hipLaunchKernelGGL((gn_slab<T, V, A, 512, 4>), grid, block, 0, s, x, weight, bias, y, mean, rstd, sl, eps);
@@ -936,6 +937,7 @@ hipError_t backward(const T* x, const float* weight, const float* bias, const T*
             const int R = threads / sl.wv, nv = (S + R - 1) / R;
             hipError_t e = by_act(act, [&](auto a) {
                 constexpr int A = decltype(a)::value;
+                if ((int64_t)B * (C / sl.W) > 0x7FFFFFFF) return hipErrorInvalidValue;
                 const dim3 grid(B * (C / sl.W)), block(512);
                 if (nv <= 4) hipLaunchKernelGGL((gn_slab_bwd<T, V, A, 512, 4>), grid, block, 0, s, x, dy, weight, bias, mean, rstd, dx, ws, sl);
                 else hipLaunchKernelGGL((gn_slab_bwd<T, V, A, 512, kSlabMost>), grid, block, 0, s, x, dy, weight, bias, mean, rstd, dx, ws, sl);

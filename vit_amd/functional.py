@@ -45,7 +45,8 @@ def diff_attention(q, k, v, lam, lambda_init=0.8, scale=None, key_lens=None, cau
     dimension: the fused projection's qkv [3, B, H, N, 2d] goes in as `qkv[i].view(B, H, N, 2, d).permute(0, 2, 1, 3, 4)`.
     lam f32 [4, H, d], or [4, d] for all heads; scale defaults to d ** -0.5 and must be positive.
     key_lens (int32 [B] on the device) hides the keys from key_lens[b] on: they are never read and get no gradient.  causal:
-    query t sees keys up to t + Nk - Nq (the last query all of them).  A row without a visible key gives 0 and no gradient.
+    query t sees keys up to t + Nk - Nq (the last query all of them); keys and values that only some queries see have to be
+    finite, since a probability of 0 still multiplies them.  A row without a visible key gives 0 and no gradient.
     Single query tokens against a long cache take a form that splits the keys.  Differentiable once in q, k, v and lam."""
     if scale is None:
         scale = q.shape[-1] ** -0.5

@@ -652,6 +652,8 @@ def _diff_sizes(q, k, v, lam, key_lens):
     for n, t in (("q", q), ("k", k), ("v", v), ("lam", lam), ("key_lens", key_lens)):
         if t is not None and (not t.is_cuda or t.get_device() != dev):
             raise _lib.VitkError(f"diff_attention: {n} is on {t.device}, q on {q.device}")
+    if max(B, nq, nk, H) > 0x7FFFFFFF:
+        raise _lib.VitkError(f"diff_attention: q {tuple(q.shape)}, k {tuple(k.shape)} are too large")
     if q.numel() and k.numel() and (q.stride(4) != 1 or k.stride(4) != 1 or v.stride(3) != 1):
         raise _lib.VitkError("diff_attention: the last dimension of q, k and v must be dense")
     return B, nq, nk, H, K, d, code
@@ -738,7 +740,10 @@ def _gn_sizes(x, num_groups, weight, bias, activation):
                 raise _lib.VitkError(f"group_norm: {n} has {t.numel()} elements, expected {C}")
             if t.device != x.device:
                 raise _lib.VitkError(f"group_norm: {n} is on {t.device}, x on {x.device}")
-    return B, (x.numel() // (B * C) if B * C else 0), C
+    S = x.numel() // (B * C) if B * C else 0
+    if max(B, S, C) > 0x7FFFFFFF:
+        raise _lib.VitkError(f"group_norm: {tuple(x.shape)} is too large")
+    return B, S, C
 
 
 def group_norm(x, num_groups, weight, bias, eps, activation="none", want_stats=False):
