@@ -121,7 +121,7 @@ struct Slice;
 template <>
 struct Slice<bf16_t> {
     bf16x8 v;
-    // the rounding to bf16 of a probability or of its gradient: 2^-9 relative, of terms that are then added in f32
+    // the rounding to bf16 of a probability or of its gradient: up to 2^-8 of it, of terms that are then added in f32
     __device__ __forceinline__ void take(const f32x16& s, int st) {
         const u32x4 pk = {pack_bf16(s[8 * st], s[8 * st + 1]), pack_bf16(s[8 * st + 2], s[8 * st + 3]),
                           pack_bf16(s[8 * st + 4], s[8 * st + 5]), pack_bf16(s[8 * st + 6], s[8 * st + 7])};

@@ -25,7 +25,9 @@ using namespace diff;
 
 namespace {
 
-// pairs of waves in a workgroup
+// Pairs of waves in a workgroup.  Few rows: as many as LDS has room for with two buffers of 32 keys each.  Many rows: four in f32
+// and at size 32, two else, measured with two / four: 197 tokens of 32 (64 x 12 heads) 37.4 / 37.2 us, 197 of 64 (64 x 6)
+// 40.6 / 43.5, 4096 causal ones of 64 151 / 161, f32 55 / 55.
 template <class T, int DP>
 constexpr int keys_pairs() { return row_bytes<T, 2 * DP>() == 512 ? 2 : 4; }
 
