@@ -154,6 +154,22 @@ def test_every_head_size(d, dtype):
     _run((70, 70, 95, 4, 2, d), dtype, backward=False)
 
 
+SPLIT = [                                                                       # the backward's parts, added by kernels of their own
+    ((2, 40, 1500, 4, 2, 40), dict(causal=True, lens=[1500, 700])),             # keys split, the second sample's in part
+    ((1, 600, 600, 2, 1, 48), dict(causal=True)),                               # rows and keys split
+    ((1, 1030, 1030, 4, 1, 64), dict(causal=True, shared=True)),
+    ((2, 700, 530, 3, 1, 16), dict(lens=[0, 530])),                             # an empty sample, a group of three
+    ((1, 5, 2570, 5, 1, 8), {}),
+]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [H16, F])
+@pytest.mark.parametrize("case,kw", SPLIT)
+def test_gradients_in_parts(case, kw, dtype):
+    _run(case, dtype, **kw)
+
+
 @gpu
 @pytest.mark.parametrize("dtype", [H16, F])
 def test_other_scales_and_weights(dtype):

@@ -8,8 +8,8 @@
 //     dw_h = - sum over the head's rows and keys of P_2 dA
 // Two kernels, so that nothing is added by atomics and results are reproducible: one walks the keys for 64 rows (dQ, and the
 // row's share of dw), one walks the rows for 128 keys (64 in f32: dK, dV; the rows of all query heads of a key head, so that
-// shared heads need no sum of their own).  Where that leaves CUs without work the rows are split too, and a third kernel adds
-// the parts.  dw is added from f32 probabilities and f32 accumulators, not from the rounded O_2.
+// shared heads need no sum of their own).  Where that leaves CUs without work the keys or rows are split too, and kernels of
+// their own add the parts.  dw is added from f32 probabilities and f32 accumulators, not from the rounded O_2.
 // As in the forward a pair of waves shares 32 rows or keys, one map each: dA is computed by both, everything else once, and
 // the registers that leaves allow two waves and more to a SIMD, which hide each other's waiting (one wave with both maps
 // took 2.3 times as long at 577 tokens of head size 48, most of it waiting).
@@ -44,7 +44,8 @@ __device__ __forceinline__ float dot(typename Op<T>::Chunk x, typename Op<T>::Ch
 // NP: pairs of waves in a workgroup, 32 rows each; OCC: waves to a SIMD that the registers have to allow
 template <class T, int DP, int NP, int NB, int OCC>
 __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_q(DiffArgs a, DiffGrads g, float* __restrict__ ws_d,
-                                                             float* __restrict__ ws_w, int tiles) {
+                                                             float* __restrict__ ws_w, float* __restrict__ parts, int tiles,
+                                                             int splits) {
     constexpr int kThreads = NP * 128, kBlock = NP * 32;
     constexpr int DV = 2 * DP;
     constexpr int RB = row_bytes<T, DV>();
@@ -62,7 +63,8 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_q(DiffArgs a, DiffGrad
     const int r = lane & 31, hh = lane >> 5;
     const int bks = a.batch * a.kv_heads;
     const int rest = quotient(blockIdx.x, a.by_bks), bk = blockIdx.x - rest * bks;
-    const int tile = a.causal ? tiles - 1 - rest : rest;
+    const int turn = rest / splits, split = rest - turn * splits;
+    const int tile = a.causal ? tiles - 1 - turn : turn;
     const int b = quotient(bk, a.by_kv_heads), kh = bk - b * a.kv_heads;
     const int nrows = a.nq * a.group;
     const int row0 = tile * kBlock + grp * 32, end = (tile + 1) * kBlock;
@@ -76,8 +78,13 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_q(DiffArgs a, DiffGrad
     const T* s_src = stage.row * s_step + (stage.second ? reinterpret_cast<const T*>(a.v) + b * a.vs[0] + kh * a.vs[2] + stage.col * PER
                                                         : reinterpret_cast<const T*>(a.k) + b * a.ks[0] + kh * a.ks[2] + stage.map * a.ks[3] + stage.e * PER);
     auto fetch = [&](int key0) { stage.fetch(key0, kmax, s_src, s_step, 0, [&](int key) { return s_src + (key - stage.row) * s_step; }); };
-    const int c1 = (kmax + KC - 1) / KC;
-    if (c1 > 0) fetch(0);
+    int c0 = 0, c1 = (kmax + KC - 1) / KC;
+    if (splits > 1) {                                                 // this workgroup's share of the keys
+        const int per = (c1 + splits - 1) / splits;
+        c0 = split * per;
+        c1 = c0 + per < c1 ? c0 + per : c1;
+    }
+    if (c0 < c1) fetch(c0 * KC);
 
     const int row = row0 + r;
     const RowPlace place = row_place(a, kh, row < nrows ? row : nrows - 1);
@@ -119,11 +126,11 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_q(DiffArgs a, DiffGrad
     float dw = 0.f;
     const float sc = a.scale * kLog2e;
 
-    if (c1 > 0) stage.put(bufs[0]);
+    if (c0 < c1) stage.put(bufs[0]);
     loads_done();
     __syncthreads();
     const float dd = map ? s_dot[grp][1][r] : fmaf(weight, s_dot[grp][1][r], s_dot[grp][0][r]);
-    if (row < nrows && hh == 0) ws_d[map * lmap + lrow] = dd;
+    if (row < nrows && hh == 0 && split == 0) ws_d[map * lmap + lrow] = dd;
     auto chunk = [&](int c, auto which) __attribute__((always_inline)) {                            // the buffer is known when compiled: no address arithmetic
         const char* kt = bufs[decltype(which)::value];
         const char* vt = kt + TILE;
@@ -160,7 +167,7 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_q(DiffArgs a, DiffGrad
         if (more) stage.put(bufs[decltype(which)::value ^ 1]);
         __syncthreads();
     };
-    for (int c = 0; c < c1; c += 2) {
+    for (int c = c0; c < c1; c += 2) {
         chunk(c, std::integral_constant<int, 0>{});
         if (c + 1 < c1) chunk(c + 1, std::integral_constant<int, 1>{});
     }
@@ -173,15 +180,20 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_q(DiffArgs a, DiffGrad
         const int first = tile * kBlock;
         float t = 0.f;
         for (int i = (h - first % a.group + a.group) % a.group; i < kBlock; i += a.group) t += s_dw[i];
-        ws_w[((int64_t)bk * tiles + tile) * a.group + h] = t;
+        ws_w[(((int64_t)bk * tiles + tile) * splits + split) * a.group + h] = t;
     }
+    // [split][sample, head, token][map][d]
+    float* part = splits > 1 ? parts + ((split * lmap + lrow) * 2 + map) * a.d : nullptr;
     T* out = reinterpret_cast<T*>(g.dq) + b * g.dqs[0] + place.tok * g.dqs[1] + place.head * g.dqs[2] + map * g.dqs[3];
     const float f = map == 0 ? inv * a.scale : -weight * inv * a.scale;
 #pragma unroll
     for (int e = 0; e < EB; ++e)
 #pragma unroll
-        for (int q = 0; q < 4; q += 2)
-            store_pair(out, e * 32 + 8 * q, hh, a.d, row < nrows, four(dq[e], q, f), four(dq[e], q + 1, f));
+        for (int q = 0; q < 4; q += 2) {
+            const f32x4 x = four(dq[e], q, f), y = four(dq[e], q + 1, f);
+            if (part) store_pair(part, e * 32 + 8 * q, hh, a.d, row < nrows, x, y);
+            else store_pair(out, e * 32 + 8 * q, hh, a.d, row < nrows, x, y);
+        }
 }
 
 // dK and dV of 32 NP keys.  What a row contributes beside its Q and dO is folded into the products' initial accumulators:
@@ -412,6 +424,22 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_kv(DiffArgs a, DiffGra
     }
 }
 
+// The key splits' dQ added, four columns of a row to a lane.
+template <class T>
+__global__ __launch_bounds__(256) void diff_bwd_q_join(DiffArgs a, DiffGrads g, const float* __restrict__ parts, int splits) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, rows = (int64_t)a.batch * a.heads * a.nq;
+    const int per = a.d / 2;                                          // lanes of a row
+    const int64_t row = i / per;
+    if (row >= rows) return;
+    const int col = (int)(i - row * per) * 4;
+    const float* p = parts + row * 2 * a.d + col;
+    f32x4 x = *reinterpret_cast<const f32x4*>(p);
+    for (int s = 1; s < splits; ++s) x = x + *reinterpret_cast<const f32x4*>(p + s * rows * 2 * a.d);
+    const int64_t bh = row / a.nq, tok = row - bh * a.nq, b = bh / a.heads, head = bh - b * a.heads;
+    const int map = col >= a.d;
+    store4(reinterpret_cast<T*>(g.dq) + b * g.dqs[0] + tok * g.dqs[1] + head * g.dqs[2] + map * g.dqs[3] + col - map * a.d, x);
+}
+
 // The row splits' dK and dV added, four columns of a key to a lane.
 template <class T>
 __global__ __launch_bounds__(256) void diff_bwd_join(DiffArgs a, DiffGrads g, const float* __restrict__ parts, int splits) {
@@ -479,22 +507,28 @@ constexpr int kRowPairs = 2;
 int64_t row_tiles(const DiffArgs& a, int np) { return ((int64_t)a.nq * a.group + 32 * np - 1) / (32 * np); }
 int64_t key_tiles(const DiffArgs& a, int np) { return ((int64_t)a.nk + 32 * np - 1) / (32 * np); }
 
-// Into how many parts the rows of a key tile are split: so many that there are two workgroups to a CU, where most CUs would
-// have none, or where the rows are long enough to pay for adding the parts (under a causal mask the first keys' workgroups
-// have twice the average work).  Measured with / without, the addition included: 10000 causal rows, 20 workgroups 66 / 621
-// us; 1800, 45: 31 / 95; 600, 80: 27 / 30; 8192, 256: 305 / 452;  1500 unmasked rows, 384 workgroups 183 / 183, 1200 causal
-// ones, 240: 64 / 55.
-int row_splits(const DiffArgs& a, int np) {
-    const int64_t blocks = (int64_t)a.batch * a.kv_heads * key_tiles(a, np), rows = (int64_t)a.nq * a.group;
-    if (blocks >= 128 && rows < 2048) return 1;
-    int64_t s = 511 / blocks + 1, most = rows / 256;
+// Into how many parts the rows of a key tile (or the keys of a row tile) are split: so many that there are two workgroups to
+// a CU, where most CUs would have none, or where they are long enough to pay for adding the parts (under a causal mask the
+// first keys' workgroups have twice the average work).  Measured with / without, the addition included, dK and dV: 10000
+// causal rows, 20 workgroups 66 / 621 us; 1800, 45: 31 / 95; 600, 80: 27 / 30; 8192, 256: 305 / 452;  1500 unmasked rows, 384
+// workgroups 183 / 183, 1200 causal ones, 240: 64 / 55.  dQ: 10000 causal rows on 2500 keys, 157 workgroups 40 / 67; one f32
+// token on 6614 keys, 6 workgroups: the whole step 141 / 993.
+int splits_of(int64_t blocks, int64_t length) {
+    if (blocks >= 128 && length < 2048) return 1;
+    int64_t s = 511 / blocks + 1, most = length / 256;
     s = s < most ? s : most;
-    return (int)(s < 1 ? 1 : s > 16 ? 16 : s);
+    return (int)(s < 1 ? 1 : s > 32 ? 32 : s);
 }
+int row_splits(const DiffArgs& a, int np) {
+    return splits_of((int64_t)a.batch * a.kv_heads * key_tiles(a, np), (int64_t)a.nq * a.group);
+}
+int key_splits(const DiffArgs& a) { return splits_of((int64_t)a.batch * a.kv_heads * row_tiles(a, kRowPairs), a.nk); }
 
+// f32 values of the parts, of one kernel after the other
 int64_t parts_floats(const DiffArgs& a, int np) {
-    const int s = row_splits(a, np);
-    return s > 1 ? (int64_t)s * a.batch * a.kv_heads * a.nk * 4 * a.d : 0;
+    const int64_t r = row_splits(a, np), k = key_splits(a);
+    const int64_t kv = r > 1 ? r * a.batch * a.kv_heads * a.nk * 4 * a.d : 0, q = k > 1 ? k * a.batch * a.heads * a.nq * 2 * a.d : 0;
+    return kv > q ? kv : q;
 }
 
 template <class T, int DP>
@@ -507,14 +541,21 @@ hipError_t launch(const DiffArgs& a, const DiffGrads& g, float* ws, hipStream_t 
     constexpr int NBQ = sizeof(T) == 2 && DP == 64 ? 2 : 1, NBK = sizeof(T) == 4 ? 2 : 1;
     const int64_t bks = (int64_t)a.batch * a.kv_heads;
     const int64_t qt = row_tiles(a, kRowPairs), kt = key_tiles(a, NP), keys = (int64_t)a.batch * a.kv_heads * a.nk;
-    const int splits = row_splits(a, NP);
-    if (bks * qt > 0x7FFFFFFF || bks * kt * splits > 0x7FFFFFFF || keys * a.d / 256 > 0x7FFFFFF0) return hipErrorInvalidValue;
+    const int splits = row_splits(a, NP), ksplits = key_splits(a);
+    const int64_t rows = (int64_t)a.batch * a.heads * a.nq;
+    if (bks * qt * ksplits > 0x7FFFFFFF || rows * a.d / 512 > 0x7FFFFFF0 || bks * kt * splits > 0x7FFFFFFF || keys * a.d / 256 > 0x7FFFFFF0) return hipErrorInvalidValue;
     float* parts = ws;
     float* ws_d = ws + parts_floats(a, NP);
     float* ws_w = ws_d + 2 * (int64_t)a.batch * a.heads * a.nq;
-    hipLaunchKernelGGL((diff_bwd_q<T, DP, kRowPairs, NBQ, OCC>), dim3((int)(bks * qt)), dim3(kRowPairs * 128), 0, s, a, g, ws_d, ws_w, (int)qt);
+    hipLaunchKernelGGL((diff_bwd_q<T, DP, kRowPairs, NBQ, OCC>), dim3((int)(bks * qt * ksplits)), dim3(kRowPairs * 128), 0, s, a, g, ws_d, ws_w,
+                       parts, (int)qt, ksplits);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
+    if (ksplits > 1) {
+        hipLaunchKernelGGL((diff_bwd_q_join<T>), dim3((int)((rows * (a.d / 2) + 255) / 256)), dim3(256), 0, s, a, g, parts, ksplits);
+        e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
     const dim3 grid((int)(bks * kt * splits)), block(NP * 128);
     if (a.group == 1) hipLaunchKernelGGL((diff_bwd_kv<T, DP, true, NP, NBK, OCC>), grid, block, 0, s, a, g, ws_d, parts, splits);
     else hipLaunchKernelGGL((diff_bwd_kv<T, DP, false, NP, NBK, OCC>), grid, block, 0, s, a, g, ws_d, parts, splits);
@@ -526,7 +567,7 @@ hipError_t launch(const DiffArgs& a, const DiffGrads& g, float* ws, hipStream_t 
         if (e != hipSuccess) return e;
     }
     if (!g.dlam) return hipSuccess;
-    hipLaunchKernelGGL(diff_bwd_lam, dim3(a.lam_heads), dim3(256), 0, s, a, ws_w, (int)qt, g.dlam);
+    hipLaunchKernelGGL(diff_bwd_lam, dim3(a.lam_heads), dim3(256), 0, s, a, ws_w, (int)qt * ksplits, g.dlam);
     return hipGetLastError();
 }
 
@@ -535,7 +576,7 @@ hipError_t launch(const DiffArgs& a, const DiffGrads& g, float* ws, hipStream_t 
 // f32 values of scratch of the backward
 int64_t diff_attention_bwd_workspace(const DiffArgs& a, bool bf16) {
     const int np = bf16 ? pairs<bf16_t>() : pairs<float>();
-    return parts_floats(a, np) + 2 * (int64_t)a.batch * a.heads * a.nq + (int64_t)a.batch * a.heads * row_tiles(a, kRowPairs);
+    return parts_floats(a, np) + 2 * (int64_t)a.batch * a.heads * a.nq + (int64_t)a.batch * a.heads * row_tiles(a, kRowPairs) * key_splits(a);
 }
 
 hipError_t launch_diff_attention_backward(const DiffArgs& a, const DiffGrads& g, float* ws, bool bf16, hipStream_t s) {
