@@ -4,7 +4,7 @@ Each function checks device/dtype/contiguity, passes raw device pointers and
 the current HIP stream to the matching `vitk_*` entry point (include/vitk.h)
 and raises on any non-zero return.  torch is used for memory and streams only.
 """
-import array
+import struct
 
 import torch
 
@@ -825,16 +825,18 @@ class GradList:
             dense = all(map(torch.Tensor.is_contiguous, tensors)) or all(map(_dense, tensors))
         except RuntimeError:
             dense = False
-        kind = list(map(_DTYPE_CODES.get, map(torch.Tensor.dtype.__get__, tensors)))
-        if not dense or dev < 0 or None in kind or set(map(torch.Tensor.get_device, tensors)) != {dev}:
+        types = list(map(torch.Tensor.dtype.__get__, tensors))
+        if not dense or dev < 0 or not set(types) <= _DTYPE_CODES.keys() or set(map(torch.Tensor.get_device, tensors)) != {dev}:
             for t in tensors:
                 if t.layout is not torch.strided or t.dtype not in _DTYPE_CODES or t.get_device() != dev or dev < 0 or not _dense(t):
                     self._refuse(t, tensors[0])
+            raise _lib.VitkError("gradients must have memory of their own")
         n = self.n = len(tensors)
-        # array.array copies a list of ints several times faster than a ctypes array does
-        self._held = (array.array("Q", addr), array.array("q", map(torch.Tensor.numel, tensors)), array.array("i", kind))
-        self.addr, self.size, self.kind = (a.buffer_info()[0] for a in self._held)
-        self.empty = not any(self._held[1])
+        size = list(map(torch.Tensor.numel, tensors))
+        kind = [_DTYPE_CODES[types[0]]] * n if types.count(types[0]) == n else [_DTYPE_CODES[t] for t in types]
+        # packed: a list of ints is copied several times faster than by a ctypes array
+        self.addr, self.size, self.kind = struct.pack(f"{n}Q", *addr), struct.pack(f"{n}q", *size), struct.pack(f"{n}i", *kind)
+        self.empty = not any(size)
         self.device = tensors[0].device
 
     @staticmethod
