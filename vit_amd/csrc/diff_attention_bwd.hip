@@ -196,6 +196,48 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_q(DiffArgs a, DiffGrad
         }
 }
 
+// dlam of one lam head from the dQ workgroups' shares of dw: dlam_0 = dw e_1 lam_1, dlam_1 = dw e_1 lam_0, and the second
+// pair with -e_2; a lam that all heads share collects all of them.  By a workgroup of NT threads, red: NT doubles.
+template <int NT>
+__device__ __forceinline__ void lam_gradient(const DiffArgs& a, const float* __restrict__ ws_w, int tiles, float* __restrict__ dlam,
+                                             int lh, double* red) {
+    const int tid = threadIdx.x;
+    const int64_t per = (int64_t)tiles * a.group, total = (int64_t)a.batch * a.kv_heads * per;
+    double t = 0.0;
+    if (a.lam_heads == 1) {
+        for (int64_t i = tid; i < total; i += NT) t += ws_w[i];
+    } else {
+        const int kh = lh / a.group, h = lh - kh * a.group;
+        for (int64_t i = tid; i < (int64_t)a.batch * tiles; i += NT) {
+            const int64_t b = i / tiles, tl = i - b * tiles;
+            t += ws_w[((b * a.kv_heads + kh) * tiles + tl) * a.group + h];
+        }
+    }
+    red[tid] = t;
+    __syncthreads();
+#pragma unroll
+    for (int o = NT / 2; o > 0; o >>= 1) {
+        if (tid < o) red[tid] += red[tid + o];
+        __syncthreads();
+    }
+    if (tid >= 64) return;
+    const float dw = (float)red[0];
+    const int64_t vs = (int64_t)a.lam_heads * a.d, at = (int64_t)lh * a.d;
+    const float* p = a.lam + at;
+    float s1 = 0.f, s2 = 0.f;
+    for (int e = tid; e < a.d; e += 64) {
+        s1 = fmaf(p[e], p[vs + e], s1);
+        s2 = fmaf(p[2 * vs + e], p[3 * vs + e], s2);
+    }
+    const float f1 = dw * expf(wave_sum(s1)), f2 = -dw * expf(wave_sum(s2));
+    for (int e = tid; e < a.d; e += 64) {
+        dlam[at + e] = f1 * p[vs + e];
+        dlam[vs + at + e] = f1 * p[e];
+        dlam[2 * vs + at + e] = f2 * p[3 * vs + e];
+        dlam[3 * vs + at + e] = f2 * p[2 * vs + e];
+    }
+}
+
 // dK and dV of 32 NP keys.  What a row contributes beside its Q and dO is folded into the products' initial accumulators:
 //     S_m starts at -lse_m / (scale log2 e), so that P_m = exp2(scale log2(e) S_m);  dA starts at -D_m.
 // In f32 it starts at the reference point alone and 1 / l_m is multiplied on: lse is the larger number, and its rounding
@@ -203,7 +245,8 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_q(DiffArgs a, DiffGrad
 // ONE: one query head to a key head, so that w is the workgroup's and can wait until the end (else the rows bring theirs).
 template <class T, int DP, bool ONE, int NP, int NB, int OCC>
 __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_kv(DiffArgs a, DiffGrads g, const float* __restrict__ ws_d,
-                                                             float* __restrict__ parts, int splits) {
+                                                             float* __restrict__ parts, int splits,
+                                                             const float* __restrict__ ws_w, int row_tiles, unsigned blocks) {
     constexpr int kThreads = NP * 128, kBlock = NP * 32;
     constexpr int DV = 2 * DP;
     constexpr int RB = row_bytes<T, DV>();
@@ -219,6 +262,13 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_kv(DiffArgs a, DiffGra
     __shared__ __align__(16) float s_row[2][NS][RC];                  // -lse_1 / sc, -lse_2 / sc, -D_1, -D_2, 1 / l_1, 1 / l_2, w
     __shared__ __align__(16) int s_lim[2][RC];
 
+    // The last workgroups add up the learned weight's gradient from the shares that the dQ kernel has left: a few sums, not
+    // worth a launch
+    static_assert(kThreads * 8 <= 2 * BUF, "the sums fit the buffers");
+    if (blockIdx.x >= blocks) {
+        lam_gradient<kThreads>(a, ws_w, row_tiles, g.dlam, blockIdx.x - blocks, reinterpret_cast<double*>(bufs[0]));
+        return;
+    }
     arguments(a);
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), map = wave & 1, grp = wave >> 1;
@@ -457,46 +507,6 @@ __global__ __launch_bounds__(256) void diff_bwd_join(DiffArgs a, DiffGrads g, co
     store4(to, x);
 }
 
-// dlam of one lam head from the workgroups' shares of dw: dlam_0 = dw e_1 lam_1, dlam_1 = dw e_1 lam_0, and the second
-// pair with -e_2; a lam that all heads share collects all of them.
-__global__ __launch_bounds__(256) void diff_bwd_lam(DiffArgs a, const float* __restrict__ ws_w, int tiles, float* __restrict__ dlam) {
-    __shared__ double red[256];
-    const int lh = blockIdx.x, tid = threadIdx.x;
-    const int64_t per = (int64_t)tiles * a.group, total = (int64_t)a.batch * a.kv_heads * per;
-    double t = 0.0;
-    if (a.lam_heads == 1) {
-        for (int64_t i = tid; i < total; i += 256) t += ws_w[i];
-    } else {
-        const int kh = lh / a.group, h = lh - kh * a.group;
-        for (int64_t i = tid; i < (int64_t)a.batch * tiles; i += 256) {
-            const int64_t b = i / tiles, tl = i - b * tiles;
-            t += ws_w[((b * a.kv_heads + kh) * tiles + tl) * a.group + h];
-        }
-    }
-    red[tid] = t;
-    __syncthreads();
-    for (int o = 128; o > 0; o >>= 1) {
-        if (tid < o) red[tid] += red[tid + o];
-        __syncthreads();
-    }
-    if (tid >= 64) return;
-    const float dw = (float)red[0];
-    const int64_t vs = (int64_t)a.lam_heads * a.d, at = (int64_t)lh * a.d;
-    const float* p = a.lam + at;
-    float s1 = 0.f, s2 = 0.f;
-    for (int e = tid; e < a.d; e += 64) {
-        s1 = fmaf(p[e], p[vs + e], s1);
-        s2 = fmaf(p[2 * vs + e], p[3 * vs + e], s2);
-    }
-    const float f1 = dw * expf(wave_sum(s1)), f2 = -dw * expf(wave_sum(s2));
-    for (int e = tid; e < a.d; e += 64) {
-        dlam[at + e] = f1 * p[vs + e];
-        dlam[vs + at + e] = f1 * p[e];
-        dlam[2 * vs + at + e] = f2 * p[3 * vs + e];
-        dlam[3 * vs + at + e] = f2 * p[2 * vs + e];
-    }
-}
-
 // Pairs of a workgroup.  dK and dV: four share the staged tiles in bf16 (with two 577 tokens of size 48 take 95 instead of 100
 // us, 1500 of 64 189 instead of 172); in f32 a lane holds twice the bytes, and two pairs leave it all 512 registers.  dQ: two,
 // so that a CU holds several workgroups, whose prologues (Q, dO, O) and loops overlap (85 against 101 us, 117 against 131).
@@ -543,7 +553,7 @@ hipError_t launch(const DiffArgs& a, const DiffGrads& g, float* ws, hipStream_t 
     const int64_t qt = row_tiles(a, kRowPairs), kt = key_tiles(a, NP), keys = (int64_t)a.batch * a.kv_heads * a.nk;
     const int splits = row_splits(a, NP), ksplits = key_splits(a);
     const int64_t rows = (int64_t)a.batch * a.heads * a.nq;
-    if (bks * qt * ksplits > 0x7FFFFFFF || rows * a.d / 512 > 0x7FFFFFF0 || bks * kt * splits > 0x7FFFFFFF || keys * a.d / 256 > 0x7FFFFFF0) return hipErrorInvalidValue;
+    if (bks * qt * ksplits > 0x7FFFFFFF || rows * a.d / 512 > 0x7FFFFFF0 || bks * kt * splits + a.lam_heads > 0x7FFFFFFF || keys * a.d / 256 > 0x7FFFFFF0) return hipErrorInvalidValue;
     float* parts = ws;
     float* ws_d = ws + parts_floats(a, NP);
     float* ws_w = ws_d + 2 * (int64_t)a.batch * a.heads * a.nq;
@@ -556,9 +566,10 @@ hipError_t launch(const DiffArgs& a, const DiffGrads& g, float* ws, hipStream_t 
         e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    const dim3 grid((int)(bks * kt * splits)), block(NP * 128);
-    if (a.group == 1) hipLaunchKernelGGL((diff_bwd_kv<T, DP, true, NP, NBK, OCC>), grid, block, 0, s, a, g, ws_d, parts, splits);
-    else hipLaunchKernelGGL((diff_bwd_kv<T, DP, false, NP, NBK, OCC>), grid, block, 0, s, a, g, ws_d, parts, splits);
+    const int blocks = (int)(bks * kt * splits);
+    const dim3 grid(blocks + (g.dlam ? a.lam_heads : 0)), block(NP * 128);
+    if (a.group == 1) hipLaunchKernelGGL((diff_bwd_kv<T, DP, true, NP, NBK, OCC>), grid, block, 0, s, a, g, ws_d, parts, splits, ws_w, (int)qt * ksplits, blocks);
+    else hipLaunchKernelGGL((diff_bwd_kv<T, DP, false, NP, NBK, OCC>), grid, block, 0, s, a, g, ws_d, parts, splits, ws_w, (int)qt * ksplits, blocks);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
     if (splits > 1) {
@@ -566,9 +577,7 @@ hipError_t launch(const DiffArgs& a, const DiffGrads& g, float* ws, hipStream_t 
         e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    if (!g.dlam) return hipSuccess;
-    hipLaunchKernelGGL(diff_bwd_lam, dim3(a.lam_heads), dim3(256), 0, s, a, ws_w, (int)qt * ksplits, g.dlam);
-    return hipGetLastError();
+    return hipSuccess;
 }
 
 }  // namespace
