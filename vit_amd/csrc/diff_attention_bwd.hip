@@ -255,11 +255,11 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_kv(DiffArgs a, DiffGra
     constexpr int DB = DV / 32, EB = (DP + 31) / 32;
     constexpr int RC = 32 * NB, TILE = RC * RB;                       // RC: rows of a chunk
     constexpr bool APART = sizeof(T) == 4;                            // 1 / l apart from the exponent
-    constexpr int NS = 4 + (APART ? 2 : ONE ? 0 : 1);
+    constexpr int NS = 4 + (APART ? 2 : 0) + (ONE ? 0 : 1);
     typedef typename Op<T>::Chunk Chunk;
     constexpr int BUF = 2 * TILE > NP * DB * 2048 ? 2 * TILE : NP * DB * 2048;              // DB sums of a pair fit
     __shared__ __align__(16) char bufs[2][BUF];                       // Q of both maps, dO
-    __shared__ __align__(16) float s_row[2][NS][RC];                  // -lse_1 / sc, -lse_2 / sc, -D_1, -D_2, in f32 1 / l_1, 1 / l_2, else w
+    __shared__ __align__(16) float s_row[2][NS][RC];                  // -lse_1 / sc, -lse_2 / sc, -D_1, -D_2, 1 / l_1, 1 / l_2, w
     __shared__ __align__(16) int s_lim[2][RC];
 
     // The last workgroups add up the learned weight's gradient from the shares that the dQ kernel has left: a few sums, not
@@ -312,15 +312,6 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_kv(DiffArgs a, DiffGra
     const int role = tid / RC, s_at = tid % RC;                       // 0, 1: -lse of a map;  2, 3: -D of a map
     const float* s_from = role < 2 ? g.stats + role * lmap : ws_d + (role - 2) * lmap;
     float held0 = 0.f, held1 = 0.f, held_w = 0.f;
-    // w of the rows' heads belongs to P_2: in bf16 its logarithm goes into lse_2, unless one of the group's is negative; then it is
-    // read and multiplied on block by block (4096 causal tokens, two heads to a key head: 286 instead of 276 us; a loop of
-    // its own for each way spills more registers, 288)
-    bool in_lse = !ONE && !APART;
-    if (in_lse) {
-        bool other = false;
-        for (int h = lane; h < a.group; h += 64) other |= !(g.weight[kh * a.group + h] >= 0.f);
-        in_lse = !__any(other);
-    }
     auto fetch = [&](int c) {
         stage.fetch(c * RC, nrows, s_src, s_tok, s_shift, addr);
         const int row = c * RC + s_at;
@@ -337,13 +328,11 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_kv(DiffArgs a, DiffGra
         if (role >= 4) return;
         const int row = c * RC + s_at;
         const bool on = row < nrows;                                  // a row past the last one: P = 0
-        const bool second_map = !ONE && role == 1;
         float x = role < 2 ? -__builtin_inff() : 0.f;
-        if (on) x = role >= 2 ? -held0 : APART ? -held0 * rsc
-                  : (__builtin_amdgcn_logf(held1) - held0 + (second_map && in_lse ? __builtin_amdgcn_logf(held_w) : 0.f)) * rsc;
+        if (on) x = role >= 2 ? -held0 : APART ? -held0 * rsc : (__builtin_amdgcn_logf(held1) - held0) * rsc;
         s_row[k][role][s_at] = x;
-        if (APART && role < 2) s_row[k][4 + role][s_at] = on ? (second_map ? held1 * held_w : held1) : 0.f;
-        if (!APART && second_map && !in_lse) s_row[k][NS - 1][s_at] = on ? held_w : 0.f;
+        if (APART && role < 2) s_row[k][4 + role][s_at] = on ? held1 : 0.f;
+        if (!ONE && role == 1) s_row[k][NS - 1][s_at] = on ? held_w : 0.f;
         if (role == 0) s_lim[k][s_at] = on ? key_limit(a, len, ONE ? row : row_place(a, kh, row).tok) : 0;
     };
     if (first < c1) fetch(first);
@@ -409,8 +398,8 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_kv(DiffArgs a, DiffGra
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i] * sc);
             if constexpr (APART) s = s * rows16(4 + map);
-            if constexpr (!ONE && !APART) {
-                if (map == 1 && !in_lse) s = s * rows16(NS - 1);
+            if constexpr (!ONE) {
+                if (map == 1) s = s * rows16(NS - 1);
             }
 #pragma unroll
             for (int st = 0; st < 2; ++st) {
