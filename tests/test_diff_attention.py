@@ -175,6 +175,8 @@ def test_gradients_in_parts(case, kw, dtype):
 def test_other_scales_and_weights(dtype):
     _run((2, 40, 60, 2, 2, 32), dtype, scale=0.02, lambda_init=0.0)
     _run((2, 40, 60, 2, 2, 32), dtype, scale=1.5, lambda_init=-3.0)
+    _run((2, 40, 60, 6, 2, 48), dtype, lambda_init=-3.0)                        # negative and shared
+    _run((2, 40, 60, 6, 2, 64), dtype, lambda_init=-0.3)                        # of both signs in a group
 
 
 @gpu
