@@ -160,6 +160,7 @@ SPLIT = [                                                                       
     ((1, 1030, 1030, 4, 1, 64), dict(causal=True, shared=True)),
     ((2, 700, 530, 3, 1, 16), dict(lens=[0, 530])),                             # an empty sample, a group of three
     ((1, 5, 2570, 5, 1, 8), {}),
+    ((1, 1100, 1050, 9, 9, 24), dict(causal=True)),                             # f32 in parts, bf16 not
 ]
 
 

@@ -408,13 +408,14 @@ struct Plan {
 };
 
 // Which form, and into how many workgroups.  At most 32 rows to a key head, or at most one block of 32 rows to each of the
-// 256 CUs: the pairs share the rows and split the keys.  Measured, keys split / not: 64 rows, 2048 keys, 128 key heads of
-// size 64 (256 blocks) 50 / 105 us, 256 heads (512 blocks) 105 / 108; 577 rows and keys, 16 heads of 64 (304) 29.2 / 27.4.
+// 256 CUs (two in f32, whose products take eight times as long): the pairs share the rows and split the keys.  Measured, keys split / not: 64 rows, 2048 keys, 128 key heads of
+// size 64 (256 blocks) 50 / 105 us, 256 heads (512 blocks) 105 / 108; 577 rows and keys, 16 heads of 64 (304) 29.2 / 27.4;  in f32
+// 577 tokens, 24 heads of 64 (456) 101 / 133, 257, 64 of 64 (576) 84 / 72.
 template <class T, int DP>
 Plan plan(const DiffArgs& a) {
     const int64_t nrows = (int64_t)a.nq * a.group, bks = (int64_t)a.batch * a.kv_heads;
     Plan p;
-    p.keys = nrows <= 32 || bks * ((nrows + 31) / 32) <= 256;
+    p.keys = nrows <= 32 || bks * ((nrows + 31) / 32) <= (sizeof(T) == 4 ? 512 : 256);
     constexpr int R = 32 * rows_pairs<T, DP>();
     p.tiles = (int)(p.keys ? (nrows + 31) / 32 : (nrows + R - 1) / R);
     p.splits = 1;

@@ -522,21 +522,22 @@ int64_t key_tiles(const DiffArgs& a, int np) { return ((int64_t)a.nk + 32 * np -
 // first keys' workgroups have twice the average work).  Measured with / without, the addition included, dK and dV: 10000
 // causal rows, 20 workgroups 66 / 621 us; 1800, 45: 31 / 95; 600, 80: 27 / 30; 8192, 256: 305 / 452;  1500 unmasked rows, 384
 // workgroups 183 / 183, 1200 causal ones, 240: 64 / 55.  dQ: 10000 causal rows on 2500 keys, 157 workgroups 40 / 67; one f32
-// token on 6614 keys, 6 workgroups: the whole step 141 / 993.
-int splits_of(int64_t blocks, int64_t length) {
-    if (blocks >= 128 && length < 2048) return 1;
+// token on 6614 keys, 6 workgroups: the whole step 141 / 993.  f32 takes eight times as long for the same rows and splits earlier (1200 causal rows and
+// keys, 152 workgroups: the whole step 302 / 578).
+int splits_of(int64_t blocks, int64_t length, bool bf16) {
+    if (blocks >= 128 && length < (bf16 ? 2048 : 1024)) return 1;
     int64_t s = 511 / blocks + 1, most = length / 256;
     s = s < most ? s : most;
     return (int)(s < 1 ? 1 : s > 32 ? 32 : s);
 }
-int row_splits(const DiffArgs& a, int np) {
-    return splits_of((int64_t)a.batch * a.kv_heads * key_tiles(a, np), (int64_t)a.nq * a.group);
+int row_splits(const DiffArgs& a, int np, bool bf16) {
+    return splits_of((int64_t)a.batch * a.kv_heads * key_tiles(a, np), (int64_t)a.nq * a.group, bf16);
 }
-int key_splits(const DiffArgs& a) { return splits_of((int64_t)a.batch * a.kv_heads * row_tiles(a, kRowPairs), a.nk); }
+int key_splits(const DiffArgs& a, bool bf16) { return splits_of((int64_t)a.batch * a.kv_heads * row_tiles(a, kRowPairs), a.nk, bf16); }
 
 // f32 values of the parts, of one kernel after the other
-int64_t parts_floats(const DiffArgs& a, int np) {
-    const int64_t r = row_splits(a, np), k = key_splits(a);
+int64_t parts_floats(const DiffArgs& a, int np, bool bf16) {
+    const int64_t r = row_splits(a, np, bf16), k = key_splits(a, bf16);
     const int64_t kv = r > 1 ? r * a.batch * a.kv_heads * a.nk * 4 * a.d : 0, q = k > 1 ? k * a.batch * a.heads * a.nq * 2 * a.d : 0;
     return kv > q ? kv : q;
 }
@@ -551,11 +552,11 @@ hipError_t launch(const DiffArgs& a, const DiffGrads& g, float* ws, hipStream_t 
     constexpr int NBQ = sizeof(T) == 2 && DP == 64 ? 2 : 1, NBK = sizeof(T) == 4 ? 2 : 1;
     const int64_t bks = (int64_t)a.batch * a.kv_heads;
     const int64_t qt = row_tiles(a, kRowPairs), kt = key_tiles(a, NP), keys = (int64_t)a.batch * a.kv_heads * a.nk;
-    const int splits = row_splits(a, NP), ksplits = key_splits(a);
+    const int splits = row_splits(a, NP, sizeof(T) == 2), ksplits = key_splits(a, sizeof(T) == 2);
     const int64_t rows = (int64_t)a.batch * a.heads * a.nq;
     if (bks * qt * ksplits > 0x7FFFFFFF || rows * a.d / 512 > 0x7FFFFFF0 || bks * kt * splits + a.lam_heads > 0x7FFFFFFF || keys * a.d / 256 > 0x7FFFFFF0) return hipErrorInvalidValue;
     float* parts = ws;
-    float* ws_d = ws + parts_floats(a, NP);
+    float* ws_d = ws + parts_floats(a, NP, sizeof(T) == 2);
     float* ws_w = ws_d + 2 * (int64_t)a.batch * a.heads * a.nq;
     hipLaunchKernelGGL((diff_bwd_q<T, DP, kRowPairs, NBQ, OCC>), dim3((int)(bks * qt * ksplits)), dim3(kRowPairs * 128), 0, s, a, g, ws_d, ws_w,
                        parts, (int)qt, ksplits);
@@ -585,7 +586,7 @@ hipError_t launch(const DiffArgs& a, const DiffGrads& g, float* ws, hipStream_t 
 // f32 values of scratch of the backward
 int64_t diff_attention_bwd_workspace(const DiffArgs& a, bool bf16) {
     const int np = bf16 ? pairs<bf16_t>() : pairs<float>();
-    return parts_floats(a, np) + 2 * (int64_t)a.batch * a.heads * a.nq + (int64_t)a.batch * a.heads * row_tiles(a, kRowPairs) * key_splits(a);
+    return parts_floats(a, np, bf16) + 2 * (int64_t)a.batch * a.heads * a.nq + (int64_t)a.batch * a.heads * row_tiles(a, kRowPairs) * key_splits(a, bf16);
 }
 
 hipError_t launch_diff_attention_backward(const DiffArgs& a, const DiffGrads& g, float* ws, bool bf16, hipStream_t s) {
