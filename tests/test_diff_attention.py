@@ -343,7 +343,7 @@ def test_sizes_with_nothing_to_attend_to():
 
 
 @gpu
-@pytest.mark.parametrize("case", [(3, 1, 3000, 8, 2, 64), (16, 200, 200, 4, 4, 48)])
+@pytest.mark.parametrize("case", [(3, 1, 3000, 8, 2, 64), (16, 200, 200, 4, 4, 48), (1, 600, 600, 2, 1, 48)])
 def test_streams_capture_and_repeats(case):
     q, k, v, lam, do, _ = (None if t is None else t.cuda() for t in _inputs(*case, H16))
     lens = torch.full((case[0],), case[2], dtype=torch.int32, device="cuda")

@@ -38,6 +38,14 @@ __device__ __forceinline__ float lanes_sum(float v, int L) {
     return v;
 }
 
+__device__ __forceinline__ void lanes_sum2(float& a, float& b, int L) {
+    for (int o = L >> 1; o > 0; o >>= 1) {
+        const float x = __shfl_xor(a, o, 64), y = __shfl_xor(b, o, 64);
+        a += x;
+        b += y;
+    }
+}
+
 // f(group, lane of it) for ng groups by the workgroup's threads, L neighbouring lanes to a group (power of two up to 64);
 // every lane of a wave makes every call, with group < ng or not
 template <int NT, class F>
@@ -60,6 +68,16 @@ struct Raw<bf16_t, 8> {
             v[2 * j + 1] = bf16_hi(r[j]);
         }
     }
+    __device__ __forceinline__ float plus(float t) const {             // t + the values, two to an instruction
+        typedef bf16_t bf16x2 __attribute__((ext_vector_type(2)));
+        const bf16x2 one = {(bf16_t)1.f, (bf16_t)1.f};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const unsigned u = r[j];
+            t = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, u), one, t, false);
+        }
+        return t;
+    }
     __device__ __forceinline__ static void store(bf16_t* p, const float (&v)[8]) {
         *reinterpret_cast<u32x4*>(p) = u32x4{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])};
     }
@@ -81,6 +99,7 @@ struct Raw<float, 4> {
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = r[j];
     }
+    __device__ __forceinline__ float plus(float t) const { return t + ((r[0] + r[1]) + (r[2] + r[3])); }
     __device__ __forceinline__ static void store(float* p, const float (&v)[4]) {
         *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
     }
@@ -589,20 +608,37 @@ __device__ __forceinline__ void slab_sums(const Slab& q, int R, float v1, float 
     by_groups<NT>(q.W / q.Cg, q.L, [&](int g, int l) {
         const bool on = g < q.W / q.Cg;
         float t1 = 0.f, t2 = 0.f;
-        if (on)
-            for (int i = l; i < R * gv; i += q.L) {
-                const int r = i / gv, at = r * q.wv + g * gv + i - r * gv;
-                t1 += s_in[0][at];
-                t2 += s_in[1][at];
-            }
-        t1 = lanes_sum(t1, q.L);
-        t2 = lanes_sum(t2, q.L);
+        if (on) {
+            // lanes over a row's threads first, over the rows with what is left of them
+            int sh = 0;
+            while ((1 << sh) < q.L && (1 << sh) < gv) ++sh;
+            for (int r = l >> sh; r < R; r += q.L >> sh)
+                for (int c = l & ((1 << sh) - 1); c < gv; c += 1 << sh) {
+                    const int at = r * q.wv + g * gv + c;
+                    t1 += s_in[0][at];
+                    t2 += s_in[1][at];
+                }
+        }
+        lanes_sum2(t1, t2, q.L);
         if (on && l == 0) {
             s_out[0][g] = t1;
             s_out[1][g] = t2;
         }
     });
     __syncthreads();
+}
+
+// V neighbouring channels' weights and biases, all loads at once (a column of the slab is one for every thread)
+template <int V>
+__device__ __forceinline__ void load_params(const float* __restrict__ weight, const float* __restrict__ bias, int c, float (&w)[V], float (&sh)[V]) {
+    if (weight) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) w[j] = weight[c + j];
+    }
+    if (bias) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) sh[j] = bias[c + j];
+    }
 }
 
 template <class T, int V, int ACT, int NT, int NV>
@@ -625,18 +661,16 @@ __global__ __launch_bounds__(NT) void gn_slab(const T* __restrict__ x, const flo
     float w[V], sh[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        w[j] = live && weight ? weight[c0 + col * V + j] : 1.f;
-        sh[j] = live && bias ? bias[c0 + col * V + j] : 0.f;
+        w[j] = 1.f;
+        sh[j] = 0.f;
     }
+    load_params<V>(weight, bias, c0 + col * V, w, sh);
     const float inv_n = 1.0f / ((float)q.S * (float)q.Cg);
     float t = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
         if (live && row + i * R < q.S) {
-            float v[V];
-            r[i].get(v);
-#pragma unroll
-            for (int j = 0; j < V; ++j) t += v[j];
+            t = r[i].plus(t);
         }
     slab_sums<NT, V>(q, R, t, 0.f, s_in, s_out);
     const float mu0 = s_out[0][gl] * inv_n;
@@ -705,10 +739,10 @@ __global__ __launch_bounds__(NT) void gn_slab_bwd(const T* __restrict__ x, const
     const float mu = live ? mean[b * q.G + c0 / q.Cg + gl] : 0.f, rs = live ? rstd[b * q.G + c0 / q.Cg + gl] : 0.f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        w[j] = live && weight ? weight[c0 + col * V + j] : 1.f;
-        sh[j] = live && bias ? bias[c0 + col * V + j] : 0.f;
-        a1[j] = a2[j] = 0.f;
+        w[j] = 1.f;
+        sh[j] = a1[j] = a2[j] = 0.f;
     }
+    load_params<V>(weight, bias, c0 + col * V, w, sh);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
         if (live && row + i * R < q.S) {
