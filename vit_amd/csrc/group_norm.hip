@@ -135,6 +135,38 @@ __device__ __forceinline__ float dact_of(float z) {
     return 1.f;
 }
 
+// V neighbouring channels' weights and biases, all loads at once (1 and 0 where there are none)
+template <int V>
+__device__ __forceinline__ void load_params(const float* __restrict__ weight, const float* __restrict__ bias, int c, float (&w)[V], float (&sh)[V]) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        w[j] = 1.f;
+        sh[j] = 0.f;
+    }
+    if (weight) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) w[j] = weight[c + j];
+    }
+    if (bias) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) sh[j] = bias[c + j];
+    }
+}
+
+// f(j, group) for V neighbouring channels from c on
+template <int V, class F>
+__device__ __forceinline__ void groups_of(int c, int Cg, F&& f) {
+    int g = c / Cg, left = (g + 1) * Cg - c;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        f(j, g);
+        if (--left == 0) {
+            ++g;
+            left = Cg;
+        }
+    }
+}
+
 struct Geometry {
     int S, C, G, Cg;          // pixels, channels, groups, channels of a group
     int cv;                   // lanes side by side in a slab = slab channels / V
@@ -302,10 +334,12 @@ __global__ __launch_bounds__(kT) void gn_apply(const T* __restrict__ x, const Mo
     const bool live = row < rows && col * V < wc;
     constexpr int U = 4;
     Raw<T, V> ahead[U];
+    float a[V], sh[V];
     if (live) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (s0 + row + u * rows < s1) ahead[u].load(x + base + (int64_t)(s0 + row + u * rows) * q.C);
+        load_params<V>(weight, bias, c0 + col * V, a, sh);
     }
     merge_groups(part, q, V, b, g0, g1, eps, s_mean, s_rstd);
     __syncthreads();
@@ -315,14 +349,11 @@ __global__ __launch_bounds__(kT) void gn_apply(const T* __restrict__ x, const Mo
             rstd_out[b * q.G + g] = s_rstd[g - g0];
         }
     if (!live) return;
-    float mu[V], a[V], sh[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const int c = c0 + col * V + j, g = c / q.Cg - g0;
-        mu[j] = s_mean[g];
-        a[j] = s_rstd[g] * (weight ? weight[c] : 1.f);
-        sh[j] = bias ? bias[c] : 0.f;
-    }
+    float mu[V];
+    groups_of<V>(c0 + col * V, q.Cg, [&](int j, int g) {
+        mu[j] = s_mean[g - g0];
+        a[j] *= s_rstd[g - g0];
+    });
     auto one = [&](const Raw<T, V>& r, int s) {
         float v[V];
         r.get(v);
@@ -367,15 +398,12 @@ __global__ __launch_bounds__(kT) void gn_bwd_sums(const T* __restrict__ x, const
     const int s0 = blockIdx.x * q.chunk, s1 = min(s0 + q.chunk, q.S);
     if (row < rows && col * V < wc) {
         float mu[V], rs[V], w[V], sh[V], a1[V], a2[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int c = c0 + col * V + j, g = b * q.G + c / q.Cg;
-            mu[j] = mean[g];
-            rs[j] = rstd[g];
-            w[j] = weight ? weight[c] : 1.f;
-            sh[j] = bias ? bias[c] : 0.f;
+        load_params<V>(weight, bias, c0 + col * V, w, sh);
+        groups_of<V>(c0 + col * V, q.Cg, [&](int j, int g) {
+            mu[j] = mean[b * q.G + g];
+            rs[j] = rstd[b * q.G + g];
             a1[j] = a2[j] = 0.f;
-        }
+        });
         const int64_t base = ((int64_t)b * q.S) * q.C + c0 + col * V;
         auto add = [&](const Raw<T, V>& rx, const Raw<T, V>& rg) {
             float v[V], g[V];
@@ -484,6 +512,7 @@ __global__ __launch_bounds__(kT) void gn_bwd_apply(const T* __restrict__ x, cons
     const bool live = row < rows && col * V < wc;
     constexpr int U = 2;
     Raw<T, V> ax[U], ag[U];
+    float mu[V], rs[V], w[V], sh[V];
     if (live) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -491,6 +520,11 @@ __global__ __launch_bounds__(kT) void gn_bwd_apply(const T* __restrict__ x, cons
                 ax[u].load(x + base + (int64_t)(s0 + row + u * rows) * q.C);
                 ag[u].load(dy + base + (int64_t)(s0 + row + u * rows) * q.C);
             }
+        load_params<V>(weight, bias, c0 + col * V, w, sh);
+        groups_of<V>(c0 + col * V, q.Cg, [&](int j, int g) {
+            mu[j] = mean[b * q.G + g];
+            rs[j] = rstd[b * q.G + g];
+        });
     }
     by_groups<kT>(g1 - g0 + 1, q.L, [&](int gi, int l) {
         const bool on = g0 + gi <= g1;
@@ -529,17 +563,11 @@ __global__ __launch_bounds__(kT) void gn_bwd_apply(const T* __restrict__ x, cons
     });
     __syncthreads();
     if (!live) return;
-    float mu[V], rs[V], w[V], sh[V], m1[V], m2[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const int c = c0 + col * V + j, g = c / q.Cg;
-        mu[j] = mean[b * q.G + g];
-        rs[j] = rstd[b * q.G + g];
-        w[j] = weight ? weight[c] : 1.f;
-        sh[j] = bias ? bias[c] : 0.f;
+    float m1[V], m2[V];
+    groups_of<V>(c0 + col * V, q.Cg, [&](int j, int g) {
         m1[j] = s_1[g - g0];
         m2[j] = s_2[g - g0];
-    }
+    });
     auto one = [&](const Raw<T, V>& rx, const Raw<T, V>& rg, int s) {
         float v[V], g[V];
         rx.get(v);
@@ -628,19 +656,6 @@ __device__ __forceinline__ void slab_sums(const Slab& q, int R, float v1, float 
     __syncthreads();
 }
 
-// V neighbouring channels' weights and biases, all loads at once (a column of the slab is one for every thread)
-template <int V>
-__device__ __forceinline__ void load_params(const float* __restrict__ weight, const float* __restrict__ bias, int c, float (&w)[V], float (&sh)[V]) {
-    if (weight) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) w[j] = weight[c + j];
-    }
-    if (bias) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) sh[j] = bias[c + j];
-    }
-}
-
 template <class T, int V, int ACT, int NT, int NV>
 __global__ __launch_bounds__(NT) void gn_slab(const T* __restrict__ x, const float* __restrict__ weight,
                                               const float* __restrict__ bias, T* __restrict__ y, float* __restrict__ mean_out,
@@ -659,11 +674,6 @@ __global__ __launch_bounds__(NT) void gn_slab(const T* __restrict__ x, const flo
     for (int i = 0; i < NV; ++i)
         if (live && row + i * R < q.S) r[i].load(x + base + (int64_t)(row + i * R) * q.C);
     float w[V], sh[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        w[j] = 1.f;
-        sh[j] = 0.f;
-    }
     load_params<V>(weight, bias, c0 + col * V, w, sh);
     const float inv_n = 1.0f / ((float)q.S * (float)q.Cg);
     float t = 0.f;
@@ -738,10 +748,7 @@ __global__ __launch_bounds__(NT) void gn_slab_bwd(const T* __restrict__ x, const
     float w[V], sh[V], a1[V], a2[V];
     const float mu = live ? mean[b * q.G + c0 / q.Cg + gl] : 0.f, rs = live ? rstd[b * q.G + c0 / q.Cg + gl] : 0.f;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        w[j] = 1.f;
-        sh[j] = a1[j] = a2[j] = 0.f;
-    }
+    for (int j = 0; j < V; ++j) a1[j] = a2[j] = 0.f;
     load_params<V>(weight, bias, c0 + col * V, w, sh);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
