@@ -114,7 +114,8 @@ __global__ __launch_bounds__(NG * 128, OCC) void diff_fwd(DiffArgs a, DiffOut o,
             qf[t] = chunk_or_zero<T>(qg, c, c < dc);
         }
     }
-    const float weight = KEYS && map ? 0.f : map_weight<DP>(a, place.head, lane);
+    // few rows: the first wave's, and none where the second kernel joins the splits
+    const float weight = KEYS && (wave != 0 || splits > 1) ? 0.f : map_weight<DP>(a, place.head, lane);
 
     constexpr bool MSUM = !TRAIN && sizeof(T) == 2;
     f32x16 acc[DB], l_acc = zero16();
