@@ -283,20 +283,20 @@ struct Stage {
     }
 };
 
-// w_h = exp(lam0 . lam1) - exp(lam2 . lam3) + lambda_init, all loads at once.  Where all lanes want the same head the first
+// w_h = exp(lam0 . lam1) - exp(lam2 . lam3) + lambda_init, all loads at once.  Where all lanes want the same head (same: they do) the first
 // half-wave adds the first product, a column to a lane, and the second the other; else the half-waves share the sums of a
 // lane's own head.
 template <int DP>
-__device__ __forceinline__ float map_weight(const DiffArgs& a, int head, int lane) {
+__device__ __forceinline__ float map_weight(const DiffArgs& a, int head, int lane, bool same) {
     const int hh = lane >> 5, col = lane & 31;
     const int64_t vs = (int64_t)a.lam_heads * a.d;
     float s1, s2;
-    if (a.group == 1 || a.lam_heads == 1) {
+    if (same || a.group == 1 || a.lam_heads == 1) {
         const float* p = a.lam + (a.lam_heads == 1 ? 0 : (int64_t)__builtin_amdgcn_readfirstlane(head) * a.d) + 2 * hh * vs;
         const int e = col < a.d ? col : 0, e2 = DP > 32 && col + 32 < a.d ? col + 32 : 0;
         const float x = p[e], y = p[vs + e], x2 = p[e2], y2 = p[vs + e2];
         float s = col < a.d ? x * y : 0.f;
-        if (DP > 32 && col + 32 < a.d) s = fmaf(x2, y2, s);
+        if constexpr (DP > 32) s += col + 32 < a.d ? x2 * y2 : 0.f;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) s += __shfl_xor(s, o, 64);
         const unsigned u = __builtin_bit_cast(unsigned, s);

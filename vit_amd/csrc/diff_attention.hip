@@ -115,7 +115,7 @@ __global__ __launch_bounds__(NG * 128, OCC) void diff_fwd(DiffArgs a, DiffOut o,
         }
     }
     // few rows: the first wave's, and none where the second kernel joins the splits
-    const float weight = KEYS && (wave != 0 || splits > 1) ? 0.f : map_weight<DP>(a, place.head, lane);
+    const float weight = KEYS && (wave != 0 || splits > 1) ? 0.f : map_weight<DP>(a, place.head, lane, false);
 
     constexpr bool MSUM = !TRAIN && sizeof(T) == 2;
     f32x16 acc[DB], l_acc = zero16();
@@ -332,8 +332,17 @@ __global__ __launch_bounds__(256) void diff_fwd_join(DiffArgs a, DiffOut o, cons
     // the splits' values are on their way while the factors are computed
     const int m = tid / (CH * NP), c = tid % CH, part = tid / CH % NP;
     const float* p = base + (int64_t)part * STRIDE + rr * 2 * DV + m * DV + c * 4;
-    f32x4 first = {0.f, 0.f, 0.f, 0.f};
-    if (tid < 2 * CH * NP && part < splits) first = *reinterpret_cast<const f32x4*>(p);
+    constexpr int U = 4;                                             // loads on their way at once
+    auto batch = [&](int s0, f32x4 (&v)[U]) {                         // splits past the last one: the last one again
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (u && u * NP >= splits) break;                        // the same for all
+            const int s = s0 + u * NP < splits ? s0 + u * NP : splits - 1;
+            v[u] = *reinterpret_cast<const f32x4*>(p + (int64_t)(s - part) * STRIDE);
+        }
+    };
+    f32x4 v[U];
+    if (tid < 2 * CH * NP) batch(part, v);
     if (wave < 2) {                                                  // wave m joins map m's maxima and sums
         float mx[2], l[2];
 #pragma unroll
@@ -364,7 +373,7 @@ __global__ __launch_bounds__(256) void diff_fwd_join(DiffArgs a, DiffOut o, cons
             }
         }
     } else if (wave == 2) {
-        const float w = map_weight<DV / 2>(a, pl.head, lane);
+        const float w = map_weight<DV / 2>(a, pl.head, lane, true);
         if (lane == 0) {
             s_w = w;
             if (o.out2 && b == 0 && pl.tok == 0) o.weight[pl.head] = w;
@@ -373,16 +382,15 @@ __global__ __launch_bounds__(256) void diff_fwd_join(DiffArgs a, DiffOut o, cons
     __syncthreads();
     if (tid < 2 * CH * NP) {
         f32x4 x = {0.f, 0.f, 0.f, 0.f};
-        if (part < splits) {
-            const float f = s_f[m][part];
+        for (int s0 = part; s0 < splits; s0 += U * NP) {
+            if (s0 != part) batch(s0, v);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = first[j] * f;
-        }
-        for (int s = part + NP; s < splits; s += NP) {
-            const f32x4 v = *reinterpret_cast<const f32x4*>(p + (int64_t)(s - part) * STRIDE);
-            const float f = s_f[m][s];
+            for (int u = 0; u < U; ++u) {
+                if (u && u * NP >= splits) break;
+                const float f = s0 + u * NP < splits ? s_f[m][s0 + u * NP] : 0.f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = fmaf(v[j], f, x[j]);
+                for (int j = 0; j < 4; ++j) x[j] = s0 + u * NP < splits ? fmaf(v[u][j], f, x[j]) : x[j];
+            }
         }
         s_part[part][m][c] = x;
     }
