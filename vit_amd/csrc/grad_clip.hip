@@ -170,7 +170,16 @@ __global__ __launch_bounds__(kThreads) void grad_norm_partials(GradTable t, doub
 template <bool INF>
 __device__ __forceinline__ double norm_of(const double* __restrict__ partials, int n, double* red) {
     double v = 0.0;
-    for (int i = threadIdx.x; i < n; i += kThreads) v = INF ? max_nan(v, partials[i]) : v + partials[i];
+    for (int i = threadIdx.x; i < n; i += 4 * kThreads) {
+        double w[4];                                                 // loads on their way at once
+#pragma unroll
+        for (int u = 0; u < 4; ++u) w[u] = partials[i + u * kThreads < n ? i + u * kThreads : i];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const double x = i + u * kThreads < n ? w[u] : 0.0;
+            v = INF ? max_nan(v, x) : v + x;
+        }
+    }
     const double r = block_reduce<INF>(v, red);
     return INF ? r : sqrt(r);
 }
