@@ -18,7 +18,12 @@ def _on_device(x):
 
 
 def _needs_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if not torch.is_grad_enabled():
+        return False
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return True
+    return False
 
 
 def group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, activation="none"):

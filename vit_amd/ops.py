@@ -630,30 +630,31 @@ def _scratch(floats, device):
 def _strides(*tensors):
     """Host array of the element strides of all but the last dimension (0 where a dimension has one entry)."""
     st = [s if n > 1 else 0 for t in tensors for s, n in zip(t.stride()[:-1], t.shape)]
-    return (_lib.ctypes.c_int64 * len(st))(*st)
+    return struct.pack(f"{len(st)}q", *st)
 
 
 def _diff_sizes(q, k, v, lam, key_lens):
-    code = _DTYPE_CODES.get(q.dtype)
+    code, qs, ks, vs = _DTYPE_CODES.get(q.dtype), q.shape, k.shape, v.shape
     if code is None or k.dtype != q.dtype or v.dtype != q.dtype:
         raise _lib.VitkError(f"diff_attention: q, k and v must be bf16 or f32 alike, got {q.dtype}, {k.dtype}, {v.dtype}")
-    if q.dim() != 5 or k.dim() != 5 or v.dim() != 4:
-        raise _lib.VitkError(f"diff_attention: expected q [B,Nq,H,2,d], k [B,Nk,K,2,d], v [B,Nk,K,2d], got {tuple(q.shape)}, "
-                             f"{tuple(k.shape)}, {tuple(v.shape)}")
-    B, nq, H, two, d = q.shape
-    nk, K = k.shape[1], k.shape[2]
-    if two != 2 or tuple(k.shape) != (B, nk, K, 2, d) or tuple(v.shape) != (B, nk, K, 2 * d) or K < 1 or H % K:
-        raise _lib.VitkError(f"diff_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not match")
-    if lam.dtype != torch.float32 or not lam.is_contiguous() or tuple(lam.shape) not in ((4, d), (4, H, d)):
+    if len(qs) != 5 or len(ks) != 5 or len(vs) != 4:
+        raise _lib.VitkError(f"diff_attention: expected q [B,Nq,H,2,d], k [B,Nk,K,2,d], v [B,Nk,K,2d], got {tuple(qs)}, "
+                             f"{tuple(ks)}, {tuple(vs)}")
+    B, nq, H, two, d = qs
+    nk, K = ks[1], ks[2]
+    if two != 2 or ks != (B, nk, K, 2, d) or vs != (B, nk, K, 2 * d) or K < 1 or H % K:
+        raise _lib.VitkError(f"diff_attention: q {tuple(qs)}, k {tuple(ks)}, v {tuple(vs)} do not match")
+    if lam.dtype != torch.float32 or not lam.is_contiguous() or lam.shape not in ((4, d), (4, H, d)):
         raise _lib.VitkError(f"diff_attention: lam must be contiguous f32 [4,{d}] or [4,{H},{d}], got {lam.dtype} {tuple(lam.shape)}")
-    if key_lens is not None and (key_lens.dtype != torch.int32 or tuple(key_lens.shape) != (B,) or not key_lens.is_contiguous()):
+    if key_lens is not None and (key_lens.dtype != torch.int32 or key_lens.shape != (B,) or not key_lens.is_contiguous()):
         raise _lib.VitkError(f"diff_attention: key_lens must be contiguous int32 [{B}], got {key_lens.dtype} {tuple(key_lens.shape)}")
     dev = q.get_device()
-    for n, t in (("q", q), ("k", k), ("v", v), ("lam", lam), ("key_lens", key_lens)):
-        if t is not None and (not t.is_cuda or t.get_device() != dev):
-            raise _lib.VitkError(f"diff_attention: {n} is on {t.device}, q on {q.device}")
+    if dev < 0 or not dev == k.get_device() == v.get_device() == lam.get_device() or key_lens is not None and key_lens.get_device() != dev:
+        for n, t in (("q", q), ("k", k), ("v", v), ("lam", lam), ("key_lens", key_lens)):
+            if t is not None and (not t.is_cuda or t.get_device() != dev):
+                raise _lib.VitkError(f"diff_attention: {n} is on {t.device}, q on {q.device}")
     if max(B, nq, nk, H) > 0x7FFFFFFF:
-        raise _lib.VitkError(f"diff_attention: q {tuple(q.shape)}, k {tuple(k.shape)} are too large")
+        raise _lib.VitkError(f"diff_attention: q {tuple(qs)}, k {tuple(ks)} are too large")
     if q.numel() and k.numel() and (q.stride(4) != 1 or k.stride(4) != 1 or v.stride(3) != 1):
         raise _lib.VitkError("diff_attention: the last dimension of q, k and v must be dense")
     return B, nq, nk, H, K, d, code
