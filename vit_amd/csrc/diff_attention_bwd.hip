@@ -118,19 +118,29 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_q(DiffArgs a, DiffGrad
         for (int t = 0; t < 2 * KT; ++t) s += dot<T>(of[t], o[t]);
         s = both_sum(s);
         if (hh == 0) s_dot[grp][map][r] = s;
+        // The matrix pipe's rounding leans to one side by some 1e-9 of dA, which a sum over all rows collects while the rows' own
+        // terms cancel (dw off by 1e-5 of itself and more at 16 x 577 rows of 8 heads): every other row goes through it negated.
+        if (r & 1) {
+#pragma unroll
+            for (int t = 0; t < 2 * KT; ++t)
+#pragma unroll
+                for (int j = 0; j < PER; ++j) of[t][j] = -of[t][j];
+        }
     }
+    const float sign = r & 1 ? -1.f : 1.f;
 
     f32x16 dq[EB];
 #pragma unroll
     for (int e = 0; e < EB; ++e) dq[e] = zero16();
-    float dw = 0.f;
+    double dw = 0.0;      // the terms nearly cancel: what a block of keys adds in f32 is collected in f64
     const float sc = a.scale * kLog2e;
 
     if (c0 < c1) stage.put(bufs[0]);
     loads_done();
     __syncthreads();
-    const float dd = map ? s_dot[grp][1][r] : fmaf(weight, s_dot[grp][1][r], s_dot[grp][0][r]);
+    float dd = map ? s_dot[grp][1][r] : fmaf(weight, s_dot[grp][1][r], s_dot[grp][0][r]);
     if (row < nrows && hh == 0 && split == 0) ws_d[map * lmap + lrow] = dd;
+    dd *= sign;
     auto chunk = [&](int c, auto which) __attribute__((always_inline)) {                            // the buffer is known when compiled: no address arithmetic
         const char* kt = bufs[decltype(which)::value];
         const char* vt = kt + TILE;
@@ -146,12 +156,14 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_q(DiffArgs a, DiffGrad
 #pragma unroll
             for (int t = 0; t < 2 * KT; ++t) da = Op<T>::mma(chunk_at<T, RB>(vt, kb + r, 2 * t + hh), of[t], da);
             if (key0 + 32 > wave_min) hide(s, lim - key0 - 4 * hh);
+            float part = 0.f;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const float p = __builtin_amdgcn_exp2f(fmaf(s[i], sc, -ref));     // times 1 / l at the end
-                dw = fmaf(p, da[i], dw);
+                part = fmaf(p, da[i], part);
                 s[i] = p * (da[i] - dd);
             }
+            dw += (double)part;
 #pragma unroll
             for (int st = 0; st < 2; ++st) {
                 Slice<T> ds;
@@ -172,20 +184,20 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_q(DiffArgs a, DiffGrad
         if (c + 1 < c1) chunk(c + 1, std::integral_constant<int, 1>{});
     }
 
-    dw = both_sum(dw) * inv;
-    if (map == 1 && hh == 0) s_dw[grp * 32 + r] = row < nrows ? -dw : 0.f;
+    const float row_dw = both_sum((float)dw) * inv * sign;
+    if (map == 1 && hh == 0) s_dw[grp * 32 + r] = row < nrows ? -row_dw : 0.f;
     __syncthreads();
     for (int h = tid; h < a.group; h += kThreads) {
         // rows of the workgroup that belong to the group's head h
         const int first = tile * kBlock;
-        float t = 0.f;
+        double t = 0.0;
         for (int i = (h - first % a.group + a.group) % a.group; i < kBlock; i += a.group) t += s_dw[i];
-        ws_w[(((int64_t)bk * tiles + tile) * splits + split) * a.group + h] = t;
+        ws_w[(((int64_t)bk * tiles + tile) * splits + split) * a.group + h] = (float)t;
     }
     // [split][sample, head, token][map][d]
     float* part = splits > 1 ? parts + ((split * lmap + lrow) * 2 + map) * a.d : nullptr;
     T* out = reinterpret_cast<T*>(g.dq) + b * g.dqs[0] + place.tok * g.dqs[1] + place.head * g.dqs[2] + map * g.dqs[3];
-    const float f = map == 0 ? inv * a.scale : -weight * inv * a.scale;
+    const float f = sign * (map == 0 ? inv * a.scale : -weight * inv * a.scale);
 #pragma unroll
     for (int e = 0; e < EB; ++e)
 #pragma unroll
