@@ -49,6 +49,41 @@ def test_shipped_kernels_have_no_scalar_load_inside_counted_waits():
     assert build.check_counted_waits(verbose=False)
 
 
+def test_in_flight_scanner_flags_uses_of_a_transposed_lds_read_before_its_wait():
+    """The compiler takes the result of an inline-asm LDS read as there at once: a copy or a spill of it ahead of the wait
+    moves whatever the register held."""
+    from vit_amd import build
+    clean = """
+_Z6kernelPv:
+\tds_read_b64_tr_b16 v[0:1], v2 offset:0
+\tds_read_b64_tr_b16 v[4:5], v2 offset:1024
+\tv_exp_f32_e32 v3, v3
+\ts_waitcnt lgkmcnt(1)
+\tv_mov_b64_e32 v[6:7], v[0:1]
+\ts_waitcnt lgkmcnt(0)
+\tv_mov_b32_e32 v9, v5
+\ts_endpgm
+.Lfunc_end0:
+"""
+    assert build.scan_in_flight(clean) == []
+    copy = clean.replace("\tv_exp_f32_e32 v3, v3\n", "\tv_mov_b64_e32 v[6:7], v[0:1]\n")
+    assert [ins for _, _, ins in build.scan_in_flight(copy)] == ["v_mov_b64_e32 v[6:7], v[0:1]"]
+    spill = clean.replace("\tv_exp_f32_e32 v3, v3\n", "\tscratch_store_dwordx2 off, v[4:5], off offset:72\n")
+    assert len(build.scan_in_flight(spill)) == 1
+    early = clean.replace("lgkmcnt(1)", "lgkmcnt(2)")               # two reads on their way, one of them used
+    assert len(build.scan_in_flight(early)) == 1
+    younger = early.replace("\tv_exp_f32_e32 v3, v3\n", "\tds_read_b128 v[20:23], v2\n")
+    assert build.scan_in_flight(younger) == []                       # two younger ones: lgkmcnt(2) covers the first
+    # along a loop's back edge: the read at the end of the body is used at its start
+    loop = ("_Z6kernelPv:\n.LBB0_1:\n\tv_add_u32_e32 v3, v0, v3\n\tds_read_b64_tr_b16 v[0:1], v2\n"
+            "\ts_cbranch_vccnz .LBB0_1\n\ts_endpgm\n.Lfunc_end0:\n")
+    assert len(build.scan_in_flight(loop)) == 1
+    # an LDS-DMA that no wait has covered when its barrier comes
+    dma = "_Z6kernelPv:\n\tglobal_load_lds_dwordx4 v[0:1], off\n\ts_waitcnt vmcnt({})\n\ts_barrier\n\ts_endpgm\n.Lfunc_end0:\n"
+    assert build.scan_in_flight(dma.format(0)) == []
+    assert len(build.scan_in_flight(dma.format(1))) == 1
+
+
 def test_two_plane_representation_of_f32_round_trips_every_bit_pattern_class():
     """The residual stream between the folded blocks is held as plane H = upper half of bits(x) + 0x8000 (bf16 rounded
     half up) and plane L = lower half of bits(x); bits(x) = (H << 16) + sext16(L).  Host-side helpers (torch ops, the

@@ -7,6 +7,7 @@ No torch headers are involved: the library is a bare `hipcc -shared -fPIC
 cross-compiles gfx950 code without a GPU.
 """
 import os
+import re
 import subprocess
 import sys
 from concurrent.futures import ThreadPoolExecutor
@@ -81,17 +82,19 @@ def build(force=False, verbose=True, probes=False):
     return lib
 
 
-# Sources whose kernels wait for inline-asm LDS reads with counted `s_waitcnt lgkmcnt(n)`: the counts hold only while
-# nothing else of the wave is outstanding on that counter.  LDS returns in order, scalar memory does not, so one scalar
-# load (a kernel-argument or descriptor reload) between a transposed LDS read and the wait that covers it could let
-# the wait pass early.
+# Sources whose transposed LDS reads are looked at in the compiled code.  gemm_tn.hip waits for inline-asm LDS reads with
+# counted `s_waitcnt lgkmcnt(n)`: the counts hold only while nothing else of the wave is outstanding on that counter.  LDS
+# returns in order, scalar memory does not, so one scalar load (a kernel-argument or descriptor reload) between a
+# transposed LDS read and the wait that covers it could let the wait pass early.  And the compiler does not know that such
+# a read's result is still on its way, so it may copy or spill the register before the wait: that too fails the build.
+# attention.hip leaves the waits of its reads to the compiler; its LDS-DMA is inline asm that the compiler does not know
+# of, so a barrier that one reaches without the kernel's own wait fails the build.
 COUNTED_WAIT_SOURCES = ["attention.hip", "gemm_tn.hip"]
 
 
 def scan_counted_waits(asm_text):
     """(kernel, line number, instruction) of every scalar-memory instruction that sits, in program text order, between
     a ds_read_b64_tr_b16 and the next `s_waitcnt` with lgkmcnt(0) of the same kernel."""
-    import re
     found, kernel, pending = [], None, False
     for ln, line in enumerate(asm_text.splitlines(), 1):
         t = line.strip()
@@ -112,9 +115,89 @@ def scan_counted_waits(asm_text):
     return found
 
 
+def _asm_kernels(asm_text):
+    """(name, [(line number, instruction or label)]) of every function in compiler-written assembly."""
+    name, body = None, []
+    for ln, line in enumerate(asm_text.splitlines(), 1):
+        t = line.split(";")[0].strip()
+        if re.match(r"^_Z\w+:", t):
+            name, body = t[:-1], []
+        elif name and t.startswith(".Lfunc_end"):
+            yield name, body
+            name = None
+        elif name and t and (t[0] != "." or t.endswith(":")):
+            body.append((ln, t))
+    if name:
+        yield name, body
+
+
+def _vector_registers(operands):
+    regs = set()
+    for one, lo, hi in re.findall(r"\bv(?:(\d+)|\[(\d+):(\d+)\])", operands):
+        regs.update([int(one)] if one else range(int(lo), int(hi) + 1))
+    return regs
+
+
+def scan_in_flight(asm_text):
+    """(kernel, line number, instruction) of every instruction that touches the result of a transposed LDS read before a
+    wait that covers the read, and of every barrier that an LDS-DMA reaches without an `s_waitcnt` with vmcnt(0), along any
+    path through a kernel.  A read is covered by lgkmcnt(n) if n LDS instructions or more have followed it, since LDS
+    returns in order."""
+    found = []
+    for kernel, body in _asm_kernels(asm_text):
+        blocks, label = [[]], {}
+        for ln, t in body:
+            if t.endswith(":"):
+                blocks.append([])
+                label[t[:-1]] = len(blocks) - 1
+                continue
+            blocks[-1].append((ln, t))
+            if t.startswith(("s_branch", "s_cbranch", "s_endpgm")):
+                blocks.append([])
+        after = [[i + 1] if i + 1 < len(blocks) else [] for i in range(len(blocks))]
+        for i, b in enumerate(blocks):
+            op = b[-1][1].split() if b else [""]
+            if op[0] in ("s_branch", "s_endpgm"):
+                after[i] = []
+            if op[0].startswith(("s_branch", "s_cbranch")):
+                after[i] = after[i] + [label[op[1]]]
+        # state: in-flight register -> LDS instructions since its read (the fewest over all paths), "dma" -> 0 if one is out
+        states, work, bad = {0: {}}, [0], {}
+        while work:
+            i = work.pop()
+            st = dict(states[i])
+            for ln, t in blocks[i]:
+                op, _, rest = t.partition(" ")
+                if op == "s_waitcnt":
+                    m = re.search(r"lgkmcnt\((\d+)\)", t)
+                    if m:
+                        st = {r: n for r, n in st.items() if r == "dma" or n < int(m.group(1))}
+                    if "vmcnt(0)" in t:
+                        st.pop("dma", None)
+                    continue
+                is_read = op == "ds_read_b64_tr_b16"
+                dst, _, src = rest.partition(",") if is_read else ("", "", rest)
+                if _vector_registers(src) & st.keys() or op == "s_barrier" and "dma" in st:
+                    bad[ln] = t
+                if op.startswith("ds_"):
+                    st = {r: n if r == "dma" else n + 1 for r, n in st.items()}
+                for r in _vector_registers(dst):
+                    st[r] = 0
+                if "_lds_" in op and op.startswith(("global_load", "buffer_load")):
+                    st["dma"] = 0
+            for j in after[i]:
+                old = states.get(j)
+                new = dict(st) if old is None else {r: min(n for n in (old.get(r), st.get(r)) if n is not None) for r in old.keys() | st.keys()}
+                if new != old:
+                    states[j] = new
+                    work.append(j)
+        found += [(kernel, ln, t) for ln, t in sorted(bad.items())]
+    return found
+
+
 def check_counted_waits(verbose=True):
     """Compile COUNTED_WAIT_SOURCES to gfx950 assembly (cached beside the objects) and fail if the compiler put a
-    scalar-memory instruction inside a counted-wait region."""
+    scalar-memory instruction inside a counted-wait region, or uses a transposed LDS read's result before its wait."""
     objdir = os.path.join(HERE, "build")
     os.makedirs(objdir, exist_ok=True)
     hipcc = _hipcc()
@@ -132,10 +215,16 @@ def check_counted_waits(verbose=True):
         outs = list(ex.map(asm_of, COUNTED_WAIT_SOURCES))
     for src, out in zip(COUNTED_WAIT_SOURCES, outs):
         with open(out) as f:
-            bad = scan_counted_waits(f.read())
+            asm = f.read()
+        bad = scan_counted_waits(asm)
         if bad:
             k, ln, ins = bad[0]
             raise RuntimeError(f"{src}: {len(bad)} scalar-memory instruction(s) inside a counted lgkmcnt wait region, "
+                               f"first in {k} at {os.path.basename(out)}:{ln}: {ins}")
+        bad = scan_in_flight(asm)
+        if bad:
+            k, ln, ins = bad[0]
+            raise RuntimeError(f"{src}: {len(bad)} instruction(s) ahead of the wait for a transposed LDS read or an LDS-DMA, "
                                f"first in {k} at {os.path.basename(out)}:{ln}: {ins}")
     return True
 

@@ -30,6 +30,16 @@ typedef __attribute__((address_space(1))) const void gbl_void;
 
 constexpr float kMaskedScore = -1.0e30f;
 
+// One LDS-DMA instruction of the wave: 64 lanes x 16 bytes from `src` (per lane) to 1 KiB of LDS at `dst` (wave-uniform).
+// Through inline asm, so that the compiler does not know of the LDS write: it cannot tell that the write goes to another
+// buffer than the one being read, and would wait for all vector memory in front of every transposed LDS read of the key
+// loop.  The kernel itself waits (vmcnt(0), then a barrier) before it reads what was written.  No register is written; m0
+// has to be set one wait state before its use.
+__device__ __forceinline__ void lds_dma16(const void* src, char* dst) {
+    const int at = __builtin_amdgcn_readfirstlane((int)(uintptr_t)(lds_void*)dst);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(src) : "m0", "memory");
+}
+
 // f(integral_constant<int, I>) for I = First .. Last - 1, unrolled at compile time
 template <int First, int Last, class F>
 __device__ __forceinline__ void static_for(F&& f) {
@@ -135,7 +145,8 @@ __global__ __launch_bounds__((NW + (LW ? 1 : 0)) * 64) void attention_fwd(const 
             c = c < HD / 8 ? c : HD / 8 - 1;
             const int grow = row0 + lrow < ntok ? row0 + lrow : ntok - 1;
             const bf16_t* src = (is_v ? vg : kg) + (size_t)grow * HD + c * 8;
-            __builtin_amdgcn_global_load_lds((gbl_void*)src, (lds_void*)(dst + pi * 1024), 16, 0, 0);
+            if constexpr (OVL) lds_dma16(src, dst + pi * 1024);
+            else __builtin_amdgcn_global_load_lds((gbl_void*)src, (lds_void*)(dst + pi * 1024), 16, 0, 0);
         }
     };
 
@@ -278,41 +289,25 @@ __global__ __launch_bounds__((NW + (LW ? 1 : 0)) * 64) void attention_fwd(const 
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o_acc[d][i] *= alpha;
         }
-        // OVL: V^T fragments of the first 16-key slice are requested before the exponentials (the inline asm is a
-        // scheduling barrier: issued after them, the first P.V of every step would wait out the LDS latency)
+        // V^T fragments of 16-key slice g of the step.  OVL: those of the first two slices are requested before the
+        // exponentials, whose time hides the LDS latency, the others two slices ahead of their products.
         constexpr int G = NB * 2;
-        bf16x4 vv[2][DB][2];
-        uint32_t vblk[DB];                  // this step's first V row for each 32-column block of O^T
-        if constexpr (OVL) {
-            const uint32_t vb = (uint32_t)(uintptr_t)(lds_void*)(v_lds + lb * (32 * RB));
-#pragma unroll
-            for (int d = 0; d < DB; ++d) vblk[d] = vb + (uint32_t)vfrag[d];
-        }
-        auto issue = [&](auto gc, bf16x4 (&dst)[DB][2]) {
-            constexpr int g = decltype(gc)::value;
-            constexpr int off = ((g >> 1) * 32 + 16 * (g & 1)) * RB;      // 16-key slice g of the step
+        bf16x8 vf[2][DB];
+        const char* vblk = v_lds + lb * (32 * RB);          // this step's first V row
+        auto fragments = [&](int g, bf16x8 (&dst)[DB]) __attribute__((always_inline)) {
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
-                const uint32_t addr = vblk[d];
-                asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(dst[d][0]) : "v"(addr), "n"(off));
-                asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(dst[d][1]) : "v"(addr), "n"(off + 8 * RB));
-            }
-        };
-        auto landed = [&](bf16x4 (&w)[DB][2], auto last_c) {
-            constexpr bool last = decltype(last_c)::value;       // no younger group in flight
-            if constexpr (DB == 2) {
-                if constexpr (last) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(w[0][0]), "+v"(w[0][1]), "+v"(w[1][0]), "+v"(w[1][1]));
-                else asm volatile("s_waitcnt lgkmcnt(4)" : "+v"(w[0][0]), "+v"(w[0][1]), "+v"(w[1][0]), "+v"(w[1][1]));
-            } else {
-                if constexpr (last) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(w[0][0]), "+v"(w[0][1]), "+v"(w[1][0]), "+v"(w[1][1]), "+v"(w[2][0]), "+v"(w[2][1]));
-                else asm volatile("s_waitcnt lgkmcnt(6)" : "+v"(w[0][0]), "+v"(w[0][1]), "+v"(w[1][0]), "+v"(w[1][1]), "+v"(w[2][0]), "+v"(w[2][1]));
+                const char* a = vblk + vfrag[d] + ((g >> 1) * 32 + 16 * (g & 1)) * RB;
+                const bf16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)a);
+                const bf16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(a + 8 * RB));
+                dst[d] = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
             }
         };
         // the last block's second 16-key slice holds no key at all when at most 16 of its keys exist (wave-uniform)
         const bool skip_tail = gb + NB == kblocks && tail_keys <= 16;
         if constexpr (OVL) {
-            issue(std::integral_constant<int, 0>{}, vv[0]);
-            if (G > 2 || !skip_tail) issue(std::integral_constant<int, 1>{}, vv[1]);
+            fragments(0, vf[0]);
+            if (G > 2 || !skip_tail) fragments(1, vf[1]);
         }
         float psum = 0.f;
 #pragma unroll
@@ -332,36 +327,25 @@ __global__ __launch_bounds__((NW + (LW ? 1 : 0)) * 64) void attention_fwd(const 
         if constexpr (!MSUM) l_run += psum;
         // O^T[d][q] += V^T[d][key] P^T[key][q]; the packed P^T accumulators are the B operand
         if constexpr (OVL) {
-            // The transposed LDS reads go through inline asm with hand-placed lgkmcnt waits.  Issued through
-            // the builtin, the compiler puts an s_waitcnt vmcnt(0) in front of them for as long as any
-            // LDS-DMA is in flight (it cannot tell that the DMA fills the other buffer), i.e. the first
-            // P.V of a head would wait for the whole staging of the next head.  Groups of 2 DB reads
-            // (one 16-key slice) are issued two groups ahead of the MFMAs that use them (the first two before the
-            // exponentials); the wait is tied to the group's registers so that the MFMAs cannot move above it.
-            auto slice = [&](auto gc, auto last_c, auto gs_c) {
+            auto slice = [&](auto gc, auto gs_c) __attribute__((always_inline)) {
                 constexpr int g = decltype(gc)::value;
                 constexpr int GS = decltype(gs_c)::value;            // slices this step works through
                 constexpr int u = g >> 1, st = g & 1;
                 u32x4 pk = {pack_bf16(s[u][8 * st + 0], s[u][8 * st + 1]), pack_bf16(s[u][8 * st + 2], s[u][8 * st + 3]),
                             pack_bf16(s[u][8 * st + 4], s[u][8 * st + 5]), pack_bf16(s[u][8 * st + 6], s[u][8 * st + 7])};
                 const bf16x8 pf = __builtin_bit_cast(bf16x8, pk);
-                landed(vv[g & 1], last_c);
-                // copies: the slot is refilled (slice g + 2) while these MFMAs are still being issued
-                bf16x8 vf[DB];
 #pragma unroll
-                for (int d = 0; d < DB; ++d) vf[d] = __builtin_shufflevector(vv[g & 1][d][0], vv[g & 1][d][1], 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-                for (int d = 0; d < DB; ++d) o_acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[d], pf, o_acc[d], 0, 0, 0);
+                for (int d = 0; d < DB; ++d) o_acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[g & 1][d], pf, o_acc[d], 0, 0, 0);
                 l_acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ones, pf, l_acc, 0, 0, 0);
-                if constexpr (g + 2 < GS) issue(std::integral_constant<int, g + 2>{}, vv[g & 1]);
+                if constexpr (g + 2 < GS) fragments(g + 2, vf[g & 1]);
             };
             if (skip_tail) {
                 static_for<0, G - 1>([&](auto gc) {
-                    slice(gc, std::integral_constant<bool, decltype(gc)::value + 1 == G - 1>{}, std::integral_constant<int, G - 1>{});
+                    slice(gc, std::integral_constant<int, G - 1>{});
                 });
             } else {
                 static_for<0, G>([&](auto gc) {
-                    slice(gc, std::integral_constant<bool, decltype(gc)::value + 1 == G>{}, std::integral_constant<int, G>{});
+                    slice(gc, std::integral_constant<int, G>{});
                 });
             }
         } else {
