@@ -84,6 +84,17 @@ _Z6kernelPv:
     assert len(build.scan_in_flight(dma.format(1))) == 1
 
 
+def test_no_source_is_compiled_with_packed_f32_instructions():
+    """Some forms of v_pk_add/mul/fma_f32 have given wrong results on this hardware."""
+    from vit_amd import build
+    pk = "_Z1aPv:\n\tv_pk_mul_f32 v[0:1], v[2:3], v[4:5]\n\tv_pk_add_bf16 v0, v1, v2\n\ts_endpgm\n.Lfunc_end0:\n"
+    assert [ins.split()[0] for _, _, ins in build.scan_packed_f32(pk)] == ["v_pk_mul_f32"]
+    assert build.check_counted_waits(verbose=False)
+    flags = build.FLAGS
+    at = flags.index("-packed-fp32-ops")
+    assert flags[at - 3:at] == ["-Xclang", "-target-feature", "-Xclang"]
+
+
 def test_two_plane_representation_of_f32_round_trips_every_bit_pattern_class():
     """The residual stream between the folded blocks is held as plane H = upper half of bits(x) + 0x8000 (bf16 rounded
     half up) and plane L = lower half of bits(x); bits(x) = (H << 16) + sext16(L).  Host-side helpers (torch ops, the

@@ -7,7 +7,7 @@
 // 256 workgroups of 8 waves (one per CU), each wave keeps DEPTH batches of 4 instructions in flight over a
 // window small enough to stay in its XCD's L2.  Prints bytes per clock per CU from the shader clock counter.
 //
-//   hipcc -O3 --offload-arch=gfx950 tools/dma_probe.hip -o tools/dma_probe && tools/dma_probe
+//   hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops tools/dma_probe.hip -o tools/dma_probe && tools/dma_probe
 #include <hip/hip_runtime.h>
 
 #include <cstdint>

@@ -2,7 +2,7 @@
 // work: the shape that needs fewer register-file reads per flop may hold a higher clock).
 // 256 workgroups x 8 waves, operands loaded once from a random buffer, `iters` x 32 independent MFMAs per wave.
 //
-//   hipcc -O3 --offload-arch=gfx950 tools/mfma_power_probe.hip -o tools/mfma_power_probe && tools/mfma_power_probe
+//   hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops tools/mfma_power_probe.hip -o tools/mfma_power_probe && tools/mfma_power_probe
 #include <hip/hip_runtime.h>
 
 #include <cstdint>

@@ -1,7 +1,7 @@
 // Issue-rate probe for one CDNA4 SIMD: how many cycles a loop of 32x32x16 bf16 MFMAs, of exponentials, and of both
 // interleaved takes with one and with two waves per SIMD.  It answers whether the matrix pipe and the vector ALU
 // overlap within a wave and across the waves of a SIMD.
-//     hipcc -O2 --offload-arch=gfx950 tools/probe_issue.hip -o tools/probe_issue && tools/probe_issue
+//     hipcc -O2 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops tools/probe_issue.hip -o tools/probe_issue && tools/probe_issue
 #include <hip/hip_runtime.h>
 
 #include <cstdio>

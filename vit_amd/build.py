@@ -19,19 +19,10 @@ SOURCES = ["vitk_api.hip", "gemm.hip", "gemm_pipe.hip", "gemm_pp.hip", "attentio
            "group_norm.hip", "grad_clip.hip", "diff_attention.hip", "diff_attention_bwd.hip"]
 HEADERS = [os.path.join(CSRC, "vitk_common.h"), os.path.join(CSRC, "vitk_kernels.h"), os.path.join(CSRC, "gemm_common.h"), os.path.join(CSRC, "gemm_plan.h"), os.path.join(CSRC, "diff_attention.h"),
            os.path.join(os.path.dirname(HERE), "include", "vitk.h")]
-FLAGS = ["-O3", "-std=c++17", "--offload-arch=gfx950", "-fPIC", "-ffp-contract=fast"]
 # Packed f32 instructions (v_pk_add/mul/fma_f32) are switched off: some of their forms have given wrong results on this
-# hardware now and then, without an error, and -O3 makes them from ordinary float code by itself.  attention.hip keeps
-# them: without them its variants of head size 80 and 96 with five waves or more need so many registers that the compiler
-# spills the results of transposed LDS reads that are still on their way (their waits are placed by hand), and the output
-# is wrong; as it is, none is spilled.
-NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-PACKED_F32_SOURCES = ["attention.hip"]
-
-
-def _flags(src):
-    return FLAGS + ([] if os.path.basename(src) in PACKED_F32_SOURCES else NO_PACKED_F32)
-
+# hardware now and then, without an error, and -O3 makes them from ordinary float code by itself.
+FLAGS = ["-O3", "-std=c++17", "--offload-arch=gfx950", "-fPIC", "-ffp-contract=fast",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _hipcc():
@@ -60,12 +51,12 @@ def build(force=False, verbose=True, probes=False):
     for src in SOURCES:
         s = os.path.join(CSRC, src)
         o = os.path.join(objdir, src.replace(".hip", ".o"))
-        if force or _stale(o, [s] + HEADERS):
+        if force or _stale(o, [s, __file__] + HEADERS):
             jobs.append((s, o))
 
     def compile_one(job):
         s, o = job
-        cmd = [hipcc] + _flags(s) + (["-DVITK_PROBES"] if probes else []) + ["-c", s, "-o", o]
+        cmd = [hipcc] + FLAGS + (["-DVITK_PROBES"] if probes else []) + ["-c", s, "-o", o]
         if verbose:
             print("[vit_amd.build]", " ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)
@@ -195,17 +186,23 @@ def scan_in_flight(asm_text):
     return found
 
 
+def scan_packed_f32(asm_text):
+    """(kernel, line number, instruction) of every packed f32 instruction."""
+    return [(k, ln, t) for k, body in _asm_kernels(asm_text) for ln, t in body if re.match(r"v_pk_(add|mul|fma)_f32\b", t)]
+
+
 def check_counted_waits(verbose=True):
     """Compile COUNTED_WAIT_SOURCES to gfx950 assembly (cached beside the objects) and fail if the compiler put a
-    scalar-memory instruction inside a counted-wait region, or uses a transposed LDS read's result before its wait."""
+    scalar-memory instruction inside a counted-wait region, uses a transposed LDS read's result before its wait,
+    or made packed f32 instructions."""
     objdir = os.path.join(HERE, "build")
     os.makedirs(objdir, exist_ok=True)
     hipcc = _hipcc()
 
     def asm_of(src):
         s, out = os.path.join(CSRC, src), os.path.join(objdir, src.replace(".hip", ".s"))
-        if _stale(out, [s] + HEADERS):
-            cmd = [hipcc] + _flags(s) + ["-S", "--cuda-device-only", s, "-o", out]
+        if _stale(out, [s, __file__] + HEADERS):
+            cmd = [hipcc] + FLAGS + ["-S", "--cuda-device-only", s, "-o", out]
             if verbose:
                 print("[vit_amd.build]", " ".join(cmd), flush=True)
             subprocess.run(cmd, check=True, stderr=subprocess.DEVNULL)
@@ -226,6 +223,10 @@ def check_counted_waits(verbose=True):
             k, ln, ins = bad[0]
             raise RuntimeError(f"{src}: {len(bad)} instruction(s) ahead of the wait for a transposed LDS read or an LDS-DMA, "
                                f"first in {k} at {os.path.basename(out)}:{ln}: {ins}")
+        bad = scan_packed_f32(asm)
+        if bad:
+            k, ln, ins = bad[0]
+            raise RuntimeError(f"{src}: {len(bad)} packed f32 instruction(s), first in {k} at {os.path.basename(out)}:{ln}: {ins}")
     return True
 
 
