@@ -447,6 +447,20 @@ def test_stem_attention_and_clipping_in_one_step():
 
 # ---- refusals --------------------------------------------------------------------------------------
 
+@gpu
+def test_forward_mode_is_refused():
+    """A tangent would come back as none at all, which reads as a derivative of zero."""
+    from torch.autograd import forward_ad
+    tensors = [t.cuda() for t in _inputs(1, 5, 7, 2, 2, 16, F)[:4]]
+    with forward_ad.dual_level():
+        for i in range(4):
+            args = list(tensors)
+            args[i] = forward_ad.make_dual(args[i], args[i])
+            with pytest.raises(VitkError, match="forward-mode"):
+                vit_amd.diff_attention(*args)
+        assert vit_amd.diff_attention(*tensors).isfinite().all()
+
+
 def test_refusals_without_a_gpu():
     t = _inputs(1, 3, 4, 1, 1, 8, F)
     with pytest.raises(VitkError, match="no CPU fallback"):

@@ -243,6 +243,31 @@ def test_second_derivatives_are_refused():
 
 # ---- refusals --------------------------------------------------------------------------------------
 
+def test_forward_mode_tangents_are_found_without_a_gpu():
+    from torch.autograd import forward_ad
+    from vit_amd.functional import _needs_grad
+    x = torch.ones(2, 4)
+    with forward_ad.dual_level():
+        assert not _needs_grad(x, None)
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), pytest.raises(VitkError, match="forward-mode"):
+                _needs_grad(None, forward_ad.make_dual(x, x))
+    assert not _needs_grad(x, None) and _needs_grad(x.clone().requires_grad_(True))
+
+
+@gpu
+def test_forward_mode_is_refused():
+    """A tangent would come back as none at all, which reads as a derivative of zero."""
+    from torch.autograd import forward_ad
+    x = torch.ones(2, 3, 8, device="cuda")
+    w = torch.ones(8, device="cuda")
+    with forward_ad.dual_level():
+        for args in ((forward_ad.make_dual(x, x), 2, w, w), (x, 2, forward_ad.make_dual(w, w), w)):
+            with pytest.raises(VitkError, match="forward-mode"):
+                vit_amd.group_norm(*args)
+        assert vit_amd.group_norm(x, 2, w, w).isfinite().all()
+
+
 def test_refusals_without_a_gpu():
     with pytest.raises(VitkError, match="no CPU fallback"):
         vit_amd.group_norm(torch.randn(2, 5, 8), 2)

@@ -1,9 +1,11 @@
 """Operators beside the model's own layers, as functions of tensors with gradients.
 
 Each checks its arguments, launches the HIP kernels of libvitk on the current stream of its inputs' device, and raises
-VitkError for what they do not take; there is no CPU path.
+VitkError for what they do not take; there is no CPU path.  Gradients are those of reverse mode: an input with a forward-mode
+tangent is refused.
 """
 import torch
+from torch.autograd import forward_ad
 
 from . import ops
 from .autograd import DiffAttentionFn, GroupNormFn
@@ -18,6 +20,10 @@ def _on_device(x):
 
 
 def _needs_grad(*tensors):
+    if getattr(forward_ad, "_current_level", 0) >= 0:          # inside a dual level: tangents would be dropped
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise VitkError("these operators have no forward-mode derivative")
     if not torch.is_grad_enabled():
         return False
     for t in tensors:
