@@ -224,6 +224,24 @@ def test_runs_on_another_stream_and_in_a_captured_graph():
         assert all(torch.equal(p.grad, q.grad) for p, q in zip(params, eager))
 
 
+@gpu
+def test_a_graph_that_saved_a_gradient_notices_the_clipping():
+    a, b = _params([64, 7], [F, H])
+    saved = torch.ones(64, device="cuda", requires_grad=True)
+    for bound in (0.25 * _norm64([a, b]), 4.0 * _norm64([a, b])):              # scaled, and under the bound
+        versions = a.grad._version, b.grad._version
+        out = (saved * a.grad).sum()
+        vit_amd.clip_grad_norm_([a, b], bound)
+        assert a.grad._version > versions[0] and b.grad._version > versions[1]
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out.backward()
+    with torch.inference_mode():                                               # tensors without a counter
+        p = torch.zeros(5, device="cuda")
+        p.grad = torch.ones(5, device="cuda")
+        vit_amd.clip_grad_norm_([p], 1.0)
+        assert abs(float(p.grad.norm()) - 1.0) < 1e-5
+
+
 # ---- refusals that touch no GPU --------------------------------------------------------------------
 
 def _list(addr, size, kind):

@@ -90,10 +90,12 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
             if error_if_nonfinite and not math.isfinite(float(norm)):
                 raise _lib.VitkError(f"the gradients' norm is {float(norm)}, so they cannot be clipped (error_if_nonfinite)")
             _ops.grad_clip(grads, partials, max_norm, kind)
-            return norm
-        partials, _ = _ops.grad_norm(grads, kind, want_norm=False)
-        norm = torch.empty((), dtype=torch.float32, device=grads.device)
-        return _ops.grad_clip(grads, partials, max_norm, kind, norm)
+        else:
+            partials, _ = _ops.grad_norm(grads, kind, want_norm=False)
+            norm = torch.empty((), dtype=torch.float32, device=grads.device)
+            _ops.grad_clip(grads, partials, max_norm, kind, norm)
+    torch.autograd.graph.increment_version(tensors)      # for graphs that saved a gradient: autograd saw no write
+    return norm
 
 
 def pos_embed_scale(pos_embed, img_size, patch_size, mode='constant', order=1):
