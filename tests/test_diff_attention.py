@@ -299,6 +299,26 @@ def test_gradients_that_arrive_in_any_layout():
 
 
 @gpu
+@pytest.mark.parametrize("shared", [False, True])
+def test_lam_at_any_address(shared):
+    """A parameter that is a view into a flat buffer starts at any element."""
+    q, k, v, lam, do, _ = _inputs(2, 9, 33, 4, 2, 24, F, shared=shared)
+    def grads(x):                                                              # noqa: E306
+        out = vit_amd.diff_attention(q.cuda(), k.cuda(), v.cuda(), x)
+        return out.detach(), torch.autograd.grad(out, x, do.cuda())[0]
+    want = grads(lam.cuda().requires_grad_(True))
+    for at in (1, 2, 3):
+        flat = torch.zeros(lam.numel() + 4, device="cuda")
+        flat[at:at + lam.numel()] = lam.cuda().flatten()
+        x = flat[at:at + lam.numel()].view(lam.shape).requires_grad_(True)
+        assert x.data_ptr() % 16
+        assert all(torch.equal(a, b) for a, b in zip(grads(x), want))
+        with torch.no_grad():
+            out = vit_amd.diff_attention(q.cuda(), k.cuda(), v.cuda(), x)
+            assert torch.equal(out, vit_amd.diff_attention(q.cuda(), k.cuda(), v.cuda(), lam.cuda()))
+
+
+@gpu
 def test_broadcast_inputs():
     """Keys that all samples share by a stride of 0: their gradient is the sum over the samples, each rounded to the type."""
     q, k, v, lam, do, _ = _inputs(3, 20, 33, 2, 2, 32, F)

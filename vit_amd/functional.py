@@ -54,13 +54,15 @@ def diff_attention(q, k, v, lam, lambda_init=0.8, scale=None, key_lens=None, cau
     q [B, Nq, H, 2, d], k [B, Nk, K, 2, d], v [B, Nk, K, 2d] (bf16 or f32; d a multiple of 8 up to 64; H a multiple of K,
     query heads h * H / K ... share key head h), out [B, Nq, H, 2d].  Any strides in multiples of 16 bytes with a dense last
     dimension: the fused projection's qkv [3, B, H, N, 2d] goes in as `qkv[i].view(B, H, N, 2, d).permute(0, 2, 1, 3, 4)`.
-    lam f32 [4, H, d], or [4, d] for all heads; scale defaults to d ** -0.5 and must be positive.
+    q, k and v start at multiples of 16 bytes too.  lam f32 [4, H, d], or [4, d] for all heads, contiguous; scale defaults to d ** -0.5 and must be positive.
     key_lens (int32 [B] on the device) hides the keys from key_lens[b] on: they are never read and get no gradient.  causal:
     query t sees keys up to t + Nk - Nq (the last query all of them); keys and values that only some queries see have to be
     finite, since a probability of 0 still multiplies them.  A row without a visible key gives 0 and no gradient.
     Single query tokens against a long cache take a form that splits the keys.  Differentiable once in q, k, v and lam."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
+    if lam.data_ptr() % 16:                      # a view into something larger: the kernels load 16 bytes at a time
+        lam = lam.clone()
     with _on_device(q):
         if _needs_grad(q, k, v, lam):
             return DiffAttentionFn.apply(q, k, v, lam, lambda_init, scale, key_lens, causal)
