@@ -362,7 +362,8 @@ int vitk_diff_attention_backward(const void* q, const void* k, const void* v, co
 
 #define VITK_ACT_NONE 0
 #define VITK_ACT_RELU 1
-#define VITK_ACT_GELU_ERF 2  /* exact erf, as nn.GELU() */
+#define VITK_ACT_GELU_ERF 2  /* z Phi(z), as nn.GELU().  f32: Phi to a few f32 roundings, times z^2 in the negative tail; bf16: erf
+                                to 1.5e-7, which from z = -6 on (results under 1e-8) is more than bf16's own rounding */
 #define VITK_ACT_SILU 3
 
 /* f32 values of scratch for vitk_group_norm (backward = 0) or vitk_group_norm_backward; -1 for sizes it does not take. */

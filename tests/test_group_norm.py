@@ -134,6 +134,30 @@ def test_gradients_against_differences(act):
 
 
 @gpu
+@pytest.mark.parametrize("shape", [(1, 4, 2048), (3, 3000, 64)])                # one pass, two passes
+def test_gelu_in_f32_is_accurate_relative_to_small_results(shape):
+    """A weight of 0 makes z the bias: the activation and its derivative alone, over both tails."""
+    C = shape[-1]
+    z = torch.linspace(-12.0, 6.0, C, dtype=torch.float32)
+    Z = z.double()
+    cdf, den = 0.5 * torch.special.erfc(-Z / math.sqrt(2)), torch.exp(-Z * Z / 2) / math.sqrt(2 * math.pi)
+    x = _rnd(*shape, seed=8).float().cuda()
+    w, b = torch.zeros(C, device="cuda"), z.cuda().requires_grad_(True)
+    y = vit_amd.group_norm(x, 2, w, b, 1e-5, "gelu")
+    # erfc's argument is off by 2 eps (the constant, the product), which erfc turns into at most (z^2 + 1) times as much;
+    # erfc itself within 16 units in the last place (32 eps), two products
+    ecdf = (2 * (Z * Z + 1) + 32 + 4) * EPS32
+    err = ((y.detach().double().cpu() - Z * cdf).abs() / (Z * cdf).abs().clamp(min=1e-300)).amax(tuple(range(y.dim() - 1)))
+    assert (err <= ecdf)[Z != 0].all(), (err / ecdf).max()
+    dy = torch.zeros(shape, device="cuda")
+    dy[0, 1] = 1.0                                                              # one term of each channel's sum
+    slope = torch.autograd.grad(y, b, dy)[0].double().cpu()
+    # the exponent off by eps of z^2 / 2 twice, exp within 4 units, the constant and two products; their sum rounded once
+    bound = ecdf * cdf + (Z * Z + 8 + 4) * EPS32 * Z.abs() * den + EPS32 * (cdf + Z * den).abs()
+    assert ((slope - (cdf + Z * den)).abs() <= bound).all(), ((slope - (cdf + Z * den)).abs() / bound).max()
+
+
+@gpu
 def test_large_mean_against_small_deviation():
     # values of 1000 +- 1: sums of squares in f32 would leave no digit of the variance
     x = _rnd(2, 500, 32, seed=5, scale=1.0, shift=1000.0).float()

@@ -116,18 +116,54 @@ __device__ __forceinline__ float sigmoid(float z) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896340736f));
 }
 
-template <int ACT>
+// Phi(z) and exp(-z^2 / 2), for f32 results: gelu_erf's polynomial is off by up to 1.5e-7 of erf, 2e-7 of a result near 1 and
+// 0.2 % of one at z = -5 (-1.4e-6), below half a step of bf16 but not of f32.  Here erfc(|z| / sqrt 2) exp(z^2 / 2) = t P(t),
+// t = 1 / (1 + 0.3 |z|), with P of degree 9 fitted (least squares reweighted towards the largest relative error, |z| <= 14)
+// to 4e-9; the two halves then share the exponential, whose argument's rounding, z^2 / 2 steps, is most of the error.
+// 32 x 56 x 56 x 256 forward 47.5 us with gelu_erf, 51.7 with this, 68 with the library's erfcf.
+__device__ __forceinline__ float normal_cdf(float z, float& e) {
+    const float az = fabsf(z);
+    const float t = __builtin_amdgcn_rcpf(fmaf(az, 0.3f, 1.0f));
+    e = __builtin_amdgcn_exp2f(z * z * (-0.5f * 1.44269504088896340736f));
+    float q = -0.0412258916f;
+    q = fmaf(q, t, 0.224752828f);
+    q = fmaf(q, t, -0.456138015f);
+    q = fmaf(q, t, 0.383167386f);
+    q = fmaf(q, t, -0.158498019f);
+    q = fmaf(q, t, 0.192117453f);
+    q = fmaf(q, t, 0.156850532f);
+    q = fmaf(q, t, 0.220454782f);
+    q = fmaf(q, t, 0.239145666f);
+    q = fmaf(q, t, 0.239373267f);
+    q = 0.5f * q * t * e;
+    return z < 0.f ? q : 1.0f - q;
+}
+
+template <class T, int ACT>
 __device__ __forceinline__ float act_of(float z) {
     if constexpr (ACT == GN_RELU) return z > 0.f ? z : (z == z ? 0.f : z);      // a NaN stays one
-    if constexpr (ACT == GN_GELU) return gelu_erf(z);
+    if constexpr (ACT == GN_GELU) {
+        if constexpr (sizeof(T) == 4) {
+            float e;
+            return z * normal_cdf(z, e);
+        }
+        return gelu_erf(z);
+    }
     if constexpr (ACT == GN_SILU) return z * sigmoid(z);
     return z;
 }
 
-template <int ACT>
+template <class T, int ACT>
 __device__ __forceinline__ float dact_of(float z) {
     if constexpr (ACT == GN_RELU) return z > 0.f ? 1.f : 0.f;
-    if constexpr (ACT == GN_GELU) return dgelu_erf(z);
+    if constexpr (ACT == GN_GELU) {
+        if constexpr (sizeof(T) == 4) {
+            float e;
+            const float cdf = normal_cdf(z, e);
+            return fmaf(z * e, 0.39894228040143267794f, cdf);
+        }
+        return dgelu_erf(z);
+    }
     if constexpr (ACT == GN_SILU) {
         const float s = sigmoid(z);
         return s * fmaf(z, 1.0f - s, 1.0f);
@@ -358,7 +394,7 @@ __global__ __launch_bounds__(kT) void gn_apply(const T* __restrict__ x, const Mo
         float v[V];
         r.get(v);
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = act_of<ACT>(fmaf(v[j] - mu[j], a[j], sh[j]));
+        for (int j = 0; j < V; ++j) v[j] = act_of<T, ACT>(fmaf(v[j] - mu[j], a[j], sh[j]));
         Raw<T, V>::store(y + base + (int64_t)s * q.C, v);
     };
     int s = s0 + row;
@@ -412,7 +448,7 @@ __global__ __launch_bounds__(kT) void gn_bwd_sums(const T* __restrict__ x, const
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 const float h = (v[j] - mu[j]) * rs[j];
-                const float dz = ACT == GN_NONE ? g[j] : g[j] * dact_of<ACT>(fmaf(h, w[j], sh[j]));
+                const float dz = ACT == GN_NONE ? g[j] : g[j] * dact_of<T, ACT>(fmaf(h, w[j], sh[j]));
                 a1[j] += dz;
                 a2[j] = fmaf(dz, h, a2[j]);
             }
@@ -575,7 +611,7 @@ __global__ __launch_bounds__(kT) void gn_bwd_apply(const T* __restrict__ x, cons
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const float h = (v[j] - mu[j]) * rs[j];
-            const float dz = ACT == GN_NONE ? g[j] : g[j] * dact_of<ACT>(fmaf(h, w[j], sh[j]));
+            const float dz = ACT == GN_NONE ? g[j] : g[j] * dact_of<T, ACT>(fmaf(h, w[j], sh[j]));
             v[j] = rs[j] * (fmaf(dz, w[j], -m1[j]) - h * m2[j]);
         }
         Raw<T, V>::store(dx + base + (int64_t)s * q.C, v);
@@ -715,7 +751,7 @@ __global__ __launch_bounds__(NT) void gn_slab(const T* __restrict__ x, const flo
             float v[V];
             r[i].get(v);
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[j] = act_of<ACT>(fmaf(v[j] - mu, w[j], sh[j]));
+            for (int j = 0; j < V; ++j) v[j] = act_of<T, ACT>(fmaf(v[j] - mu, w[j], sh[j]));
             Raw<T, V>::store(y + base + (int64_t)(row + i * R) * q.C, v);
         }
 }
@@ -759,7 +795,7 @@ __global__ __launch_bounds__(NT) void gn_slab_bwd(const T* __restrict__ x, const
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 const float h = (v[j] - mu) * rs;
-                const float dz = ACT == GN_NONE ? g[j] : g[j] * dact_of<ACT>(fmaf(h, w[j], sh[j]));
+                const float dz = ACT == GN_NONE ? g[j] : g[j] * dact_of<T, ACT>(fmaf(h, w[j], sh[j]));
                 if constexpr (HOLD) held[i][j] = dz;
                 a1[j] += dz;
                 a2[j] = fmaf(dz, h, a2[j]);
@@ -829,7 +865,7 @@ __global__ __launch_bounds__(NT) void gn_slab_bwd(const T* __restrict__ x, const
                 const float h = (v[j] - mu) * rs;
                 float dz;
                 if constexpr (HOLD) dz = held[i][j];
-                else dz = ACT == GN_NONE ? g[j] : g[j] * dact_of<ACT>(fmaf(h, w[j], sh[j]));
+                else dz = ACT == GN_NONE ? g[j] : g[j] * dact_of<T, ACT>(fmaf(h, w[j], sh[j]));
                 v[j] = rs * (fmaf(dz, w[j], -m1) - h * m2);
             }
             Raw<T, V>::store(dx + base + (int64_t)(row + i * R) * q.C, v);

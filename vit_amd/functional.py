@@ -37,7 +37,8 @@ def group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, activation="none
     are, a feature map in torch's channels_last format as `x.permute(0, 2, 3, 1)`, which is a view.
 
     Statistics over all positions of channels / num_groups neighbouring channels per sample, in f32; weight and bias f32
-    [channels] or None; activation "none", "relu", "gelu" (exact erf) or "silu".  Returns x's shape and type.
+    [channels] or None; activation "none", "relu", "gelu" (nn.GELU()'s z Phi(z): Phi to f32's rounding in
+    f32, from an erf good to 1.5e-7 in bf16) or "silu".  Returns x's shape and type.
     Differentiable once in x, weight and bias."""
     with _on_device(x):
         if _needs_grad(x, weight, bias):
