@@ -385,7 +385,7 @@ int vitk_group_norm_backward(const void* x, const float* weight, const float* bi
 /* ---- global gradient norm and clipping -----------------------------------------------------------------
  * clip_grad_norm_ of the training step (main.py:221-223) over a list of n device tensors of any sizes: addr, size
  * (elements, 0 allowed) and dtype (VITK_F32 / VITK_BF16) are HOST arrays, read before the call returns.  Tensors are dense
- * and aligned to their type. */
+ * and aligned to their type, up to 16 TiB in all. */
 
 #define VITK_NORM_2 0        /* sqrt of the sum of squares, added in f64 */
 #define VITK_NORM_INF 1      /* largest magnitude */

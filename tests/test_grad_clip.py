@@ -283,3 +283,13 @@ def test_refusals_without_a_gpu():
     assert clip([4096], [4], [0], partials=None) == 1
     assert L.vitk_grad_norm(*_list([4096], [4], [0]), 0, None, ws, None, None) == 1
     assert L.vitk_grad_norm(None, None, None, 3, 0, part, ws, None, None) == 1
+
+
+def test_sizes_beyond_the_piece_counter_are_refused():
+    """A tensor of more than 2^31 pieces was never cut: the host went round for good."""
+    L = lib.load()
+    for size in ([(1 << 46) - 1], [(1 << 42) + 1], [1 << 42, 1], [1 << 41, 1 << 40, 1 << 40, 1]):
+        args = _list([4096 << i for i in range(len(size))], size, [lib.VITK_F32] * len(size))
+        assert L.vitk_grad_norm(*args, 0, 4096, 1 << 20, None, None) == lib.VITK_ERR_UNSUPPORTED, size
+        assert b"16 TiB" in L.vitk_last_error()
+        assert L.vitk_grad_clip(*args, 0, 4096, 1 << 20, 1.0, None, None) == lib.VITK_ERR_UNSUPPORTED

@@ -236,7 +236,8 @@ __global__ __launch_bounds__(kThreads) void grad_scale(GradTable t, const double
     }
 }
 
-// fills t with up to kTensors tensors from index i on; returns the next index
+// fills t with up to kTensors tensors from index i on; returns the next index.  The entry points take up to 16 TiB: at most
+// 2^30 pieces and one more at either end of a tensor.
 int fill(GradTable& t, const uint64_t* addr, const int64_t* size, const int* bf16, int n, int i) {
     t.n = 0;
     uint64_t pieces = 0;
@@ -244,7 +245,6 @@ int fill(GradTable& t, const uint64_t* addr, const int64_t* size, const int* bf1
         if (size[i] == 0) continue;
         const uint64_t bytes = (uint64_t)size[i] * (bf16[i] ? 2 : 4) + (addr[i] & 15);
         const uint64_t more = (bytes + kPieceBytes - 1) / kPieceBytes;
-        if (pieces + more > 0x7FFFFFFFull) break;
         t.addr[t.n] = addr[i];
         t.size[t.n] = (uint64_t)size[i] | (bf16[i] ? kTypeBit : 0);
         t.first[t.n] = (uint32_t)pieces;

@@ -740,7 +740,7 @@ static int grad_list(const char* name, const uint64_t* addr, const int64_t* size
     if (n < 0 || (n > 0 && (!addr || !size || !dtype))) return fail(VITK_ERR_INVALID, "%s: null pointer", name);
     if (norm_kind != VITK_NORM_2 && norm_kind != VITK_NORM_INF) return fail(VITK_ERR_INVALID, "%s: norm_kind=%d", name, norm_kind);
     bool ordered = true;
-    uint64_t end = 0;
+    uint64_t end = 0, bytes = 0;
     for (int i = 0; i < n; ++i) {
         if (dtype[i] != VITK_F32 && dtype[i] != VITK_BF16) return fail(VITK_ERR_UNSUPPORTED, "%s: dtype %d of tensor %d", name, dtype[i], i);
         if (size[i] < 0 || size[i] >= (int64_t)1 << 46) return fail(VITK_ERR_INVALID, "%s: size %lld of tensor %d", name, (long long)size[i], i);
@@ -749,6 +749,9 @@ static int grad_list(const char* name, const uint64_t* addr, const int64_t* size
         if (!addr[i] || addr[i] % es) return fail(VITK_ERR_INVALID, "%s: null or misaligned tensor %d", name, i);
         ordered &= addr[i] >= end;
         end = addr[i] + (uint64_t)size[i] * es;
+        bytes += (uint64_t)size[i] * es;
+        // a launch counts its pieces of 16 KiB in 31 bits
+        if (bytes > (uint64_t)1 << 44) return fail(VITK_ERR_UNSUPPORTED, "%s: tensors of more than 16 TiB together", name);
     }
     if (!written || ordered) return VITK_OK;
     // Tensors that share memory would be scaled by two workgroups at once.
