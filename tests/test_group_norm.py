@@ -112,6 +112,22 @@ def test_gradients(shape, G, dtype, act):
         assert ((g - want).abs() <= bound).all(), ((g - want).abs() / bound).max()
 
 
+# The one-pass form's other cuts.  3136 pixels: 1,024 threads and rows of 64 bytes in the forward, the two of a 128-byte line
+# on one XCD where batch * slabs is a multiple of 16 (f32: 4 x 4, bf16: 4 x 2), the backward in two passes.  1536 pixels:
+# 512 threads and paired rows of 64 bytes in both directions (8 x 4, 8 x 2), 2000 with samples that are no multiple of the
+# pairs (3 x 4, 3 x 2: unpaired), 1600 with one pair a sample (f32: 16 x 2) and with none (bf16: 16 x 1).
+CUTS = [((4, 56, 56, 64), 8), ((8, 32, 48, 64), 8), ((3, 2000, 64), 8), ((16, 1600, 32), 4)]
+
+
+@gpu
+@pytest.mark.parametrize("act", ["none", "gelu"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape,G", CUTS)
+def test_cuts_of_the_one_pass_form(shape, G, dtype, act):
+    test_forward(shape, G, dtype, act)
+    test_gradients(shape, G, dtype, act)
+
+
 @gpu
 @pytest.mark.parametrize("act", ACTS)
 def test_gradients_against_differences(act):
