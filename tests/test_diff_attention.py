@@ -299,6 +299,33 @@ def test_gradients_that_arrive_in_any_layout():
 
 
 @gpu
+def test_learned_weight_collects_no_one_sided_error():
+    """w's gradient sums -P_2 dA over 73,856 rows whose own terms cancel.  The matrix pipe's products lean to one side by some
+    1e-9, which adds up to 7e-5 in the sum where every row leans alike; the backward negates every other row."""
+    B, N, H, d, w0 = 16, 577, 8, 48, 0.6
+    rows = B * N * H
+    errors = []
+    for seed in (20, 21, 22, 23):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")          # noqa: E731
+        q, k, v, do = (rnd(*s).to(H16) for s in ((B, N, H, 2, d), (B, N, H, 2, d), (B, N, H, 2 * d), (B, N, H, 2 * d)))
+        lam = (rnd(4, d) * 0.1).requires_grad_(True)
+        dlam = torch.autograd.grad(vit_amd.diff_attention(q, k, v, lam, w0), lam, do)[0].double()
+        dw = 0.0
+        for b in range(B):
+            Q, K = (t[b, :, :, 1].double().permute(1, 0, 2) for t in (q, k))
+            p = torch.softmax(Q @ K.transpose(1, 2).contiguous() * d ** -0.5, -1)
+            dw -= float(((p @ v[b].double().permute(1, 0, 2)) * do[b].double().permute(1, 0, 2)).sum())
+        L = lam.detach().double()
+        e1, e2 = (L[0] * L[1]).sum().exp(), (L[2] * L[3]).sum().exp()
+        unit = torch.stack([e1 * L[1], e1 * L[0], -e2 * L[3], -e2 * L[2]])     # dlam is dw times this
+        errors.append(float((dlam * unit).sum() / (unit * unit).sum()) - dw)
+    # A row's own f32 roundings (16 terms to a sum of size 0.7, its denominator) are off by 1e-7 or so to either side: 1e-7
+    # sqrt(rows) = 2.7e-5 for one seed, half of that for the mean of four; the lean's 7.4e-5 stays in the mean.
+    assert abs(sum(errors) / len(errors)) <= 0.5e-9 * rows, errors
+
+
+@gpu
 @pytest.mark.parametrize("shared", [False, True])
 def test_lam_at_any_address(shared):
     """A parameter that is a view into a flat buffer starts at any element."""
