@@ -85,7 +85,7 @@ __device__ __forceinline__ typename Op<T>::Chunk chunk_at(const char* tile, int 
 
 // Transposed operand: element j of a lane is tile[row0 + 8 (j >> 2) + 4 (lane >> 5) + (j & 3)][col0 + (lane & 31)], j < 8:
 // the A operand of (tile slice)^T x B where B is an accumulator's elements 8 s .. 8 s + 7 (rows 16 s + ...).
-// row0 is a multiple of 16, col0 of 32.
+// row0 is a multiple of 16, col0 of 8.
 template <class T, int RB>
 struct Trans;
 template <int RB>
@@ -121,7 +121,9 @@ struct Slice;
 template <>
 struct Slice<bf16_t> {
     bf16x8 v;
-    // the rounding to bf16 of a probability or of its gradient: up to 2^-8 of it, of terms that are then added in f32
+    // the rounding to bf16 of a probability or of its gradient: up to 2^-8 of it, of terms that are then added in f32.  The two
+    // maps' probabilities are rounded apart, also for dV, where one rounding of P_1 - w P_2 would do: their products lie in two
+    // waves.  The matrix pipe multiplies bf16 at 8 times the rate of f32.
     __device__ __forceinline__ void take(const f32x16& s, int st) {
         const u32x4 pk = {pack_bf16(s[8 * st], s[8 * st + 1]), pack_bf16(s[8 * st + 2], s[8 * st + 3]),
                           pack_bf16(s[8 * st + 4], s[8 * st + 5]), pack_bf16(s[8 * st + 6], s[8 * st + 7])};

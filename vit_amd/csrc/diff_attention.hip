@@ -13,8 +13,9 @@
 // Rows of a (sample, key head) are the tokens of all its query heads (diff_attention.h).  Two forms:
 //   many rows:  the pairs of a workgroup take 32 rows each and walk all their keys in chunks of 32 through two LDS buffers,
 //               the next chunk on its way to registers while the waves work on the one before;
-//   few rows:   the pairs take the same 32 rows and every fourth block of 32 keys, and the keys are split over so many
-//               workgroups that the chip is full; the pairs' results are joined in LDS, the workgroups' by a second kernel.
+//   few rows:   the pairs (four, in f32 from size 33 on two) take the same 32 rows and a block of 32 keys in turn, and the keys
+//               are split over so many workgroups that the chip is full; the pairs' results are joined in LDS, the workgroups'
+//               by a second kernel.
 #include <type_traits>
 
 #include "diff_attention.h"
@@ -41,7 +42,7 @@ __device__ __forceinline__ int joined(int row, int map, int col) {
     return row * (2 * DV) + ((c ^ (row & 15)) << 2);
 }
 
-// OCC: waves to a SIMD that the registers have to allow.  TRAIN: the sums for the backward are written too, and the
+// OCC: waves to a SIMD that the registers have to allow (at size 64 the form for many rows without TRAIN spills 5).  TRAIN: the sums for the backward are written too, and the
 // denominators are added from the probabilities before their rounding to bf16 (16 additions a block and lane); without it
 // the matrix pipe adds the rounded ones, which are what the product with V uses, beside that product.
 template <class T, int DP, int NG, bool KEYS, bool TRAIN, int OCC>

@@ -13,6 +13,7 @@
 // As in the forward a pair of waves shares 32 rows or keys, one map each: dA is computed by both, everything else once, and
 // the registers that leaves allow two waves and more to a SIMD, which hide each other's waiting (one wave with both maps
 // took 2.3 times as long at 577 tokens of head size 48, most of it waiting).
+// At head size 64 dK / dV fills its 256 registers and spills 7 (1 where no heads share keys).
 // Bound by the matrix pipe, the exponentials' arithmetic and the LDS reads that feed the products, which overlap in part: at
 // 4096 causal tokens (batch 2, 8 heads of 64, 4 key heads) dQ takes 190 us and 145 of them without its staging, 165 without
 // its exponentials, 115 with the products and the transposed reads alone; the products at the matrix pipe's rate are 65.
@@ -105,7 +106,9 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_q(DiffArgs a, DiffGrad
             const int c = 2 * t + hh;
             qf[t] = chunk_or_zero<T>(qg, c, c < dc);
         }
-        // dO . O by the first map's wave, dO . O_2 by the second's, all loads at once
+        // dO . O by the first map's wave, dO . O_2 by the second's, all loads at once.  In bf16 both carry the rounding of O and
+        // O_2 to their type (they are the forward's outputs, kept as such for half the bytes), so D_m is off by up to 2^-8 of a
+        // term; dw is not made of it.
         const int64_t orow = (((int64_t)b * a.nq + place.tok) * a.heads + place.head) * 2 * a.d;
         const T* og = reinterpret_cast<const T*>(map ? g.out2 : g.out) + orow;
         Chunk o[2 * KT];
@@ -438,7 +441,7 @@ __global__ __launch_bounds__(NP * 128, OCC) void diff_bwd_kv(DiffArgs a, DiffGra
         if (more) put(k ^ 1, c + 1);
         __syncthreads();
     };
-    if constexpr (sizeof(T) == 4) {                                   // twice the body costs f32 more than the addresses: 97 / 83 us
+    if constexpr (sizeof(T) == 4) {                                   // twice the body costs f32 more than the addresses: 138 / 134 us, 167 / 159
         for (int c = first; c < c1; ++c) chunk(c, (c - first) & 1);
     } else {
         for (int c = first; c < c1; c += 2) {
@@ -560,7 +563,7 @@ hipError_t launch(const DiffArgs& a, const DiffGrads& g, float* ws, hipStream_t 
     // blocks of 32 that are staged between two barriers, measured with one / two.  dQ at 577 tokens (batch 16, 8 heads of 48)
     // 70 / 81 us, at 197 (64, 12 of 32) 55 / 59: the smaller buffers leave room for a third workgroup on a CU;  at 4096
     // causal ones (2, 8 heads of 64, 4 key heads) 195 / 192, at 1500 (2, 16 of 64) 119 / 115: there the registers do not.
-    // dK and dV 100 / 102, 75 / -, 280 / 319;  in f32 at 257 tokens (4, 16 heads of 40) 93 / 85.
+    // dK and dV 100 / 102, 75 / -, 280 / 319;  in f32 at 257 tokens (4, 16 heads of 40) 140 / 134, at 577 (2, 12 of 64) 175 / 159.
     constexpr int NBQ = sizeof(T) == 2 && DP == 64 ? 2 : 1, NBK = sizeof(T) == 4 ? 2 : 1;
     const int64_t bks = (int64_t)a.batch * a.kv_heads;
     const int64_t qt = row_tiles(a, kRowPairs), kt = key_tiles(a, NP), keys = (int64_t)a.batch * a.kv_heads * a.nk;

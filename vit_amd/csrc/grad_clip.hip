@@ -6,7 +6,7 @@
 //
 // Bound by HBM: the norm reads every gradient once, the scaling reads and writes it once more; nothing is computed to
 // speak of.  One launch covers up to kTensors tensors (their addresses and sizes travel as kernel arguments: nothing has
-// to be copied to the device first), whatever their sizes: the list is cut into pieces of 64 KiB, a fixed grid of
+// to be copied to the device first), whatever their sizes: the list is cut into pieces of 16 KiB, a fixed grid of
 // workgroups walks the pieces.  Squares are added in f64: every f32 value has a square that f64 holds, so neither large
 // nor tiny gradients lose their norm, and the matrix-free f64 rate (one multiply-add per element) is far above what
 // memory delivers.  Every workgroup leaves one partial sum; the scaling kernel adds them itself, every workgroup the same

@@ -59,7 +59,12 @@ def diff_attention(q, k, v, lam, lambda_init=0.8, scale=None, key_lens=None, cau
     key_lens (int32 [B] on the device) hides the keys from key_lens[b] on: they are never read and get no gradient.  causal:
     query t sees keys up to t + Nk - Nq (the last query all of them); keys and values that only some queries see have to be
     finite, since a probability of 0 still multiplies them.  A row without a visible key gives 0 and no gradient.
-    Single query tokens against a long cache take a form that splits the keys.  Differentiable once in q, k, v and lam."""
+    Single query tokens against a long cache take a form that splits the keys.  Differentiable once in q, k, v and lam.
+
+    Scores, softmax statistics and sums are f32; in bf16 the probabilities are rounded to bf16 for the product with v.  Without
+    gradients the denominators add those rounded values, with gradients the f32 ones, so the two may differ by the output's
+    rounding.  A scaled score's own f32 rounding, 2^-24 of it, enters the exponent: probabilities lose accuracy from some
+    thousands on, gradients have none left from 2^22 on, and scores of 2^30 and more may give NaN."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
     if lam.data_ptr() % 16:                      # a view into something larger: the kernels load 16 bytes at a time

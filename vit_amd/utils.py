@@ -57,7 +57,8 @@ def _norm_kind(norm_type):
 
 def grad_norm(tensors, norm_type=2.0):
     """Norm of all the tensors' values taken together (sqrt of the sum of squares, or the largest magnitude) as an f32
-    scalar on their device; bf16 and f32 tensors of any sizes, dense, on one device.  NaN if any value is one."""
+    scalar on their device; bf16 and f32 tensors of any sizes, dense, on one device.  NaN if any value is one.  The result has no
+    gradient."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     kind = _norm_kind(norm_type)
     if not tensors:
